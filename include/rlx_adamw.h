@@ -1,5 +1,6 @@
 /*
- * rlx_adamw.h — C ABI of the MI355X (gfx950) AdamW + gradient-norm/clip library.
+ * rlx_adamw.h — C ABI of the MI355X (gfx950) AdamW + gradient-norm/clip library, and of the loss
+ * operators that produce the gradients it consumes.
  *
  * Plain pointers and sizes only; every pointer named "device" is HIP device memory,
  * `stream` is a hipStream_t passed as void* (NULL = the default stream).  All work is
@@ -83,7 +84,7 @@ int rlx_clear(void* dst, int64_t nbytes, void* stream);
  * Multi-tensor plan: a whole model's tensors in one launch.
  * ---------------------------------------------------------------------------------- */
 
-enum { RLX_DTYPE_F16 = 0, RLX_DTYPE_F32 = 1 };
+enum { RLX_DTYPE_F16 = 0, RLX_DTYPE_F32 = 1, RLX_DTYPE_BF16 = 2 /* logits of the loss operators only */ };
 
 enum {
     RLX_TENSOR_NO_DECAY  = 1,   /* weight_decay is 0 for this tensor (embedding and norm
@@ -260,6 +261,159 @@ int rlx_plan_schedule_upload(rlx_plan* plan, const rlx_step_params* steps, int64
 int rlx_plan_adamw_scheduled(rlx_plan* plan, int step_flags, void* stream);
 int rlx_plan_schedule_position(rlx_plan* plan, int64_t* steps_taken, int64_t* n_steps, void* stream);
 int rlx_plan_schedule_overrun(rlx_plan* plan, int64_t* overrun, void* stream);
+
+/* ------------------------------------------------------------------------------------
+ * Loss operators: from logits to log-probabilities, from those to a policy or preference loss
+ * and its gradient, and back to the gradient of the logits.  They stand where the reference's
+ * trainers launch their loss kernels, before rlx_scale_f32 and the backward pass.
+ *
+ * Common to all of them:
+ *  - Everything is stream-ordered and asynchronous; nothing is allocated, no value is added by an
+ *    atomic, and the results are the same bits on every run.  The device of the pointers must be
+ *    the current one.
+ *  - Scratch memory is the caller's: `workspace` (device, 16-byte aligned, contents arbitrary) of
+ *    at least the bytes that the operator's _workspace function returns.  Two calls that may overlap
+ *    (two streams, two recorded graphs) need a workspace each; calls on one stream may share one.
+ *  - Softmax statistics and sums are FP32 per lane, sums over tokens FP64; a result is rounded
+ *    once, to its own type.
+ *  - A row (token) that is masked out, or whose target is negative, is IGNORED: its logits, log
+ *    probabilities and so on are not used whatever they hold (NaN included), its outputs are 0 and its
+ *    row of gradients is 0.  A target >= vocab makes the row's outputs NaN; nothing outside the row is read.
+ * ---------------------------------------------------------------------------------- */
+
+enum { RLX_INDEX_I32 = 0, RLX_INDEX_I64 = 1 };
+
+/*
+ * Rows of logits, or of their gradient: row r lies at
+ *     data + (r / group_rows) * group_stride + (r % group_rows) * row_stride       (elements),
+ * so that logits of [batch, length, vocab] without their last position need no copy (group_rows = length - 1,
+ * group_stride = length * vocab).  group_rows = 0: all rows in one group.  Elements of a row are
+ * consecutive; any start that is aligned to the element is allowed; rows must not overlap.
+ */
+typedef struct rlx_logits {
+    void*       data;          /* device */
+    int64_t     rows, vocab;   /* rows < 2^31; 1 <= vocab <= 2^30 */
+    int64_t     row_stride;
+    int64_t     group_rows, group_stride;
+    int32_t     dtype;         /* RLX_DTYPE_F16, _F32 or _BF16 */
+    int32_t     reserved;      /* 0 */
+} rlx_logits;
+
+/*
+ * Log-probability of one target per row, with z = logits / temperature:
+ *     lse[r] = log sum_j exp(z[r][j]),  logp[r] = z[r][targets[r]] - lse[r],
+ *     entropy[r] = lse[r] - sum_j p[r][j] z[r][j]      (entropy may be NULL).
+ * Logits of -inf, or of the type's lowest value beside ordinary ones, are vocabulary that is masked out (p = 0).  A
+ * row of the lowest value only is uniform; a row of -inf only, or one that holds NaN or +inf, gives NaN.
+ * Replaces the forward half of the reference's log-softmax gather (src/model/qwen3.cu:91).
+ */
+int64_t rlx_token_logprob_workspace(const rlx_logits* x);
+int rlx_token_logprob(const rlx_logits* x, const void* targets, int index_type, float temperature, float* logp,
+                      float* lse, float* entropy, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Gradient of the logits from those of logp and entropy (dentropy and entropy both NULL, or neither), with the lse
+ * and entropy that rlx_token_logprob gave for the same logits and temperature:
+ *     dx[r][j] = (dlogp[r] ([j = target] - p[r][j]) - dentropy[r] p[r][j] (log p[r][j] + entropy[r])) / temperature,
+ * p = exp(z - lse).  A row whose two gradients are 0 gets zeros without being read.  dx has x's rows, vocab and dtype;
+ * it may be x itself (same data and strides) but may not overlap it otherwise.
+ * Replaces the backward half of the log-softmax gather (src/model/qwen3.cu:170).
+ */
+int rlx_token_logprob_backward(const rlx_logits* x, const void* targets, int index_type, float temperature,
+                               const float* lse, const float* entropy, const float* dlogp, const float* dentropy,
+                               const rlx_logits* dx, void* stream);
+
+/* Weights w of the tokens in a loss (m = tokens that count: not masked, target not negative): */
+enum {
+    RLX_LOSS_SEQUENCE_MEAN = 0,   /* norm / (n_seqs * m of the token's sequence): mean over sequences of means */
+    RLX_LOSS_TOKEN_MEAN = 1,      /* norm / (m of the whole batch) */
+    RLX_LOSS_SUM = 2              /* norm */
+};
+
+/*
+ * Clipped policy loss with a KL term.  With rho = exp(logp - old_logp), A the advantage and
+ * d = ref_logp - logp,
+ *     loss = sum_t w_t (-min(rho A, clip(rho, 1 - clip_low, 1 + clip_high) A)
+ *                       + kl_coef (exp(d) - d - 1) - entropy_coef entropy),
+ *     dlogp[t] = grad_scale w_t (-A rho [not clipped] + kl_coef (1 - exp(d))),
+ *     dentropy[t] = -grad_scale w_t entropy_coef.
+ * "Clipped" is logp - old_logp > log(1 + clip_high) for A >= 0, < log(1 - clip_low) for A < 0, decided in FP64.
+ * old_logp NULL: rho is 1 (logp is its own old value).  ref_logp NULL: no KL term.
+ * Sequence s is the tokens [cu_seqlens[s], cu_seqlens[s + 1]) of the packed arrays; cu_seqlens NULL: n_seqs
+ * sequences of tokens / n_seqs tokens each (a padded batch).  Sequences may be empty.  Tokens in
+ * front of the first and behind the last sequence are no part of the loss: they are ignored like masked ones (their
+ * gradients are written as 0, so that a gradient buffer never keeps what it held before).
+ * A batch in which no token counts has loss 0 and gradients 0.  Offsets outside [0, tokens] or not ascending give
+ * unspecified results, but no access outside the arrays.
+ * Replaces grpo_loss_kernel (include/training/GRPO_trainer.h, launched in grpo_training_step :452-517).
+ */
+typedef struct rlx_policy_args {
+    const float*    old_logp;       /* device [tokens] or NULL */
+    const float*    ref_logp;       /* device [tokens] or NULL */
+    const float*    advantages;     /* device [tokens] if advantage_per_token, else [n_seqs] */
+    const float*    entropy;        /* device [tokens] or NULL; rlx_policy_loss only (the other form computes it) */
+    const uint8_t*  mask;           /* device [tokens], 0 = ignored; NULL: every token counts */
+    const int32_t*  cu_seqlens;     /* device [n_seqs + 1], ascending, or NULL */
+    int64_t         n_seqs;         /* < 2^31 */
+    float           clip_low, clip_high;     /* 0 <= clip_low <= 1, clip_high >= 0 */
+    float           kl_coef, entropy_coef;
+    float           norm;           /* factor of the weights (1 for the plain means) */
+    float           grad_scale;     /* factor of the gradients only (keeps 16-bit gradients in range) */
+    int32_t         reduction;      /* RLX_LOSS_* */
+    int32_t         advantage_per_token;
+} rlx_policy_args;
+
+typedef struct rlx_policy_stats {   /* device, 8-byte aligned */
+    float   loss;                   /* policy + kl_coef kl - entropy_coef entropy */
+    float   policy, kl, entropy;    /* the terms, weighted with w */
+    float   clip_fraction, ratio;   /* share of clipped tokens and mean rho over the tokens that count */
+    int64_t tokens;                 /* how many count */
+} rlx_policy_stats;
+
+int64_t rlx_policy_loss_workspace(int64_t tokens, int64_t n_seqs);
+int rlx_policy_loss(const float* logp, int64_t tokens, const rlx_policy_args* args, float* dlogp, float* dentropy,
+                    rlx_policy_stats* stats, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * The same loss from the logits themselves: log-probabilities (written to logp, and entropies to entropy unless it is
+ * NULL), loss and the gradient of the logits in one call that reads the logits once where a row fits the registers of a
+ * compute unit.  x->rows is the number of tokens; args->entropy must be NULL.  dx as in rlx_token_logprob_backward.
+ */
+int64_t rlx_policy_loss_logits_workspace(const rlx_logits* x, int64_t n_seqs);
+int rlx_policy_loss_logits(const rlx_logits* x, const void* targets, int index_type, float temperature,
+                           const rlx_policy_args* args, float* logp, float* entropy, const rlx_logits* dx,
+                           rlx_policy_stats* stats, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Preference loss over pairs of sequences.  Sequence s of the first n_pairs is the chosen answer, sequence
+ * n_pairs + s the rejected answer of pair s.  With the reward r = beta * sum over the tokens that count of
+ * (logp - ref_logp) (their mean if `average`; ref_logp NULL counts as 0; 0 if none counts) and
+ * x = r_chosen - r_rejected - margin,
+ *     loss = mean over pairs of -(1 - label_smoothing) log sigmoid(x) - label_smoothing log sigmoid(-x),
+ *     dlogp[t] = grad_scale * d loss / d logp[t].
+ * Sequences, masks and tokens outside the sequences as in rlx_policy_loss (2 n_pairs sequences).  rewards
+ * (device [2 n_pairs]) may be NULL.  The reference has no counterpart.
+ */
+typedef struct rlx_preference_args {
+    const float*    ref_logp;       /* device [tokens] or NULL */
+    const uint8_t*  mask;           /* device [tokens] or NULL */
+    const int32_t*  cu_seqlens;     /* device [2 n_pairs + 1] or NULL */
+    int64_t         n_pairs;        /* < 2^30 */
+    float           beta, label_smoothing /* 0 .. 1 */, margin, grad_scale;
+    int32_t         average;
+    int32_t         reserved;       /* 0 */
+} rlx_preference_args;
+
+typedef struct rlx_preference_stats {   /* device, 4-byte aligned */
+    float loss, accuracy;               /* accuracy: share of pairs with r_chosen > r_rejected */
+    float reward_margin;                /* mean of r_chosen - r_rejected */
+    float chosen_reward, rejected_reward;
+} rlx_preference_stats;
+
+int64_t rlx_preference_loss_workspace(int64_t tokens, int64_t n_pairs);
+int rlx_preference_loss(const float* logp, int64_t tokens, const rlx_preference_args* args, float* dlogp,
+                        float* rewards, rlx_preference_stats* stats, void* workspace, int64_t workspace_bytes,
+                        void* stream);
 
 /* ------------------------------------------------------------------------------------
  * Launch tuning (process-wide; for measurement).  Unknown keys return RLX_ERR_INVALID_ARG.

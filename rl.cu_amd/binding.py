@@ -12,7 +12,9 @@ LIB_PATH = os.path.join(HERE, "librlx_adamw.so")
 
 (OK, ERR_INVALID_ARG, ERR_MISALIGNED, ERR_BAD_HYPER, ERR_HIP, ERR_NO_DEVICE, ERR_TOO_LARGE, ERR_NO_MEMORY,
  ERR_WRONG_DEVICE) = range(9)
-DTYPE_F16, DTYPE_F32 = 0, 1
+DTYPE_F16, DTYPE_F32, DTYPE_BF16 = 0, 1, 2
+INDEX_I32, INDEX_I64 = 0, 1
+LOSS_SEQUENCE_MEAN, LOSS_TOKEN_MEAN, LOSS_SUM = 0, 1, 2
 TENSOR_NO_DECAY, TENSOR_GRAD_ONLY, TENSOR_FROZEN = 1, 2, 4
 CLIP_NONE, CLIP_FUSED, STEP_ZERO_GRADS = 0, 1, 2
 FILL_ABS = 1
@@ -32,6 +34,25 @@ class TensorDesc(C.Structure):
 class StepParams(C.Structure):
     _fields_ = [("lr", C.c_float), ("beta1", C.c_float), ("beta2", C.c_float), ("eps", C.c_float),
                 ("weight_decay", C.c_float), ("bias_correction1", C.c_float), ("bias_correction2", C.c_float)]
+
+
+class Logits(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("rows", C.c_int64), ("vocab", C.c_int64), ("row_stride", C.c_int64),
+                ("group_rows", C.c_int64), ("group_stride", C.c_int64), ("dtype", C.c_int32), ("reserved", C.c_int32)]
+
+
+class PolicyArgs(C.Structure):
+    _fields_ = [("old_logp", C.c_void_p), ("ref_logp", C.c_void_p), ("advantages", C.c_void_p),
+                ("entropy", C.c_void_p), ("mask", C.c_void_p), ("cu_seqlens", C.c_void_p), ("n_seqs", C.c_int64),
+                ("clip_low", C.c_float), ("clip_high", C.c_float), ("kl_coef", C.c_float),
+                ("entropy_coef", C.c_float), ("norm", C.c_float), ("grad_scale", C.c_float),
+                ("reduction", C.c_int32), ("advantage_per_token", C.c_int32)]
+
+
+class PreferenceArgs(C.Structure):
+    _fields_ = [("ref_logp", C.c_void_p), ("mask", C.c_void_p), ("cu_seqlens", C.c_void_p), ("n_pairs", C.c_int64),
+                ("beta", C.c_float), ("label_smoothing", C.c_float), ("margin", C.c_float), ("grad_scale", C.c_float),
+                ("average", C.c_int32), ("reserved", C.c_int32)]
 
 
 _F, _I64, _VP, _U64, _U32, _INT = C.c_float, C.c_int64, C.c_void_p, C.c_uint64, C.c_uint32, C.c_int
@@ -68,6 +89,17 @@ SIGNATURES = {
     "rlx_update_variant_name": ([_I64], C.c_char_p),
     "rlx_set_tuning": ([C.c_char_p, _I64], _INT),
     "rlx_get_tuning": ([C.c_char_p], _I64),
+    "rlx_token_logprob_workspace": ([C.POINTER(Logits)], _I64),
+    "rlx_token_logprob": ([C.POINTER(Logits), _VP, _INT, _F, _VP, _VP, _VP, _VP, _I64, _VP], _INT),
+    "rlx_token_logprob_backward": ([C.POINTER(Logits), _VP, _INT, _F, _VP, _VP, _VP, _VP, C.POINTER(Logits), _VP],
+                                   _INT),
+    "rlx_policy_loss_workspace": ([_I64, _I64], _I64),
+    "rlx_policy_loss": ([_VP, _I64, C.POINTER(PolicyArgs), _VP, _VP, _VP, _VP, _I64, _VP], _INT),
+    "rlx_policy_loss_logits_workspace": ([C.POINTER(Logits), _I64], _I64),
+    "rlx_policy_loss_logits": ([C.POINTER(Logits), _VP, _INT, _F, C.POINTER(PolicyArgs), _VP, _VP, C.POINTER(Logits),
+                                _VP, _VP, _I64, _VP], _INT),
+    "rlx_preference_loss_workspace": ([_I64, _I64], _I64),
+    "rlx_preference_loss": ([_VP, _I64, C.POINTER(PreferenceArgs), _VP, _VP, _VP, _VP, _I64, _VP], _INT),
     "rlx_fill_f16": ([_VP, _I64, _U64, _I64, _F, _F, _U32, _I64, _U32, _VP], _INT),
     "rlx_fill_f32": ([_VP, _I64, _U64, _I64, _F, _F, _U32, _I64, _U32, _VP], _INT),
 }
@@ -75,7 +107,7 @@ SIGNATURES = {
 _lib = None
 
 
-ABI_VERSION = 109        # rlx_version() of the library this binding was written against
+ABI_VERSION = 110        # rlx_version() of the library this binding was written against
 
 
 def load():

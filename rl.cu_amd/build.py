@@ -6,7 +6,7 @@ import subprocess
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
-SRC = os.path.join(HERE, "csrc", "rlx_adamw.hip")
+SOURCES = [os.path.join(HERE, "csrc", f) for f in ("rlx_adamw.hip", "rlx_losses.hip")]
 OUT = os.path.join(HERE, "librlx_adamw.so")
 
 # -ffp-contract=off: every FP32 operation of the update rounds once, as in the CPU restatement
@@ -19,14 +19,14 @@ HIPCC_FLAGS = [
 ]
 
 
-HEADER = os.path.join(ROOT, "include", "rlx_adamw.h")
+HEADERS = [os.path.join(ROOT, "include", "rlx_adamw.h"), os.path.join(HERE, "csrc", "rlx_internal.h")]
 STAMP = OUT + ".srchash"
 
 
 def source_hash():
-    """Hash of everything the library is built from (kernel source, C header, compiler flags)."""
+    """Hash of everything the library is built from (kernel sources, headers, compiler flags)."""
     h = hashlib.sha256()
-    for path in (SRC, HEADER):
+    for path in SOURCES + HEADERS:
         with open(path, "rb") as f:
             h.update(f.read())
     h.update(" ".join(HIPCC_FLAGS).encode())
@@ -59,7 +59,7 @@ def hipcc_path():
 
 def build_library(verbose=False):
     """Compiles the library every time it is called; returns the path of the .so."""
-    cmd = [hipcc_path()] + HIPCC_FLAGS + ["-I", os.path.join(ROOT, "include"), "-o", OUT + ".tmp", SRC]
+    cmd = [hipcc_path()] + HIPCC_FLAGS + ["-I", os.path.join(ROOT, "include"), "-o", OUT + ".tmp"] + SOURCES
     res = subprocess.run(cmd, capture_output=True, text=True)
     noise = "packed-fp32-ops"
     err = "\n".join(l for l in res.stderr.splitlines() if noise not in l)

@@ -39,6 +39,7 @@
 #include <vector>
 
 #include "rlx_adamw.h"
+#include "rlx_internal.h"
 
 // Intermediate sums of rlx_grad_norm_static, the entry point for callers that cannot allocate: part of the
 // library's device image (2.1 MiB on every GPU the library runs on, until the process ends).  Layout, in
@@ -133,10 +134,6 @@ __device__ __forceinline__ float h2f(uint32_t bits16) {
 __device__ __forceinline__ uint32_t f2h(float x) {
     return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)x);     // round to nearest even
 }
-
-// Every buffer handed to this library is HIP device memory, so all accesses go through
-// global-address-space pointers (global_load/global_store rather than flat).
-#define RLX_GLOBAL __attribute__((address_space(1)))
 
 template <bool NT, typename T>
 __device__ __forceinline__ T ldg(const T* p) {
@@ -1251,16 +1248,7 @@ constexpr int kMaxDevices = 64;
 std::mutex g_scratch_mutex;
 double* g_scratch_ptr[kMaxDevices];      // device address of `scratch` on each device; null until first used there
 
-int hip_fail(hipError_t e, const char* what) {
-    snprintf(g_hip_error, sizeof(g_hip_error), "%s: %s", what, hipGetErrorString(e));
-    return RLX_ERR_HIP;
-}
-
-#define RLX_HIP(call)                                        \
-    do {                                                     \
-        hipError_t e_ = (call);                              \
-        if (e_ != hipSuccess) return hip_fail(e_, #call);    \
-    } while (0)
+int hip_fail(hipError_t e, const char* what) { return rlx_internal_hip_fail(e, what); }
 
 // Process-wide launch tuning (for measurement).  Atomic, so that a thread that changes a key while another
 // launches is a defined race: every launch reads each key once and uses one consistent choice.
@@ -1286,7 +1274,7 @@ constexpr int kNumConvertVariants = 4;
 constexpr int64_t kMaxTilesPerLaunch = 1 << 23;   // workgroups per launch; times 256 lanes stays below 2^32
 constexpr int64_t kMaxNormGrid = 1 << 22;
 
-inline bool is_aligned(const void* p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
+inline bool is_aligned(const void* p, size_t a) { return rlx_is_aligned(p, a); }
 
 int check_hyper(float lr, float beta1, float beta2, float eps, float wd, float bc1, float bc2) {
     const float all[] = {lr, beta1, beta2, eps, wd, bc1, bc2};
@@ -1795,6 +1783,11 @@ int plan_update(const rlx_plan* p, const Hyper& h, const rlx_step_params* dev_pa
 
 }  // namespace
 
+int rlx_internal_hip_fail(hipError_t e, const char* what) {
+    snprintf(g_hip_error, sizeof(g_hip_error), "%s: %s", what, hipGetErrorString(e));
+    return RLX_ERR_HIP;
+}
+
 extern "C" {
 
 const char* rlx_status_string(int status) {
@@ -1814,7 +1807,7 @@ const char* rlx_status_string(int status) {
 
 const char* rlx_last_hip_error(void) { return g_hip_error; }
 
-int rlx_version(void) { return 109; }
+int rlx_version(void) { return 110; }
 
 int rlx_adamw_fp16(float* master_w, uint16_t* model_w, const uint16_t* grad, float* m, float* v, int64_t n,
                    float lr, float beta1, float beta2, float eps, float weight_decay,

@@ -1,0 +1,1131 @@
+// MI355X (gfx950) loss operators: token log-probabilities from logits with their gradient, the clipped policy
+// loss with a KL term (from log-probabilities, or straight from the logits) and the preference loss.  C ABI in
+// include/rlx_adamw.h.
+//
+// The work is streams of logits over HBM with one exponential per element; there is nothing for the matrix cores.
+//
+// Softmax statistics.  With k = log2(e) / temperature a row's softmax is 2^(z k) / sum 2^(z k).  A lane keeps
+//     ref = an integer, sum = sum 2^(z k - ref), dot = sum 2^(z k - ref) (z k - ref),
+// where ref is about the largest z k so far, rounded up.  z k - ref is one fused multiply-add (rounded once, so the
+// size of z k itself costs nothing), and because references are integers, bringing two partial results to a common
+// reference multiplies by a power of two: joining lanes, wavefronts or workgroups rounds nothing but the additions.
+// References are kept within +-2^29, so that logits of -inf and of a type's lowest value simply contribute 0.  Rows
+// whose own values lie out there (every logit the lowest value, +inf, NaN) come out with a sum of 0, infinity or NaN;
+// such rows, and only they, are computed again with the row's maximum subtracted first.
+
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+#include <cstdint>
+#include <cstring>
+
+#include "rlx_adamw.h"
+#include "rlx_internal.h"
+
+namespace {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+// 16 bytes at any 2-byte boundary: rows of an odd vocabulary start anywhere (gfx950 reads and writes these as one
+// 128-bit access)
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.693147180559945309417f;
+constexpr float kLn2Hi = 0.693145751953125f;              // 15 bits: an integer below 2^9 times this is exact
+constexpr float kLn2Lo = 1.42860682030941723212e-6f;
+constexpr float kRefMost = 536870912.0f;                  // 2^29
+constexpr float kLeastD = -1e30f;                         // keeps 0 * (-inf) out of sums of p log p
+
+struct Logits {             // rlx_logits as the kernels take it
+    char* data;
+    int64_t row_stride, group_stride;      // elements
+    uint32_t group_rows, rows;
+    int32_t vocab;
+};
+
+__device__ __forceinline__ int64_t row_at(const Logits& x, uint32_t r) {
+    if (x.group_rows >= x.rows) return (int64_t)r * x.row_stride;
+    const uint32_t g = r / x.group_rows;
+    return (int64_t)g * x.group_stride + (int64_t)(r - g * x.group_rows) * x.row_stride;
+}
+
+// --- the three logit types: PER elements in 16 bytes -----------------------------------------------------------------
+
+struct F16 {
+    static constexpr int PER = 8, SIZE = 2;
+    static __device__ __forceinline__ void unpack(u32x4 v, float (&f)[8]) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t w = v[i];
+            const f16x2 h = __builtin_bit_cast(f16x2, w);
+            f[2 * i] = (float)h[0];
+            f[2 * i + 1] = (float)h[1];
+        }
+    }
+    static __device__ __forceinline__ u32x4 pack(const float (&f)[8]) {        // round to nearest even
+        u32x4 v;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const f16x2 h = {(_Float16)f[2 * i], (_Float16)f[2 * i + 1]};
+            v[i] = __builtin_bit_cast(uint32_t, h);
+        }
+        return v;
+    }
+    static __device__ __forceinline__ float one(const char* p, int64_t i) {
+        return (float)((const RLX_GLOBAL _Float16*)p)[i];
+    }
+    static __device__ __forceinline__ void put(char* p, int64_t i, float f) { ((RLX_GLOBAL _Float16*)p)[i] = (_Float16)f; }
+};
+
+struct BF16 {
+    static constexpr int PER = 8, SIZE = 2;
+    static __device__ __forceinline__ void unpack(u32x4 v, float (&f)[8]) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t w = v[i];
+            f[2 * i] = __builtin_bit_cast(float, w << 16);
+            f[2 * i + 1] = __builtin_bit_cast(float, w & 0xffff0000u);
+        }
+    }
+    static __device__ __forceinline__ u32x4 pack(const float (&f)[8]) {
+        u32x4 v;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const f32x2 two = {f[2 * i], f[2 * i + 1]};
+            const bf16x2 h = __builtin_convertvector(two, bf16x2);
+            v[i] = __builtin_bit_cast(uint32_t, h);
+        }
+        return v;
+    }
+    static __device__ __forceinline__ float one(const char* p, int64_t i) {
+        const uint32_t w = ((const RLX_GLOBAL uint16_t*)p)[i];
+        return __builtin_bit_cast(float, w << 16);
+    }
+    static __device__ __forceinline__ void put(char* p, int64_t i, float f) { ((RLX_GLOBAL __bf16*)p)[i] = (__bf16)f; }
+};
+
+struct F32 {
+    static constexpr int PER = 4, SIZE = 4;
+    static __device__ __forceinline__ void unpack(u32x4 v, float (&f)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t w = v[i];
+            f[i] = __builtin_bit_cast(float, w);
+        }
+    }
+    static __device__ __forceinline__ u32x4 pack(const float (&f)[4]) {
+        u32x4 v;
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = __builtin_bit_cast(uint32_t, f[i]);
+        return v;
+    }
+    static __device__ __forceinline__ float one(const char* p, int64_t i) { return ((const RLX_GLOBAL float*)p)[i]; }
+    static __device__ __forceinline__ void put(char* p, int64_t i, float f) { ((RLX_GLOBAL float*)p)[i] = f; }
+};
+
+__device__ __forceinline__ u32x4 load16(const char* p) { return *(const RLX_GLOBAL u32x4_any*)(const RLX_GLOBAL char*)p; }
+__device__ __forceinline__ void store16(char* p, u32x4 v) { *(RLX_GLOBAL u32x4_any*)(RLX_GLOBAL char*)p = v; }
+__device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }     // 1 ulp
+
+// --- statistics of a row ---------------------------------------------------------------------------------------------
+
+struct Stat {
+    float ref, sum, dot;
+};
+constexpr Stat kNoStat = {-kRefMost, 0.0f, 0.0f};
+
+__device__ __forceinline__ float reference_of(float top, float k) {
+    return fminf(fmaxf(__builtin_ceilf(top * k), -kRefMost), kRefMost);
+}
+
+template <bool DOT>
+__device__ __forceinline__ Stat joined(Stat a, Stat b) {
+    const float ref = fmaxf(a.ref, b.ref), da = a.ref - ref, db = b.ref - ref;
+    const float fa = exp2_of(da), fb = exp2_of(db);              // powers of two: exact
+    Stat r;
+    r.ref = ref;
+    r.sum = a.sum * fa + b.sum * fb;
+    r.dot = 0.0f;
+    if constexpr (DOT) r.dot = fa * (a.dot + da * a.sum) + fb * (b.dot + db * b.sum);
+    return r;
+}
+
+// Adds N logits to a lane's statistics.
+template <bool DOT, int N>
+__device__ __forceinline__ void add_logits(Stat& s, const float (&z)[N], float k) {
+    float top = z[0];
+#pragma unroll
+    for (int i = 1; i < N; i++) top = fmaxf(top, z[i]);
+    // the reference follows the maximum at a distance of up to 16 powers of two: it moves a few times a row
+    if (top * k > s.ref + 16.0f && s.ref < kRefMost) {
+        const float ref = reference_of(top, k), d = s.ref - ref, f = exp2_of(d);
+        if constexpr (DOT) s.dot = f * (s.dot + d * s.sum);
+        s.sum *= f;
+        s.ref = ref;
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const float d = __builtin_fmaf(z[i], k, -s.ref), e = exp2_of(d);
+        s.sum += e;
+        if constexpr (DOT) s.dot = __builtin_fmaf(e, fmaxf(d, kLeastD), s.dot);
+    }
+}
+
+// Joins the statistics of all lanes of a workgroup; every lane gets the result.  The order is fixed.
+template <bool DOT, int BLOCK>
+__device__ Stat join_block(Stat s, Stat* shared) {
+#pragma unroll
+    for (int mask = 32; mask >= 1; mask >>= 1) {
+        Stat o;
+        o.ref = __shfl_xor(s.ref, mask);
+        o.sum = __shfl_xor(s.sum, mask);
+        o.dot = DOT ? __shfl_xor(s.dot, mask) : 0.0f;
+        s = joined<DOT>(s, o);
+    }
+    if constexpr (BLOCK > 64) {
+        if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = s;
+        __syncthreads();
+        s = shared[0];
+#pragma unroll
+        for (int w = 1; w < BLOCK / 64; w++) s = joined<DOT>(s, shared[w]);
+        __syncthreads();
+    }
+    return s;
+}
+
+// What the row's softmax is computed from: 2^((z - shift) k - ref) / sum.
+struct Row {
+    float shift, ref, sum, dot;
+};
+
+template <int BLOCK>
+__device__ float max_block(float v, float* shared) {
+#pragma unroll
+    for (int mask = 32; mask >= 1; mask >>= 1) v = fmaxf(v, __shfl_xor(v, mask));
+    if constexpr (BLOCK > 64) {
+        if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = shared[0];
+#pragma unroll
+        for (int w = 1; w < BLOCK / 64; w++) v = fmaxf(v, shared[w]);
+        __syncthreads();
+    }
+    return v;
+}
+
+// The rare rows: maximum first, then the sums with it subtracted, one element at a time.
+template <typename T, int BLOCK>
+__device__ __attribute__((noinline)) Row row_by_maximum(const char* row, int vocab, float k, Stat* shared) {
+    float top = -INFINITY;
+    for (int j = threadIdx.x; j < vocab; j += BLOCK) top = fmaxf(top, T::one(row, j));
+    top = max_block<BLOCK>(top, (float*)shared);
+    Stat s = {0.0f, 0.0f, 0.0f};
+    for (int j = threadIdx.x; j < vocab; j += BLOCK) {
+        const float d = (T::one(row, j) - top) * k, e = exp2_of(d);
+        s.sum += e;
+        s.dot = __builtin_fmaf(e, fmaxf(d, kLeastD), s.dot);
+    }
+    s = join_block<true, BLOCK>(s, shared);
+    return {top, 0.0f, s.sum, s.dot};
+}
+
+__device__ __forceinline__ bool ordinary(float sum) { return sum > 0.0f && sum < INFINITY; }
+
+struct RowValues {
+    float lse, logp, entropy, log2_sum;
+};
+
+// lse, log-probability of a target with logit zt, and entropy (nats).  The sum's exponent is folded into the integer
+// reference, so that what is rounded is of the size of the result.
+__device__ __forceinline__ RowValues row_values(const Row& row, float zt, float k, float inv_t) {
+    int e;
+    const float mant = frexpf(row.sum, &e);
+    const float ref = row.ref + (float)e, lm = log2f(mant);
+    RowValues v;
+    v.log2_sum = (float)e + lm;
+    v.lse = __builtin_fmaf(ref, kLn2Hi, __builtin_fmaf(ref, kLn2Lo, kLn2 * lm));
+    if (row.shift != 0.0f) v.lse = row.shift * inv_t + v.lse;
+    v.logp = (__builtin_fmaf(zt - row.shift, k, -ref) - lm) * kLn2;
+    v.entropy = (v.log2_sum - row.dot / row.sum) * kLn2;
+    return v;
+}
+
+__device__ __forceinline__ int64_t target_at(const void* targets, int wide, int64_t r) {
+    return wide ? ((const RLX_GLOBAL int64_t*)targets)[r] : (int64_t)((const RLX_GLOBAL int32_t*)targets)[r];
+}
+
+// Statistics of one row by a whole workgroup, streaming.
+template <typename T, int BLOCK, bool DOT>
+__device__ Row row_statistics(const char* row, int vocab, float k, Stat* shared) {
+    constexpr int PER = T::PER;
+    const int groups = vocab / PER;
+    Stat s = kNoStat;
+    for (int g = threadIdx.x; g < groups; g += BLOCK) {
+        float z[PER];
+        T::unpack(load16(row + (int64_t)g * 16), z);
+        add_logits<DOT>(s, z, k);
+    }
+    const int j = groups * PER + threadIdx.x;
+    if (j < vocab) {
+        float z[1] = {T::one(row, j)};
+        add_logits<DOT>(s, z, k);
+    }
+    s = join_block<DOT, BLOCK>(s, shared);
+    if (!ordinary(s.sum)) return row_by_maximum<T, BLOCK>(row, vocab, k, shared);
+    return {0.0f, s.ref, s.sum, s.dot};
+}
+
+// The gradient of a row: -p (b0 + b1 d) with d = (z - shift) k - ref, plus `hot` at the target.
+struct RowGrad {
+    float shift, ref, b0, b1, hot;
+};
+
+// g: gradient of logp; c: gradient of the entropy (both with 1/temperature in them).
+__device__ __forceinline__ RowGrad row_gradient(const Row& row, const RowValues& v, float g, float c) {
+    const float inv = 1.0f / row.sum;
+    RowGrad q;
+    q.shift = row.shift;
+    q.ref = row.ref;
+    // log p = ln2 (d - log2 sum), so p (g + c (log p + H)) = p (g + c (H - ln2 log2 sum) + c ln2 d)
+    q.b0 = -inv * (g + c * (v.entropy - kLn2 * v.log2_sum));
+    q.b1 = -inv * (c * kLn2);
+    q.hot = g;
+    return q;
+}
+
+template <bool DOT>
+__device__ __forceinline__ float grad_of(const RowGrad& q, float z, float k) {
+    const float d = __builtin_fmaf(z, k, -q.ref), e = exp2_of(d);
+    if constexpr (DOT) return e * __builtin_fmaf(q.b1, fmaxf(d, kLeastD), q.b0);
+    else return e * q.b0;
+}
+
+template <bool DOT>
+__device__ __forceinline__ float grad_by_maximum(const RowGrad& q, float z, float k) {
+    const float d = (z - q.shift) * k, e = exp2_of(d);
+    if constexpr (DOT) return e * __builtin_fmaf(q.b1, fmaxf(d, kLeastD), q.b0);
+    else return e * q.b0;
+}
+
+// Writes `value` over a whole row (zeros of an ignored one, NaN of one with a bad target).
+template <typename T, int BLOCK>
+__device__ void fill_row(char* out, int vocab, float value) {
+    constexpr int PER = T::PER;
+    const int groups = vocab / PER;
+    float f[PER];
+#pragma unroll
+    for (int i = 0; i < PER; i++) f[i] = value;
+    const u32x4 v = T::pack(f);
+    for (int g = threadIdx.x; g < groups; g += BLOCK) store16(out + (int64_t)g * 16, v);
+    const int j = groups * PER + threadIdx.x;
+    if (j < vocab) T::put(out, j, value);
+}
+
+template <typename T, int BLOCK, bool DOT>
+__device__ void write_gradient(const char* row, char* out, int vocab, float k, const RowGrad& q, int target) {
+    constexpr int PER = T::PER;
+    const int groups = vocab / PER;
+    if (q.shift != 0.0f) {                    // a rare row: element by element
+        for (int j = threadIdx.x; j < vocab; j += BLOCK) {
+            const float d = grad_by_maximum<DOT>(q, T::one(row, j), k);
+            T::put(out, j, j == target ? d + q.hot : d);
+        }
+        return;
+    }
+    for (int g = threadIdx.x; g < groups; g += BLOCK) {
+        float z[PER];
+        T::unpack(load16(row + (int64_t)g * 16), z);
+#pragma unroll
+        for (int i = 0; i < PER; i++) z[i] = grad_of<DOT>(q, z[i], k);
+        if (g == target / PER) {
+#pragma unroll
+            for (int i = 0; i < PER; i++)
+                if (i == target % PER) z[i] += q.hot;
+        }
+        store16(out + (int64_t)g * 16, T::pack(z));
+    }
+    const int j = groups * PER + threadIdx.x;
+    if (j < vocab) {
+        const float d = grad_of<DOT>(q, T::one(row, j), k);
+        T::put(out, j, j == target ? d + q.hot : d);
+    }
+}
+
+// --- kernels over logits ---------------------------------------------------------------------------------------------
+
+constexpr int kRowBlock = 512;
+
+// One workgroup per row.
+template <typename T, bool DOT>
+__global__ __launch_bounds__(kRowBlock) void token_logprob_kernel(Logits x, const void* __restrict__ targets, int wide,
+                                                                  float k, float inv_t, float* __restrict__ logp,
+                                                                  float* __restrict__ lse, float* __restrict__ entropy,
+                                                                  uint32_t first) {
+    __shared__ Stat shared[kRowBlock / 64];
+    const uint32_t r = first + blockIdx.x;
+    const int64_t t = target_at(targets, wide, r);
+    if (t < 0 || t >= x.vocab) {
+        if (threadIdx.x == 0) {
+            const float v = t < 0 ? 0.0f : NAN;
+            logp[r] = v;
+            lse[r] = v;
+            if (entropy) entropy[r] = v;
+        }
+        return;
+    }
+    const char* row = x.data + row_at(x, r) * T::SIZE;
+    const float zt = T::one(row, t);
+    const Row s = row_statistics<T, kRowBlock, DOT>(row, x.vocab, k, shared);
+    if (threadIdx.x == 0) {
+        const RowValues v = row_values(s, zt, k, inv_t);
+        logp[r] = v.logp;
+        lse[r] = v.lse;
+        if (entropy) entropy[r] = v.entropy;
+    }
+}
+
+// One workgroup per row: dx from the saved lse (and entropy).  p = exp(z - lse) is formed as 2^((z/T - lse) log2 e), the
+// difference first, so that the rounding is of the size of log p.
+template <typename T, bool DOT>
+__global__ __launch_bounds__(kRowBlock) void token_logprob_backward_kernel(
+    Logits x, Logits dx, const void* __restrict__ targets, int wide, float inv_t, const float* __restrict__ lse,
+    const float* __restrict__ entropy, const float* __restrict__ dlogp, const float* __restrict__ dentropy, uint32_t first) {
+    constexpr int PER = T::PER;
+    const uint32_t r = first + blockIdx.x;
+    const int64_t t = target_at(targets, wide, r);
+    const char* row = x.data + row_at(x, r) * T::SIZE;
+    char* out = dx.data + row_at(dx, r) * T::SIZE;
+    const float g = t < 0 ? 0.0f : dlogp[r], c = (DOT && t >= 0) ? dentropy[r] : 0.0f;
+    if (t >= x.vocab) {
+        fill_row<T, kRowBlock>(out, x.vocab, NAN);
+        return;
+    }
+    if (g == 0.0f && c == 0.0f) {
+        fill_row<T, kRowBlock>(out, x.vocab, 0.0f);
+        return;
+    }
+    const float l = lse[r], h = DOT ? entropy[r] : 0.0f;
+    const float gs = g * inv_t, cs = c * inv_t;
+    const int target = (int)t, groups = x.vocab / PER;
+    auto grad = [&](float z) {
+        const float lp = __builtin_fmaf(z, inv_t, -l), p = exp2_of(lp * kLog2e);
+        if constexpr (DOT) return -p * __builtin_fmaf(cs, fmaxf(lp, kLeastD) + h, gs);
+        else return -p * gs;
+    };
+    for (int i = threadIdx.x; i < groups; i += kRowBlock) {
+        float z[PER];
+        T::unpack(load16(row + (int64_t)i * 16), z);
+#pragma unroll
+        for (int e = 0; e < PER; e++) z[e] = grad(z[e]);
+        if (i == target / PER) {
+#pragma unroll
+            for (int e = 0; e < PER; e++)
+                if (e == target % PER) z[e] += gs;
+        }
+        store16(out + (int64_t)i * 16, T::pack(z));
+    }
+    const int j = groups * PER + threadIdx.x;
+    if (j < x.vocab) {
+        const float d = grad(T::one(row, j));
+        T::put(out, j, j == target ? d + gs : d);
+    }
+}
+
+// --- sequences, weights, per-token losses --------------------------------------------------------------------------------
+
+struct Batch {              // sequences of a packed or padded batch of tokens
+    const uint8_t* mask;
+    const int32_t* cu;
+    int64_t tokens, n_seqs;
+};
+
+// First token and length of a sequence, kept inside the arrays whatever the offsets hold.
+__device__ __forceinline__ void sequence_at(const Batch& b, int64_t s, int64_t& begin, int64_t& end) {
+    if (b.cu) {
+        begin = ((const RLX_GLOBAL int32_t*)b.cu)[s];
+        end = ((const RLX_GLOBAL int32_t*)b.cu)[s + 1];
+        begin = begin < 0 ? 0 : begin > b.tokens ? b.tokens : begin;
+        end = end < begin ? begin : end > b.tokens ? b.tokens : end;
+    } else {
+        const int64_t n = b.tokens / b.n_seqs;
+        begin = s * n;
+        end = begin + n;
+    }
+}
+
+// The sequence that token t belongs to, -1 if it lies in front of the first or behind the last.
+__device__ __forceinline__ int64_t sequence_of(const Batch& b, int64_t t) {
+    if (!b.cu) return t / (b.tokens / b.n_seqs);
+    int64_t lo = 0, hi = b.n_seqs + 1;                  // first index whose offset is greater than t
+    while (lo < hi) {
+        const int64_t mid = (lo + hi) >> 1;
+        if (((const RLX_GLOBAL int32_t*)b.cu)[mid] <= t) lo = mid + 1;
+        else hi = mid;
+    }
+    return lo == 0 || lo > b.n_seqs ? -1 : lo - 1;
+}
+
+struct Policy {             // rlx_policy_args as the kernels take it
+    const float *old_logp, *ref_logp, *advantages, *entropy;
+    Batch batch;
+    double log_high, log_low;      // borders of the clip
+    double norm;
+    float high, low;               // 1 + clip_high, 1 - clip_low
+    float kl_coef, entropy_coef, grad_scale;
+    int reduction, per_token;
+};
+
+constexpr int kTerms = 6;      // per token or workgroup: weighted loss, policy, kl, entropy; clipped, rho
+struct Terms {
+    double v[kTerms];
+    int64_t count;
+};
+
+// exp(d) - 1 and exp(d) - 1 - d.  Near 0 the second is a Taylor series (the direct form would lose everything to
+// cancellation): the first term left out is below 2^-25 of the sum for |d| < 1/2.
+__device__ __forceinline__ void kl_of(float d, float& em1, float& kl) {
+    if (fabsf(d) < 0.5f) {
+        float p = 1.0f / 3628800.0f;
+        p = __builtin_fmaf(p, d, 1.0f / 362880.0f);
+        p = __builtin_fmaf(p, d, 1.0f / 40320.0f);
+        p = __builtin_fmaf(p, d, 1.0f / 5040.0f);
+        p = __builtin_fmaf(p, d, 1.0f / 720.0f);
+        p = __builtin_fmaf(p, d, 1.0f / 120.0f);
+        p = __builtin_fmaf(p, d, 1.0f / 24.0f);
+        p = __builtin_fmaf(p, d, 1.0f / 6.0f);
+        p = __builtin_fmaf(p, d, 0.5f);
+        kl = p * d * d;
+        em1 = d + kl;
+    } else {
+        em1 = expf(d) - 1.0f;
+        kl = em1 == INFINITY ? em1 : em1 - d;
+    }
+}
+
+struct TokenLoss {
+    float policy, kl, ratio, slope;      // slope: gradient of the token's loss by its log-probability
+    bool clipped;
+};
+
+__device__ __forceinline__ TokenLoss token_loss(const Policy& a, float logp, float advantage, int64_t t) {
+    TokenLoss o;
+    // the side of the border is decided in FP64: the inputs' difference is exact there
+    const double lr = a.old_logp ? (double)logp - (double)((const RLX_GLOBAL float*)a.old_logp)[t] : 0.0;
+    o.clipped = advantage >= 0.0f ? lr > a.log_high : lr < a.log_low;
+    o.ratio = expf((float)lr);
+    // min(rho A, clip(rho) A) without the product of an infinite rho and A = 0
+    o.policy = -(advantage * (o.clipped ? (advantage >= 0.0f ? a.high : a.low) : o.ratio));
+    o.slope = o.clipped ? 0.0f : -(advantage * o.ratio);
+    o.kl = 0.0f;
+    if (a.ref_logp) {
+        float em1;
+        kl_of((float)((double)((const RLX_GLOBAL float*)a.ref_logp)[t] - (double)logp), em1, o.kl);
+        if (a.kl_coef != 0.0f) o.slope -= a.kl_coef * em1;
+    }
+    return o;
+}
+
+__device__ __forceinline__ double weight_of(const Policy& a, int64_t count) {
+    if (a.reduction == RLX_LOSS_SUM) return a.norm;
+    if (count < 1) count = 1;              // only with offsets that do not ascend
+    if (a.reduction == RLX_LOSS_TOKEN_MEAN) return a.norm / (double)count;
+    return a.norm / ((double)a.batch.n_seqs * (double)count);
+}
+
+template <int BLOCK>
+__device__ int64_t sum_block(int64_t v, int64_t* shared) {
+#pragma unroll
+    for (int mask = 32; mask >= 1; mask >>= 1) v += __shfl_xor(v, mask);
+    if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0;
+#pragma unroll
+    for (int w = 0; w < BLOCK / 64; w++) v += shared[w];
+    __syncthreads();
+    return v;
+}
+
+template <int BLOCK>
+__device__ double sum_block(double v, double* shared) {
+#pragma unroll
+    for (int mask = 32; mask >= 1; mask >>= 1) v += __shfl_xor(v, mask);
+    if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0.0;
+#pragma unroll
+    for (int w = 0; w < BLOCK / 64; w++) v += shared[w];
+    __syncthreads();
+    return v;
+}
+
+constexpr int kTokenBlock = 256;
+
+__device__ __forceinline__ bool counts(const Batch& b, const void* targets, int wide, int64_t t) {
+    if (b.mask && ((const RLX_GLOBAL uint8_t*)b.mask)[t] == 0) return false;
+    return !targets || target_at(targets, wide, t) >= 0;
+}
+
+// How many tokens of each sequence count.
+__global__ __launch_bounds__(kTokenBlock) void sequence_counts_kernel(Batch b, const void* __restrict__ targets, int wide,
+                                                                      int32_t* __restrict__ out) {
+    __shared__ int64_t shared[kTokenBlock / 64];
+    for (int64_t s = blockIdx.x; s < b.n_seqs; s += gridDim.x) {
+        int64_t begin, end, n = 0;
+        sequence_at(b, s, begin, end);
+        for (int64_t t = begin + threadIdx.x; t < end; t += kTokenBlock) n += counts(b, targets, wide, t) ? 1 : 0;
+        n = sum_block<kTokenBlock>(n, shared);
+        if (threadIdx.x == 0) out[s] = (int32_t)n;
+    }
+}
+
+// The count that token weights divide by: the sequence's own, or the whole batch's.
+template <int BLOCK>
+__device__ int64_t batch_count(const Batch& b, const int32_t* __restrict__ seq_counts, int64_t* shared) {
+    int64_t n = 0;
+    for (int64_t s = threadIdx.x; s < b.n_seqs; s += BLOCK) n += seq_counts[s];
+    return sum_block<BLOCK>(n, shared);
+}
+
+// Policy loss over log-probabilities: a workgroup takes kTokenBlock tokens.
+__global__ __launch_bounds__(kTokenBlock) void policy_loss_kernel(Policy a, const float* __restrict__ logp,
+                                                                  const int32_t* __restrict__ seq_counts,
+                                                                  float* __restrict__ dlogp, float* __restrict__ dentropy,
+                                                                  Terms* __restrict__ partials, int64_t first) {
+    __shared__ int64_t shared_n[kTokenBlock / 64];
+    __shared__ double shared[kTokenBlock / 64];
+    const int64_t total = a.reduction == RLX_LOSS_TOKEN_MEAN ? batch_count<kTokenBlock>(a.batch, seq_counts, shared_n) : 0;
+    const int64_t t = (first + blockIdx.x) * kTokenBlock + threadIdx.x;
+    double v[kTerms] = {0.0, 0.0, 0.0, 0.0, 0.0, 0.0};
+    int64_t n = 0;
+    const int64_t s = t < a.batch.tokens ? sequence_of(a.batch, t) : -1;
+    if (t < a.batch.tokens) {
+        float g = 0.0f, dh = 0.0f;
+        if (s >= 0 && counts(a.batch, nullptr, 0, t)) {
+            const double w = weight_of(a, a.reduction == RLX_LOSS_TOKEN_MEAN ? total
+                                          : a.reduction == RLX_LOSS_SUM ? 1 : (int64_t)seq_counts[s]);
+            const float h = a.entropy ? a.entropy[t] : 0.0f;
+            const TokenLoss o = token_loss(a, logp[t], a.advantages[a.per_token ? t : s], t);
+            g = (float)(w * (double)o.slope) * a.grad_scale;
+            dh = (float)(w * -(double)a.entropy_coef) * a.grad_scale;
+            v[1] = w * (double)o.policy;
+            v[2] = w * (double)o.kl;
+            v[3] = w * (double)h;
+            v[4] = o.clipped ? 1.0 : 0.0;
+            v[5] = (double)o.ratio;
+            n = 1;
+        }
+        dlogp[t] = g;
+        if (dentropy) dentropy[t] = dh;
+    }
+    for (int i = 1; i < kTerms; i++) v[i] = sum_block<kTokenBlock>(v[i], shared);
+    n = sum_block<kTokenBlock>(n, shared_n);
+    if (threadIdx.x == 0) {
+        Terms& p = partials[first + blockIdx.x];
+        for (int i = 0; i < kTerms; i++) p.v[i] = v[i];
+        p.count = n;
+    }
+}
+
+// Adds the partial terms, in a fixed order, and writes the statistics.
+__global__ __launch_bounds__(1024) void policy_stats_kernel(const Terms* __restrict__ partials, int64_t n, float kl_coef,
+                                                            float entropy_coef, rlx_policy_stats* __restrict__ stats) {
+    __shared__ double shared[16];
+    __shared__ int64_t shared_n[16];
+    double v[kTerms] = {0.0, 0.0, 0.0, 0.0, 0.0, 0.0};
+    int64_t count = 0;
+    for (int64_t i = threadIdx.x; i < n; i += 1024) {
+        for (int j = 1; j < kTerms; j++) v[j] += partials[i].v[j];
+        count += partials[i].count;
+    }
+    for (int j = 1; j < kTerms; j++) v[j] = sum_block<1024>(v[j], shared);
+    count = sum_block<1024>(count, shared_n);
+    if (threadIdx.x == 0) {
+        double loss = v[1];
+        if (kl_coef != 0.0f) loss += (double)kl_coef * v[2];
+        if (entropy_coef != 0.0f) loss -= (double)entropy_coef * v[3];
+        const double m = count > 0 ? (double)count : 1.0;
+        stats->loss = (float)loss;
+        stats->policy = (float)v[1];
+        stats->kl = (float)v[2];
+        stats->entropy = (float)v[3];
+        stats->clip_fraction = (float)(v[4] / m);
+        stats->ratio = (float)(v[5] / m);
+        stats->tokens = count;
+    }
+}
+
+// Policy loss from logits: one workgroup per row.
+template <typename T, bool DOT>
+__global__ __launch_bounds__(kRowBlock) void policy_loss_logits_kernel(
+    Logits x, Logits dx, const void* __restrict__ targets, int wide, float k, float inv_t, Policy a,
+    const int32_t* __restrict__ seq_counts, float* __restrict__ logp, float* __restrict__ entropy,
+    Terms* __restrict__ partials, uint32_t first) {
+    __shared__ Stat shared[kRowBlock / 64];
+    __shared__ int64_t shared_n[kRowBlock / 64];
+    const uint32_t r = first + blockIdx.x;
+    Terms p;
+    for (int i = 0; i < kTerms; i++) p.v[i] = 0.0;
+    p.count = 0;
+    const int64_t s = sequence_of(a.batch, r);
+    const char* row = x.data + row_at(x, r) * T::SIZE;
+    char* out = dx.data + row_at(dx, r) * T::SIZE;
+    const int64_t t = target_at(targets, wide, r);
+    if (s < 0 || !counts(a.batch, targets, wide, r)) {
+        fill_row<T, kRowBlock>(out, x.vocab, 0.0f);
+        if (threadIdx.x == 0) {
+            logp[r] = 0.0f;
+            if (entropy) entropy[r] = 0.0f;
+            partials[r] = p;
+        }
+        return;
+    }
+    p.count = 1;
+    if (t >= x.vocab) {
+        fill_row<T, kRowBlock>(out, x.vocab, NAN);
+        if (threadIdx.x == 0) {
+            logp[r] = NAN;
+            if (entropy) entropy[r] = NAN;
+            for (int i = 0; i < kTerms; i++) p.v[i] = NAN;
+            partials[r] = p;
+        }
+        return;
+    }
+    const float zt = T::one(row, t);
+    const int64_t m = a.reduction == RLX_LOSS_TOKEN_MEAN ? batch_count<kRowBlock>(a.batch, seq_counts, shared_n)
+                      : a.reduction == RLX_LOSS_SUM ? 1 : (int64_t)seq_counts[s];
+    const double w = weight_of(a, m);
+    const Row st = row_statistics<T, kRowBlock, true>(row, x.vocab, k, shared);
+    const RowValues v = row_values(st, zt, k, inv_t);
+    const TokenLoss o = token_loss(a, v.logp, a.advantages[a.per_token ? (int64_t)r : s], r);
+    const float ws = (float)w * (inv_t * a.grad_scale);
+    const float g = ws * o.slope, c = DOT ? -(ws * a.entropy_coef) : 0.0f;
+    const RowGrad q = row_gradient(st, v, g, c);
+    write_gradient<T, kRowBlock, DOT>(row, out, x.vocab, k, q, (int)t);
+    if (threadIdx.x == 0) {
+        logp[r] = v.logp;
+        if (entropy) entropy[r] = v.entropy;
+        p.v[1] = w * (double)o.policy;
+        p.v[2] = w * (double)o.kl;
+        p.v[3] = w * (double)v.entropy;
+        p.v[4] = o.clipped ? 1.0 : 0.0;
+        p.v[5] = (double)o.ratio;
+        partials[r] = p;
+    }
+}
+
+// --- preference loss -------------------------------------------------------------------------------------------------
+
+struct Preference {
+    const float* ref_logp;
+    Batch batch;
+    int64_t n_pairs;
+    float beta, smoothing, margin, grad_scale;
+    int average;
+};
+
+struct PairTerms {
+    double loss, correct, diff, chosen, rejected;
+};
+
+// log(1 / (1 + e^-x))
+__device__ __forceinline__ double log_sigmoid(double x) { return fmin(x, 0.0) - log1p(exp(-fabs(x))); }
+
+constexpr int kPairBlock = 512;
+
+// One workgroup per pair: both sums, the pair's loss, and the gradient of its tokens.
+__global__ __launch_bounds__(kPairBlock) void preference_loss_kernel(Preference a, const float* __restrict__ logp,
+                                                                     float* __restrict__ dlogp, float* __restrict__ rewards,
+                                                                     PairTerms* __restrict__ partials) {
+    __shared__ double shared[kPairBlock / 64];
+    __shared__ int64_t shared_n[kPairBlock / 64];
+    const int64_t pair = blockIdx.x;
+    int64_t begin[2], end[2];
+    double reward[2], per[2];
+#pragma unroll
+    for (int side = 0; side < 2; side++) {
+        sequence_at(a.batch, pair + side * a.n_pairs, begin[side], end[side]);
+        double sum = 0.0;
+        int64_t n = 0;
+        for (int64_t t = begin[side] + threadIdx.x; t < end[side]; t += kPairBlock) {
+            if (!counts(a.batch, nullptr, 0, t)) continue;
+            sum += (double)logp[t] - (a.ref_logp ? (double)((const RLX_GLOBAL float*)a.ref_logp)[t] : 0.0);
+            n++;
+        }
+        sum = sum_block<kPairBlock>(sum, shared);
+        n = sum_block<kPairBlock>(n, shared_n);
+        per[side] = (double)a.beta * (a.average ? 1.0 / (double)(n > 0 ? n : 1) : 1.0);
+        reward[side] = sum * per[side];
+    }
+    const double diff = reward[0] - reward[1], x = diff - (double)a.margin, ls = (double)a.smoothing;
+    const double log_s = log_sigmoid(x), log_n = log_sigmoid(-x);
+    const double slope = (ls * exp(log_s) - (1.0 - ls) * exp(log_n)) / (double)a.n_pairs * (double)a.grad_scale;
+#pragma unroll
+    for (int side = 0; side < 2; side++) {
+        const float g = (float)(side ? -slope * per[side] : slope * per[side]);
+        for (int64_t t = begin[side] + threadIdx.x; t < end[side]; t += kPairBlock)
+            dlogp[t] = counts(a.batch, nullptr, 0, t) ? g : 0.0f;
+    }
+    // tokens in front of the first and behind the last sequence
+    if (a.batch.cu) {
+        int64_t lo, hi, unused;
+        sequence_at(a.batch, 0, lo, unused);
+        sequence_at(a.batch, 2 * a.n_pairs - 1, unused, hi);
+        const int64_t step = (int64_t)gridDim.x * kPairBlock, at = pair * kPairBlock + threadIdx.x;
+        for (int64_t t = at; t < lo; t += step) dlogp[t] = 0.0f;
+        for (int64_t t = hi + at; t < a.batch.tokens; t += step) dlogp[t] = 0.0f;
+    }
+    if (threadIdx.x == 0) {
+        if (rewards) {
+            rewards[pair] = (float)reward[0];
+            rewards[a.n_pairs + pair] = (float)reward[1];
+        }
+        // 0 * (-inf) of a label that is not smoothed is 0
+        const double loss = -(1.0 - ls) * (ls < 1.0 ? log_s : 0.0) - ls * (ls > 0.0 ? log_n : 0.0);
+        partials[pair] = {loss, diff > 0.0 ? 1.0 : 0.0, diff, reward[0], reward[1]};
+    }
+}
+
+__global__ __launch_bounds__(1024) void preference_stats_kernel(const PairTerms* __restrict__ partials, int64_t n,
+                                                                rlx_preference_stats* __restrict__ stats) {
+    __shared__ double shared[16];
+    double v[5] = {0.0, 0.0, 0.0, 0.0, 0.0};
+    for (int64_t i = threadIdx.x; i < n; i += 1024) {
+        v[0] += partials[i].loss;
+        v[1] += partials[i].correct;
+        v[2] += partials[i].diff;
+        v[3] += partials[i].chosen;
+        v[4] += partials[i].rejected;
+    }
+    for (int j = 0; j < 5; j++) v[j] = sum_block<1024>(v[j], shared);
+    if (threadIdx.x == 0) {
+        const double m = n > 0 ? 1.0 / (double)n : 0.0;
+        *stats = {(float)(v[0] * m), (float)(v[1] * m), (float)(v[2] * m), (float)(v[3] * m), (float)(v[4] * m)};
+    }
+}
+
+// --- host side -------------------------------------------------------------------------------------------------------
+
+constexpr int64_t kMaxRows = 0x7fffffff;
+constexpr int64_t kMaxVocab = 1 << 30;
+constexpr uint32_t kRowsPerLaunch = 1u << 21;        // times up to 1,024 lanes: below the 2^32 lanes of one launch
+
+size_t elem_size(int dtype) { return dtype == RLX_DTYPE_F32 ? 4 : 2; }
+
+// Elements from the first to one past the last of a matrix of rows, -1 if its strides are not usable.
+int64_t logits_span(const rlx_logits& x) {
+    const int64_t inner = x.group_rows > 0 && x.group_rows < x.rows ? x.group_rows : x.rows;
+    const int64_t outer = inner ? (x.rows + inner - 1) / inner : 0;
+    if (x.rows == 0) return 0;
+    if (inner > 1 && x.row_stride < x.vocab) return -1;
+    if (outer > 1 && x.group_stride < x.vocab) return -1;
+    // strides that could overflow or that overlap: the larger step has to clear everything the smaller one spans
+    const int64_t lim = (int64_t)1 << 60;
+    if ((inner > 1 && x.row_stride > lim / inner) || (outer > 1 && x.group_stride > lim / outer)) return -1;
+    const int64_t in_span = inner > 1 ? (inner - 1) * x.row_stride : 0;
+    const int64_t out_span = outer > 1 ? (outer - 1) * x.group_stride : 0;
+    if (inner > 1 && outer > 1) {
+        const bool rows_inside = x.group_stride >= in_span + x.vocab, groups_inside = x.row_stride >= out_span + x.vocab;
+        if (!rows_inside && !groups_inside) return -1;
+    }
+    return in_span + out_span + x.vocab;
+}
+
+int check_logits(const rlx_logits* x) {
+    if (!x || x->rows < 0 || x->vocab < 1 || x->group_rows < 0 || x->reserved != 0) return RLX_ERR_INVALID_ARG;
+    if (x->dtype != RLX_DTYPE_F16 && x->dtype != RLX_DTYPE_F32 && x->dtype != RLX_DTYPE_BF16) return RLX_ERR_INVALID_ARG;
+    if (x->rows > kMaxRows || x->vocab > kMaxVocab) return RLX_ERR_TOO_LARGE;
+    if (x->rows == 0) return RLX_OK;
+    if (logits_span(*x) < 0 || !x->data) return RLX_ERR_INVALID_ARG;
+    if (!rlx_is_aligned(x->data, elem_size(x->dtype))) return RLX_ERR_MISALIGNED;
+    return RLX_OK;
+}
+
+// dx is x itself or does not touch it.
+int check_gradient(const rlx_logits* x, const rlx_logits* dx) {
+    const int st = check_logits(dx);
+    if (st != RLX_OK) return st;
+    if (dx->rows != x->rows || dx->vocab != x->vocab || dx->dtype != x->dtype) return RLX_ERR_INVALID_ARG;
+    if (x->rows == 0) return RLX_OK;
+    const bool one_group = (x->group_rows == 0 || x->group_rows >= x->rows) && (dx->group_rows == 0 || dx->group_rows >= dx->rows);
+    if (x->data == dx->data) {
+        const bool same = (x->rows == 1) || (x->row_stride == dx->row_stride &&
+                          (one_group || (x->group_rows == dx->group_rows && x->group_stride == dx->group_stride)));
+        return same ? RLX_OK : RLX_ERR_INVALID_ARG;
+    }
+    const char *a = (const char*)x->data, *b = (const char*)dx->data;
+    const size_t es = elem_size(x->dtype);
+    const bool apart = a + logits_span(*x) * es <= b || b + logits_span(*dx) * es <= a;
+    return apart ? RLX_OK : RLX_ERR_INVALID_ARG;
+}
+
+Logits view(const rlx_logits& x) {
+    Logits v;
+    v.data = (char*)x.data;
+    v.row_stride = x.row_stride;
+    v.group_stride = x.group_stride;
+    v.rows = (uint32_t)x.rows;
+    v.group_rows = x.group_rows > 0 && x.group_rows < x.rows ? (uint32_t)x.group_rows : (uint32_t)x.rows;
+    v.vocab = (int32_t)x.vocab;
+    return v;
+}
+
+int check_targets(const void* targets, int index_type) {
+    if (index_type != RLX_INDEX_I32 && index_type != RLX_INDEX_I64) return RLX_ERR_INVALID_ARG;
+    if (!targets) return RLX_ERR_INVALID_ARG;
+    return rlx_is_aligned(targets, index_type == RLX_INDEX_I64 ? 8 : 4) ? RLX_OK : RLX_ERR_MISALIGNED;
+}
+
+int check_temperature(float t) {
+    // its reciprocal has to be a finite number too
+    return std::isfinite(t) && t > 0.0f && std::isfinite(kLog2e / t) ? RLX_OK : RLX_ERR_BAD_HYPER;
+}
+
+int check_workspace(const void* ws, int64_t have, int64_t need) {
+    if (have < need || (need > 0 && !ws)) return RLX_ERR_INVALID_ARG;
+    return rlx_is_aligned(ws, 16) ? RLX_OK : RLX_ERR_MISALIGNED;
+}
+
+bool floats_aligned(std::initializer_list<const void*> all) {
+    for (const void* p : all)
+        if (!rlx_is_aligned(p, 4)) return false;
+    return true;
+}
+
+int check_batch(const Batch& b) {
+    if (b.tokens < 0 || b.n_seqs < 0) return RLX_ERR_INVALID_ARG;
+    if (b.tokens > kMaxRows || b.n_seqs > kMaxRows) return RLX_ERR_TOO_LARGE;
+    if (b.tokens > 0 && b.n_seqs == 0) return RLX_ERR_INVALID_ARG;
+    if (!b.cu && b.n_seqs > 0 && b.tokens % b.n_seqs != 0) return RLX_ERR_INVALID_ARG;
+    return rlx_is_aligned(b.cu, 4) ? RLX_OK : RLX_ERR_MISALIGNED;
+}
+
+int64_t round16(int64_t n) { return (n + 15) & ~(int64_t)15; }
+int64_t token_blocks(int64_t tokens) { return (tokens + kTokenBlock - 1) / kTokenBlock; }
+
+int make_policy(const rlx_policy_args* p, int64_t tokens, Policy& a) {
+    if (!p) return RLX_ERR_INVALID_ARG;
+    a.old_logp = p->old_logp;
+    a.ref_logp = p->ref_logp;
+    a.advantages = p->advantages;
+    a.entropy = p->entropy;
+    a.batch = {p->mask, p->cu_seqlens, tokens, p->n_seqs};
+    const int st = check_batch(a.batch);
+    if (st != RLX_OK) return st;
+    if (p->reduction < RLX_LOSS_SEQUENCE_MEAN || p->reduction > RLX_LOSS_SUM) return RLX_ERR_INVALID_ARG;
+    const float all[] = {p->clip_low, p->clip_high, p->kl_coef, p->entropy_coef, p->norm, p->grad_scale};
+    for (float v : all)
+        if (!std::isfinite(v)) return RLX_ERR_BAD_HYPER;
+    if (p->clip_low < 0.0f || p->clip_low > 1.0f || p->clip_high < 0.0f) return RLX_ERR_BAD_HYPER;
+    if (tokens > 0 && !p->advantages) return RLX_ERR_INVALID_ARG;
+    if (!floats_aligned({p->old_logp, p->ref_logp, p->advantages, p->entropy})) return RLX_ERR_MISALIGNED;
+    a.log_high = std::log1p((double)p->clip_high);
+    a.log_low = std::log1p(-(double)p->clip_low);
+    a.high = (float)(1.0 + (double)p->clip_high);
+    a.low = (float)(1.0 - (double)p->clip_low);
+    a.norm = (double)p->norm;
+    a.kl_coef = p->kl_coef;
+    a.entropy_coef = p->entropy_coef;
+    a.grad_scale = p->grad_scale;
+    a.reduction = p->reduction;
+    a.per_token = p->advantage_per_token ? 1 : 0;
+    return RLX_OK;
+}
+
+hipError_t launch_counts(const Batch& b, const void* targets, int wide, int32_t* out, hipStream_t s) {
+    if (b.n_seqs == 0) return hipSuccess;
+    const int64_t grid = b.n_seqs < (1 << 20) ? b.n_seqs : (1 << 20);
+    sequence_counts_kernel<<<dim3((unsigned)grid), dim3(kTokenBlock), 0, s>>>(b, targets, wide, out);
+    return hipGetLastError();
+}
+
+// Calls f(T{}) for the logit type.
+template <typename Fn>
+void for_type(int dtype, Fn f) {
+    if (dtype == RLX_DTYPE_F16) f(F16{});
+    else if (dtype == RLX_DTYPE_BF16) f(BF16{});
+    else f(F32{});
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t rlx_token_logprob_workspace(const rlx_logits* x) { return check_logits(x) == RLX_OK ? 0 : -1; }
+
+int rlx_token_logprob(const rlx_logits* x, const void* targets, int index_type, float temperature, float* logp,
+                      float* lse, float* entropy, void* workspace, int64_t workspace_bytes, void* stream) {
+    int st = check_logits(x);
+    if (st != RLX_OK) return st;
+    if ((st = check_temperature(temperature)) != RLX_OK) return st;
+    if (x->rows == 0) return RLX_OK;
+    if ((st = check_targets(targets, index_type)) != RLX_OK) return st;
+    if (!logp || !lse) return RLX_ERR_INVALID_ARG;
+    if (!floats_aligned({logp, lse, entropy})) return RLX_ERR_MISALIGNED;
+    if ((st = check_workspace(workspace, workspace_bytes, rlx_token_logprob_workspace(x))) != RLX_OK) return st;
+    const Logits v = view(*x);
+    const float inv_t = 1.0f / temperature, k = kLog2e / temperature;
+    const int wide = index_type == RLX_INDEX_I64;
+    for (uint32_t first = 0; first < v.rows; first += kRowsPerLaunch) {
+        const uint32_t here = v.rows - first < kRowsPerLaunch ? v.rows - first : kRowsPerLaunch;
+        for_type(x->dtype, [&](auto type) {
+            typedef decltype(type) T;
+            if (entropy)
+                token_logprob_kernel<T, true><<<dim3(here), dim3(kRowBlock), 0, (hipStream_t)stream>>>(
+                    v, targets, wide, k, inv_t, logp, lse, entropy, first);
+            else
+                token_logprob_kernel<T, false><<<dim3(here), dim3(kRowBlock), 0, (hipStream_t)stream>>>(
+                    v, targets, wide, k, inv_t, logp, lse, entropy, first);
+        });
+        RLX_HIP(hipGetLastError());
+    }
+    return RLX_OK;
+}
+
+int rlx_token_logprob_backward(const rlx_logits* x, const void* targets, int index_type, float temperature,
+                               const float* lse, const float* entropy, const float* dlogp, const float* dentropy,
+                               const rlx_logits* dx, void* stream) {
+    int st = check_logits(x);
+    if (st != RLX_OK) return st;
+    if ((st = check_gradient(x, dx)) != RLX_OK) return st;
+    if ((st = check_temperature(temperature)) != RLX_OK) return st;
+    if (x->rows == 0) return RLX_OK;
+    if ((st = check_targets(targets, index_type)) != RLX_OK) return st;
+    if (!lse || !dlogp || !entropy != !dentropy) return RLX_ERR_INVALID_ARG;
+    if (!floats_aligned({lse, entropy, dlogp, dentropy})) return RLX_ERR_MISALIGNED;
+    const Logits v = view(*x), dv = view(*dx);
+    const float inv_t = 1.0f / temperature;
+    const int wide = index_type == RLX_INDEX_I64;
+    for (uint32_t first = 0; first < v.rows; first += kRowsPerLaunch) {
+        const uint32_t here = v.rows - first < kRowsPerLaunch ? v.rows - first : kRowsPerLaunch;
+        for_type(x->dtype, [&](auto type) {
+            typedef decltype(type) T;
+            if (dentropy)
+                token_logprob_backward_kernel<T, true><<<dim3(here), dim3(kRowBlock), 0, (hipStream_t)stream>>>(
+                    v, dv, targets, wide, inv_t, lse, entropy, dlogp, dentropy, first);
+            else
+                token_logprob_backward_kernel<T, false><<<dim3(here), dim3(kRowBlock), 0, (hipStream_t)stream>>>(
+                    v, dv, targets, wide, inv_t, lse, entropy, dlogp, dentropy, first);
+        });
+        RLX_HIP(hipGetLastError());
+    }
+    return RLX_OK;
+}
+
+int64_t rlx_policy_loss_workspace(int64_t tokens, int64_t n_seqs) {
+    if (tokens < 0 || n_seqs < 0 || tokens > kMaxRows || n_seqs > kMaxRows) return -1;
+    return round16(4 * n_seqs) + token_blocks(tokens) * (int64_t)sizeof(Terms);
+}
+
+int rlx_policy_loss(const float* logp, int64_t tokens, const rlx_policy_args* args, float* dlogp, float* dentropy,
+                    rlx_policy_stats* stats, void* workspace, int64_t workspace_bytes, void* stream) {
+    Policy a;
+    int st = make_policy(args, tokens, a);
+    if (st != RLX_OK) return st;
+    if (!stats || (tokens > 0 && (!logp || !dlogp))) return RLX_ERR_INVALID_ARG;
+    if (tokens > 0 && a.entropy_coef != 0.0f && (!a.entropy || !dentropy)) return RLX_ERR_INVALID_ARG;
+    if (!floats_aligned({logp, dlogp, dentropy}) || !rlx_is_aligned(stats, 8)) return RLX_ERR_MISALIGNED;
+    if ((st = check_workspace(workspace, workspace_bytes, rlx_policy_loss_workspace(tokens, a.batch.n_seqs))) != RLX_OK)
+        return st;
+    hipStream_t s = (hipStream_t)stream;
+    int32_t* seq_counts = (int32_t*)workspace;
+    Terms* partials = (Terms*)((char*)workspace + round16(4 * a.batch.n_seqs));
+    if (tokens && a.reduction != RLX_LOSS_SUM) RLX_HIP(launch_counts(a.batch, nullptr, 0, seq_counts, s));
+    const int64_t blocks = token_blocks(tokens);
+    if (blocks) {
+        policy_loss_kernel<<<dim3((unsigned)blocks), dim3(kTokenBlock), 0, s>>>(a, logp, seq_counts, dlogp, dentropy,
+                                                                                partials, 0);
+        RLX_HIP(hipGetLastError());
+    }
+    policy_stats_kernel<<<dim3(1), dim3(1024), 0, s>>>(partials, blocks, a.kl_coef, a.entropy_coef, stats);
+    RLX_HIP(hipGetLastError());
+    return RLX_OK;
+}
+
+int64_t rlx_policy_loss_logits_workspace(const rlx_logits* x, int64_t n_seqs) {
+    if (check_logits(x) != RLX_OK || n_seqs < 0 || n_seqs > kMaxRows) return -1;
+    return round16(4 * n_seqs) + x->rows * (int64_t)sizeof(Terms);
+}
+
+int rlx_policy_loss_logits(const rlx_logits* x, const void* targets, int index_type, float temperature,
+                           const rlx_policy_args* args, float* logp, float* entropy, const rlx_logits* dx,
+                           rlx_policy_stats* stats, void* workspace, int64_t workspace_bytes, void* stream) {
+    int st = check_logits(x);
+    if (st != RLX_OK) return st;
+    if ((st = check_gradient(x, dx)) != RLX_OK) return st;
+    if ((st = check_temperature(temperature)) != RLX_OK) return st;
+    Policy a;
+    if ((st = make_policy(args, x->rows, a)) != RLX_OK) return st;
+    if (!stats || a.entropy || (x->rows > 0 && !logp)) return RLX_ERR_INVALID_ARG;
+    if (x->rows > 0 && (st = check_targets(targets, index_type)) != RLX_OK) return st;
+    if (!floats_aligned({logp, entropy}) || !rlx_is_aligned(stats, 8)) return RLX_ERR_MISALIGNED;
+    if ((st = check_workspace(workspace, workspace_bytes, rlx_policy_loss_logits_workspace(x, a.batch.n_seqs))) != RLX_OK)
+        return st;
+    hipStream_t s = (hipStream_t)stream;
+    const Logits v = view(*x), dv = view(*dx);
+    const float inv_t = 1.0f / temperature, k = kLog2e / temperature;
+    const int wide = index_type == RLX_INDEX_I64;
+    int32_t* seq_counts = (int32_t*)workspace;
+    Terms* partials = (Terms*)((char*)workspace + round16(4 * a.batch.n_seqs));
+    if (v.rows && a.reduction != RLX_LOSS_SUM) RLX_HIP(launch_counts(a.batch, targets, wide, seq_counts, s));
+    for (uint32_t first = 0; first < v.rows; first += kRowsPerLaunch) {
+        const uint32_t here = v.rows - first < kRowsPerLaunch ? v.rows - first : kRowsPerLaunch;
+        for_type(x->dtype, [&](auto type) {
+            typedef decltype(type) T;
+            if (a.entropy_coef != 0.0f)
+                policy_loss_logits_kernel<T, true><<<dim3(here), dim3(kRowBlock), 0, s>>>(
+                    v, dv, targets, wide, k, inv_t, a, seq_counts, logp, entropy, partials, first);
+            else
+                policy_loss_logits_kernel<T, false><<<dim3(here), dim3(kRowBlock), 0, s>>>(
+                    v, dv, targets, wide, k, inv_t, a, seq_counts, logp, entropy, partials, first);
+        });
+        RLX_HIP(hipGetLastError());
+    }
+    policy_stats_kernel<<<dim3(1), dim3(1024), 0, s>>>(partials, v.rows, a.kl_coef, a.entropy_coef, stats);
+    RLX_HIP(hipGetLastError());
+    return RLX_OK;
+}
+
+int64_t rlx_preference_loss_workspace(int64_t tokens, int64_t n_pairs) {
+    if (tokens < 0 || n_pairs < 0 || tokens > kMaxRows || n_pairs > kMaxRows / 2) return -1;
+    return n_pairs * (int64_t)sizeof(PairTerms);
+}
+
+int rlx_preference_loss(const float* logp, int64_t tokens, const rlx_preference_args* args, float* dlogp,
+                        float* rewards, rlx_preference_stats* stats, void* workspace, int64_t workspace_bytes,
+                        void* stream) {
+    if (!args || !stats || args->reserved != 0 || args->n_pairs < 0) return RLX_ERR_INVALID_ARG;
+    if (args->n_pairs > kMaxRows / 2) return RLX_ERR_TOO_LARGE;
+    Preference a;
+    a.ref_logp = args->ref_logp;
+    a.batch = {args->mask, args->cu_seqlens, tokens, 2 * args->n_pairs};
+    int st = check_batch(a.batch);
+    if (st != RLX_OK) return st;
+    const float all[] = {args->beta, args->label_smoothing, args->margin, args->grad_scale};
+    for (float v : all)
+        if (!std::isfinite(v)) return RLX_ERR_BAD_HYPER;
+    if (args->label_smoothing < 0.0f || args->label_smoothing > 1.0f) return RLX_ERR_BAD_HYPER;
+    if (tokens > 0 && (!logp || !dlogp)) return RLX_ERR_INVALID_ARG;
+    if (!floats_aligned({logp, args->ref_logp, dlogp, rewards, stats})) return RLX_ERR_MISALIGNED;
+    if ((st = check_workspace(workspace, workspace_bytes, rlx_preference_loss_workspace(tokens, args->n_pairs))) != RLX_OK)
+        return st;
+    a.n_pairs = args->n_pairs;
+    a.beta = args->beta;
+    a.smoothing = args->label_smoothing;
+    a.margin = args->margin;
+    a.grad_scale = args->grad_scale;
+    a.average = args->average ? 1 : 0;
+    hipStream_t s = (hipStream_t)stream;
+    PairTerms* partials = (PairTerms*)workspace;
+    if (a.n_pairs) {
+        preference_loss_kernel<<<dim3((unsigned)a.n_pairs), dim3(kPairBlock), 0, s>>>(a, logp, dlogp, rewards, partials);
+        RLX_HIP(hipGetLastError());
+    }
+    preference_stats_kernel<<<dim3(1), dim3(1024), 0, s>>>(partials, a.n_pairs, stats);
+    RLX_HIP(hipGetLastError());
+    return RLX_OK;
+}
+
+}  // extern "C"

@@ -403,6 +403,43 @@ def accumulation_step(optimizer, micro_batch, grad_accum_steps, max_grad_norm, l
     return accum / grad_accum_steps, grad_norm
 
 
+def policy_step(optimizer, forward, backward, n_micro, max_grad_norm, fused_clip=False, freeze=None, stream=None,
+                **loss_args):
+    """GRPOTrainer::grpo_training_step (include/training/GRPO_trainer.h:452-517): clear the gradient pools; for each of
+    n_micro micro-batches forward(k) -> dict with the arguments of losses.policy_loss_logits (logits, targets,
+    advantages, old_logp, ref_logp, mask, cu_seqlens; whatever is the same for all goes into loss_args), the clipped
+    policy loss divided by n_micro, and backward(k, dlogits), which adds its gradients into the pools; then clear the
+    gradients of the tensor views in `freeze`, clip, step.  The gradient of the logits is written over the logits, so
+    they are read and written once and no second buffer is held.  Nothing is read by the host before the clip.
+    Returns (loss, pre-clip norm, statistics per micro-batch)."""
+    import numpy as np
+    import torch
+    from . import losses
+    if n_micro < 1:
+        raise ValueError("policy_step needs at least one micro-batch")
+    if "norm" in loss_args or "out" in loss_args:
+        raise ValueError("policy_step sets norm and out itself")
+    # one stream for all of it: the loss operators follow torch's current one
+    if stream is not None and stream != _stream():
+        with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=optimizer.store.device)):
+            return policy_step(optimizer, forward, backward, n_micro, max_grad_norm, fused_clip, freeze, None,
+                               **loss_args)
+    st = _stream()
+    optimizer.store.zero_grads(st)
+    norm = float(np.float32(1.0) / np.float32(n_micro))
+    results = []
+    for k in range(n_micro):
+        batch = dict(forward(k))
+        r = losses.policy_loss_logits(out=batch["logits"], norm=norm, **batch, **loss_args)
+        backward(k, r.dlogits)
+        results.append(r._replace(dlogits=None))
+    for t in (freeze or ()):
+        B.clear(t.data_ptr(), t.numel() * t.element_size(), st)
+    grad_norm = training_step(optimizer, max_grad_norm, fused_clip=fused_clip)
+    loss = float(torch.stack([r.stats[0] for r in results]).double().sum())
+    return loss, grad_norm, results
+
+
 class Logger:
     """JSON-lines metrics logger with the reference's interface (include/training/logger.h:27-128):
     log() accumulates, commit() writes the window's means as one object with a "step" key, appends to
