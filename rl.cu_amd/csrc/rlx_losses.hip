@@ -130,6 +130,73 @@ __device__ __forceinline__ u32x4 load16(const char* p) { return *(const RLX_GLOB
 __device__ __forceinline__ void store16(char* p, u32x4 v) { *(RLX_GLOBAL u32x4_any*)(RLX_GLOBAL char*)p = v; }
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }     // 1 ulp
 
+// --- reductions over a wavefront -------------------------------------------------------------------------------------
+// Data-parallel-primitive moves: shifts by 1, 2, 4 and 8 inside rows of 16 lanes leave a row's total in its last lane,
+// two broadcasts carry it over the four rows.  Lane 63 holds the result, which every lane gets.  Lanes that a move does
+// not reach add `none`.  The order of the additions is fixed.
+
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t moved(uint32_t none, uint32_t x) {
+    return (uint32_t)__builtin_amdgcn_update_dpp((int)none, (int)x, CTRL, ROWS, 0xf, false);
+}
+
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float moved(float none, float x) {
+    return __builtin_bit_cast(float, moved<CTRL, ROWS>(__builtin_bit_cast(uint32_t, none), __builtin_bit_cast(uint32_t, x)));
+}
+
+template <int CTRL, int ROWS, typename T8>
+__device__ __forceinline__ T8 moved8(T8 x) {               // 8 bytes; lanes not reached get 0
+    const uint64_t b = __builtin_bit_cast(uint64_t, x);
+    const uint64_t lo = moved<CTRL, ROWS>(0u, (uint32_t)b), hi = moved<CTRL, ROWS>(0u, (uint32_t)(b >> 32));
+    return __builtin_bit_cast(T8, lo | (hi << 32));
+}
+
+template <int LANES>                                        // of lanes 0 .. LANES - 1 (16 or 64)
+__device__ __forceinline__ float last_lane(float x) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), LANES - 1));
+}
+
+template <int LANES>
+__device__ __forceinline__ float wave_max(float x) {
+    x = fmaxf(x, moved<0x111, 0xf>(x, x));
+    x = fmaxf(x, moved<0x112, 0xf>(x, x));
+    x = fmaxf(x, moved<0x114, 0xf>(x, x));
+    x = fmaxf(x, moved<0x118, 0xf>(x, x));
+    if constexpr (LANES == 64) {
+        x = fmaxf(x, moved<0x142, 0xa>(x, x));
+        x = fmaxf(x, moved<0x143, 0xc>(x, x));
+    }
+    return last_lane<LANES>(x);
+}
+
+template <int LANES>
+__device__ __forceinline__ float wave_sum(float x) {
+    x += moved<0x111, 0xf>(0.0f, x);
+    x += moved<0x112, 0xf>(0.0f, x);
+    x += moved<0x114, 0xf>(0.0f, x);
+    x += moved<0x118, 0xf>(0.0f, x);
+    if constexpr (LANES == 64) {
+        x += moved<0x142, 0xa>(0.0f, x);
+        x += moved<0x143, 0xc>(0.0f, x);
+    }
+    return last_lane<LANES>(x);
+}
+
+template <typename T8>                                      // double or int64_t
+__device__ __forceinline__ T8 wave_sum8(T8 x) {
+    x += moved8<0x111, 0xf>(x);
+    x += moved8<0x112, 0xf>(x);
+    x += moved8<0x114, 0xf>(x);
+    x += moved8<0x118, 0xf>(x);
+    x += moved8<0x142, 0xa>(x);
+    x += moved8<0x143, 0xc>(x);
+    const uint64_t b = __builtin_bit_cast(uint64_t, x);
+    const uint64_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, 63);
+    const uint64_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), 63);
+    return __builtin_bit_cast(T8, lo | (hi << 32));
+}
+
 // --- statistics of a row ---------------------------------------------------------------------------------------------
 
 struct Stat {
@@ -139,18 +206,6 @@ constexpr Stat kNoStat = {-kRefMost, 0.0f, 0.0f};
 
 __device__ __forceinline__ float reference_of(float top, float k) {
     return fminf(fmaxf(__builtin_ceilf(top * k), -kRefMost), kRefMost);
-}
-
-template <bool DOT>
-__device__ __forceinline__ Stat joined(Stat a, Stat b) {
-    const float ref = fmaxf(a.ref, b.ref), da = a.ref - ref, db = b.ref - ref;
-    const float fa = exp2_of(da), fb = exp2_of(db);              // powers of two: exact
-    Stat r;
-    r.ref = ref;
-    r.sum = a.sum * fa + b.sum * fb;
-    r.dot = 0.0f;
-    if constexpr (DOT) r.dot = fa * (a.dot + da * a.sum) + fb * (b.dot + db * b.sum);
-    return r;
 }
 
 // Adds N logits to a lane's statistics.
@@ -174,24 +229,29 @@ __device__ __forceinline__ void add_logits(Stat& s, const float (&z)[N], float k
     }
 }
 
-// Joins the statistics of all lanes of a workgroup; every lane gets the result.  The order is fixed.
+// Joins the statistics of the first LANES lanes of a wavefront: the largest reference first, then plain sums.
+template <bool DOT, int LANES>
+__device__ __forceinline__ Stat join_wave(Stat s) {
+    Stat r;
+    r.ref = wave_max<LANES>(s.ref);
+    const float d = s.ref - r.ref, f = exp2_of(d);              // a power of two: exact
+    r.sum = wave_sum<LANES>(s.sum * f);
+    r.dot = DOT ? wave_sum<LANES>(f * (s.dot + d * s.sum)) : 0.0f;
+    return r;
+}
+
+// Joins the statistics of all lanes of a workgroup (up to 16 wavefronts); every lane gets the result.  `shared` may be
+// used again only behind another barrier.
 template <bool DOT, int BLOCK>
-__device__ Stat join_block(Stat s, Stat* shared) {
-#pragma unroll
-    for (int mask = 32; mask >= 1; mask >>= 1) {
-        Stat o;
-        o.ref = __shfl_xor(s.ref, mask);
-        o.sum = __shfl_xor(s.sum, mask);
-        o.dot = DOT ? __shfl_xor(s.dot, mask) : 0.0f;
-        s = joined<DOT>(s, o);
-    }
+__device__ __forceinline__ Stat join_block(Stat s, Stat* shared) {
+    static_assert(BLOCK <= 1024, "one entry per wavefront, at most 16");
+    s = join_wave<DOT, 64>(s);
     if constexpr (BLOCK > 64) {
         if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = s;
         __syncthreads();
-        s = shared[0];
-#pragma unroll
-        for (int w = 1; w < BLOCK / 64; w++) s = joined<DOT>(s, shared[w]);
-        __syncthreads();
+        const int lane = threadIdx.x & 63;
+        s = lane < BLOCK / 64 ? shared[lane] : kNoStat;
+        s = join_wave<DOT, 16>(s);
     }
     return s;
 }
@@ -202,16 +262,13 @@ struct Row {
 };
 
 template <int BLOCK>
-__device__ float max_block(float v, float* shared) {
-#pragma unroll
-    for (int mask = 32; mask >= 1; mask >>= 1) v = fmaxf(v, __shfl_xor(v, mask));
+__device__ __forceinline__ float max_block(float v, float* shared) {
+    v = wave_max<64>(v);
     if constexpr (BLOCK > 64) {
         if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = v;
         __syncthreads();
-        v = shared[0];
-#pragma unroll
-        for (int w = 1; w < BLOCK / 64; w++) v = fmaxf(v, shared[w]);
-        __syncthreads();
+        const int lane = threadIdx.x & 63;
+        v = wave_max<16>(lane < BLOCK / 64 ? shared[lane] : -INFINITY);
     }
     return v;
 }
@@ -221,7 +278,9 @@ template <typename T, int BLOCK>
 __device__ __attribute__((noinline)) Row row_by_maximum(const char* row, int vocab, float k, Stat* shared) {
     float top = -INFINITY;
     for (int j = threadIdx.x; j < vocab; j += BLOCK) top = fmaxf(top, T::one(row, j));
+    __syncthreads();                                  // `shared` held the row's first result
     top = max_block<BLOCK>(top, (float*)shared);
+    __syncthreads();
     Stat s = {0.0f, 0.0f, 0.0f};
     for (int j = threadIdx.x; j < vocab; j += BLOCK) {
         const float d = (T::one(row, j) - top) * k, e = exp2_of(d);
@@ -478,9 +537,10 @@ struct Policy {             // rlx_policy_args as the kernels take it
     int reduction, per_token;
 };
 
-constexpr int kTerms = 6;      // per token or workgroup: weighted loss, policy, kl, entropy; clipped, rho
+// What a token, a workgroup or a batch adds to the statistics.
 struct Terms {
-    double v[kTerms];
+    double policy, kl, entropy;      // weighted
+    double clipped, ratio;
     int64_t count;
 };
 
@@ -535,30 +595,36 @@ __device__ __forceinline__ double weight_of(const Policy& a, int64_t count) {
     return a.norm / ((double)a.batch.n_seqs * (double)count);
 }
 
-template <int BLOCK>
-__device__ int64_t sum_block(int64_t v, int64_t* shared) {
+// Sums of N values over a workgroup; every lane gets them.  `shared` (N per wavefront) may be used again only behind
+// another barrier.
+template <int BLOCK, int N, typename T8>
+__device__ __forceinline__ void sum_block(T8 (&v)[N], T8* shared) {
 #pragma unroll
-    for (int mask = 32; mask >= 1; mask >>= 1) v += __shfl_xor(v, mask);
-    if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = 0;
+    for (int i = 0; i < N; i++) v[i] = wave_sum8(v[i]);
+    if ((threadIdx.x & 63) == 0) {
 #pragma unroll
-    for (int w = 0; w < BLOCK / 64; w++) v += shared[w];
+        for (int i = 0; i < N; i++) shared[(threadIdx.x >> 6) * N + i] = v[i];
+    }
     __syncthreads();
-    return v;
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = shared[i];
+    for (int w = 1; w < BLOCK / 64; w++)
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] += shared[w * N + i];
 }
 
 template <int BLOCK>
-__device__ double sum_block(double v, double* shared) {
-#pragma unroll
-    for (int mask = 32; mask >= 1; mask >>= 1) v += __shfl_xor(v, mask);
-    if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = 0.0;
-#pragma unroll
-    for (int w = 0; w < BLOCK / 64; w++) v += shared[w];
-    __syncthreads();
-    return v;
+__device__ __forceinline__ int64_t sum_block(int64_t v, int64_t* shared) {
+    int64_t one[1] = {v};
+    sum_block<BLOCK, 1>(one, shared);
+    return one[0];
+}
+
+template <int BLOCK>
+__device__ __forceinline__ Terms sum_terms(const Terms& t, double* shared, int64_t* shared_n) {
+    double v[5] = {t.policy, t.kl, t.entropy, t.clipped, t.ratio};
+    sum_block<BLOCK, 5>(v, shared);
+    return {v[0], v[1], v[2], v[3], v[4], sum_block<BLOCK>(t.count, shared_n)};
 }
 
 constexpr int kTokenBlock = 256;
@@ -578,6 +644,7 @@ __global__ __launch_bounds__(kTokenBlock) void sequence_counts_kernel(Batch b, c
         for (int64_t t = begin + threadIdx.x; t < end; t += kTokenBlock) n += counts(b, targets, wide, t) ? 1 : 0;
         n = sum_block<kTokenBlock>(n, shared);
         if (threadIdx.x == 0) out[s] = (int32_t)n;
+        __syncthreads();
     }
 }
 
@@ -594,12 +661,11 @@ __global__ __launch_bounds__(kTokenBlock) void policy_loss_kernel(Policy a, cons
                                                                   const int32_t* __restrict__ seq_counts,
                                                                   float* __restrict__ dlogp, float* __restrict__ dentropy,
                                                                   Terms* __restrict__ partials, int64_t first) {
-    __shared__ int64_t shared_n[kTokenBlock / 64];
-    __shared__ double shared[kTokenBlock / 64];
+    __shared__ int64_t shared_n[kTokenBlock / 64], shared_m[kTokenBlock / 64];
+    __shared__ double shared[5 * kTokenBlock / 64];
     const int64_t total = a.reduction == RLX_LOSS_TOKEN_MEAN ? batch_count<kTokenBlock>(a.batch, seq_counts, shared_n) : 0;
     const int64_t t = (first + blockIdx.x) * kTokenBlock + threadIdx.x;
-    double v[kTerms] = {0.0, 0.0, 0.0, 0.0, 0.0, 0.0};
-    int64_t n = 0;
+    Terms v = {0.0, 0.0, 0.0, 0.0, 0.0, 0};
     const int64_t s = t < a.batch.tokens ? sequence_of(a.batch, t) : -1;
     if (t < a.batch.tokens) {
         float g = 0.0f, dh = 0.0f;
@@ -610,51 +676,44 @@ __global__ __launch_bounds__(kTokenBlock) void policy_loss_kernel(Policy a, cons
             const TokenLoss o = token_loss(a, logp[t], a.advantages[a.per_token ? t : s], t);
             g = (float)(w * (double)o.slope) * a.grad_scale;
             dh = (float)(w * -(double)a.entropy_coef) * a.grad_scale;
-            v[1] = w * (double)o.policy;
-            v[2] = w * (double)o.kl;
-            v[3] = w * (double)h;
-            v[4] = o.clipped ? 1.0 : 0.0;
-            v[5] = (double)o.ratio;
-            n = 1;
+            v = {w * (double)o.policy, w * (double)o.kl, w * (double)h, o.clipped ? 1.0 : 0.0, (double)o.ratio, 1};
         }
         dlogp[t] = g;
         if (dentropy) dentropy[t] = dh;
     }
-    for (int i = 1; i < kTerms; i++) v[i] = sum_block<kTokenBlock>(v[i], shared);
-    n = sum_block<kTokenBlock>(n, shared_n);
-    if (threadIdx.x == 0) {
-        Terms& p = partials[first + blockIdx.x];
-        for (int i = 0; i < kTerms; i++) p.v[i] = v[i];
-        p.count = n;
-    }
+    v = sum_terms<kTokenBlock>(v, shared, shared_m);
+    if (threadIdx.x == 0) partials[first + blockIdx.x] = v;
 }
 
+__device__ void write_stats(const Terms& v, float kl_coef, float entropy_coef, rlx_policy_stats* stats) {
+    double loss = v.policy;
+    if (kl_coef != 0.0f) loss += (double)kl_coef * v.kl;
+    if (entropy_coef != 0.0f) loss -= (double)entropy_coef * v.entropy;
+    const double m = v.count > 0 ? (double)v.count : 1.0;
+    *stats = {(float)loss, (float)v.policy, (float)v.kl, (float)v.entropy, (float)(v.clipped / m), (float)(v.ratio / m),
+              v.count};
+}
+
+constexpr int kStatsBlock = 512;
+
 // Adds the partial terms, in a fixed order, and writes the statistics.
-__global__ __launch_bounds__(1024) void policy_stats_kernel(const Terms* __restrict__ partials, int64_t n, float kl_coef,
-                                                            float entropy_coef, rlx_policy_stats* __restrict__ stats) {
-    __shared__ double shared[16];
-    __shared__ int64_t shared_n[16];
-    double v[kTerms] = {0.0, 0.0, 0.0, 0.0, 0.0, 0.0};
-    int64_t count = 0;
-    for (int64_t i = threadIdx.x; i < n; i += 1024) {
-        for (int j = 1; j < kTerms; j++) v[j] += partials[i].v[j];
-        count += partials[i].count;
+__global__ __launch_bounds__(kStatsBlock) void policy_stats_kernel(const Terms* __restrict__ partials, int64_t n,
+                                                                   float kl_coef, float entropy_coef,
+                                                                   rlx_policy_stats* __restrict__ stats) {
+    __shared__ double shared[5 * kStatsBlock / 64];
+    __shared__ int64_t shared_n[kStatsBlock / 64];
+    Terms v = {0.0, 0.0, 0.0, 0.0, 0.0, 0};
+    for (int64_t i = threadIdx.x; i < n; i += kStatsBlock) {
+        const Terms p = partials[i];
+        v.policy += p.policy;
+        v.kl += p.kl;
+        v.entropy += p.entropy;
+        v.clipped += p.clipped;
+        v.ratio += p.ratio;
+        v.count += p.count;
     }
-    for (int j = 1; j < kTerms; j++) v[j] = sum_block<1024>(v[j], shared);
-    count = sum_block<1024>(count, shared_n);
-    if (threadIdx.x == 0) {
-        double loss = v[1];
-        if (kl_coef != 0.0f) loss += (double)kl_coef * v[2];
-        if (entropy_coef != 0.0f) loss -= (double)entropy_coef * v[3];
-        const double m = count > 0 ? (double)count : 1.0;
-        stats->loss = (float)loss;
-        stats->policy = (float)v[1];
-        stats->kl = (float)v[2];
-        stats->entropy = (float)v[3];
-        stats->clip_fraction = (float)(v[4] / m);
-        stats->ratio = (float)(v[5] / m);
-        stats->tokens = count;
-    }
+    v = sum_terms<kStatsBlock>(v, shared, shared_n);
+    if (threadIdx.x == 0) write_stats(v, kl_coef, entropy_coef, stats);
 }
 
 // Policy loss from logits: one workgroup per row.
@@ -666,9 +725,7 @@ __global__ __launch_bounds__(kRowBlock) void policy_loss_logits_kernel(
     __shared__ Stat shared[kRowBlock / 64];
     __shared__ int64_t shared_n[kRowBlock / 64];
     const uint32_t r = first + blockIdx.x;
-    Terms p;
-    for (int i = 0; i < kTerms; i++) p.v[i] = 0.0;
-    p.count = 0;
+    Terms p = {0.0, 0.0, 0.0, 0.0, 0.0, 0};
     const int64_t s = sequence_of(a.batch, r);
     const char* row = x.data + row_at(x, r) * T::SIZE;
     char* out = dx.data + row_at(dx, r) * T::SIZE;
@@ -682,14 +739,12 @@ __global__ __launch_bounds__(kRowBlock) void policy_loss_logits_kernel(
         }
         return;
     }
-    p.count = 1;
     if (t >= x.vocab) {
         fill_row<T, kRowBlock>(out, x.vocab, NAN);
         if (threadIdx.x == 0) {
             logp[r] = NAN;
             if (entropy) entropy[r] = NAN;
-            for (int i = 0; i < kTerms; i++) p.v[i] = NAN;
-            partials[r] = p;
+            partials[r] = {NAN, NAN, NAN, NAN, NAN, 1};
         }
         return;
     }
@@ -707,12 +762,8 @@ __global__ __launch_bounds__(kRowBlock) void policy_loss_logits_kernel(
     if (threadIdx.x == 0) {
         logp[r] = v.logp;
         if (entropy) entropy[r] = v.entropy;
-        p.v[1] = w * (double)o.policy;
-        p.v[2] = w * (double)o.kl;
-        p.v[3] = w * (double)v.entropy;
-        p.v[4] = o.clipped ? 1.0 : 0.0;
-        p.v[5] = (double)o.ratio;
-        partials[r] = p;
+        partials[r] = {w * (double)o.policy, w * (double)o.kl, w * (double)v.entropy, o.clipped ? 1.0 : 0.0,
+                       (double)o.ratio, 1};
     }
 }
 
@@ -733,41 +784,56 @@ struct PairTerms {
 // log(1 / (1 + e^-x))
 __device__ __forceinline__ double log_sigmoid(double x) { return fmin(x, 0.0) - log1p(exp(-fabs(x))); }
 
+struct PairValues {
+    PairTerms terms;
+    float grad[2];               // of each counted token of the chosen and of the rejected sequence
+};
+
+// A pair's loss and gradient from its sums of log ratios and counts (chosen, rejected).
+__device__ __forceinline__ PairValues pair_values(const Preference& a, const double (&sum)[2], const int64_t (&n)[2]) {
+    double per[2], reward[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        per[i] = (double)a.beta * (a.average ? 1.0 / (double)(n[i] > 0 ? n[i] : 1) : 1.0);
+        reward[i] = sum[i] * per[i];
+    }
+    const double diff = reward[0] - reward[1], x = diff - (double)a.margin, ls = (double)a.smoothing;
+    const double log_s = log_sigmoid(x), log_n = log_sigmoid(-x);
+    const double slope = (ls * exp(log_s) - (1.0 - ls) * exp(log_n)) / (double)a.n_pairs * (double)a.grad_scale;
+    // 0 * (-inf) of a label that is not smoothed is 0
+    const double loss = -(1.0 - ls) * (ls < 1.0 ? log_s : 0.0) - ls * (ls > 0.0 ? log_n : 0.0);
+    return {{loss, diff > 0.0 ? 1.0 : 0.0, diff, reward[0], reward[1]}, {(float)(slope * per[0]), (float)(-slope * per[1])}};
+}
+
 constexpr int kPairBlock = 512;
 
 // One workgroup per pair: both sums, the pair's loss, and the gradient of its tokens.
 __global__ __launch_bounds__(kPairBlock) void preference_loss_kernel(Preference a, const float* __restrict__ logp,
                                                                      float* __restrict__ dlogp, float* __restrict__ rewards,
                                                                      PairTerms* __restrict__ partials) {
-    __shared__ double shared[kPairBlock / 64];
-    __shared__ int64_t shared_n[kPairBlock / 64];
+    __shared__ double shared[2 * kPairBlock / 64];
+    __shared__ int64_t shared_n[2 * kPairBlock / 64];
     const int64_t pair = blockIdx.x;
-    int64_t begin[2], end[2];
-    double reward[2], per[2];
+    int64_t begin[2], end[2], n[2];
+    double sum[2];
 #pragma unroll
     for (int side = 0; side < 2; side++) {
         sequence_at(a.batch, pair + side * a.n_pairs, begin[side], end[side]);
-        double sum = 0.0;
-        int64_t n = 0;
+        sum[side] = 0.0;
+        n[side] = 0;
         for (int64_t t = begin[side] + threadIdx.x; t < end[side]; t += kPairBlock) {
             if (!counts(a.batch, nullptr, 0, t)) continue;
-            sum += (double)logp[t] - (a.ref_logp ? (double)((const RLX_GLOBAL float*)a.ref_logp)[t] : 0.0);
-            n++;
+            sum[side] += (double)logp[t] - (a.ref_logp ? (double)((const RLX_GLOBAL float*)a.ref_logp)[t] : 0.0);
+            n[side]++;
         }
-        sum = sum_block<kPairBlock>(sum, shared);
-        n = sum_block<kPairBlock>(n, shared_n);
-        per[side] = (double)a.beta * (a.average ? 1.0 / (double)(n > 0 ? n : 1) : 1.0);
-        reward[side] = sum * per[side];
     }
-    const double diff = reward[0] - reward[1], x = diff - (double)a.margin, ls = (double)a.smoothing;
-    const double log_s = log_sigmoid(x), log_n = log_sigmoid(-x);
-    const double slope = (ls * exp(log_s) - (1.0 - ls) * exp(log_n)) / (double)a.n_pairs * (double)a.grad_scale;
+    sum_block<kPairBlock, 2>(sum, shared);
+    sum_block<kPairBlock, 2>(n, shared_n);
+    const PairValues v = pair_values(a, sum, n);
 #pragma unroll
-    for (int side = 0; side < 2; side++) {
-        const float g = (float)(side ? -slope * per[side] : slope * per[side]);
+    for (int side = 0; side < 2; side++)
         for (int64_t t = begin[side] + threadIdx.x; t < end[side]; t += kPairBlock)
-            dlogp[t] = counts(a.batch, nullptr, 0, t) ? g : 0.0f;
-    }
+            dlogp[t] = counts(a.batch, nullptr, 0, t) ? v.grad[side] : 0.0f;
     // tokens in front of the first and behind the last sequence
     if (a.batch.cu) {
         int64_t lo, hi, unused;
@@ -779,27 +845,26 @@ __global__ __launch_bounds__(kPairBlock) void preference_loss_kernel(Preference 
     }
     if (threadIdx.x == 0) {
         if (rewards) {
-            rewards[pair] = (float)reward[0];
-            rewards[a.n_pairs + pair] = (float)reward[1];
+            rewards[pair] = (float)v.terms.chosen;
+            rewards[a.n_pairs + pair] = (float)v.terms.rejected;
         }
-        // 0 * (-inf) of a label that is not smoothed is 0
-        const double loss = -(1.0 - ls) * (ls < 1.0 ? log_s : 0.0) - ls * (ls > 0.0 ? log_n : 0.0);
-        partials[pair] = {loss, diff > 0.0 ? 1.0 : 0.0, diff, reward[0], reward[1]};
+        partials[pair] = v.terms;
     }
 }
 
-__global__ __launch_bounds__(1024) void preference_stats_kernel(const PairTerms* __restrict__ partials, int64_t n,
-                                                                rlx_preference_stats* __restrict__ stats) {
-    __shared__ double shared[16];
+__global__ __launch_bounds__(kStatsBlock) void preference_stats_kernel(const PairTerms* __restrict__ partials, int64_t n,
+                                                                       rlx_preference_stats* __restrict__ stats) {
+    __shared__ double shared[5 * kStatsBlock / 64];
     double v[5] = {0.0, 0.0, 0.0, 0.0, 0.0};
-    for (int64_t i = threadIdx.x; i < n; i += 1024) {
-        v[0] += partials[i].loss;
-        v[1] += partials[i].correct;
-        v[2] += partials[i].diff;
-        v[3] += partials[i].chosen;
-        v[4] += partials[i].rejected;
+    for (int64_t i = threadIdx.x; i < n; i += kStatsBlock) {
+        const PairTerms p = partials[i];
+        v[0] += p.loss;
+        v[1] += p.correct;
+        v[2] += p.diff;
+        v[3] += p.chosen;
+        v[4] += p.rejected;
     }
-    for (int j = 0; j < 5; j++) v[j] = sum_block<1024>(v[j], shared);
+    sum_block<kStatsBlock, 5>(v, shared);
     if (threadIdx.x == 0) {
         const double m = n > 0 ? 1.0 / (double)n : 0.0;
         *stats = {(float)(v[0] * m), (float)(v[1] * m), (float)(v[2] * m), (float)(v[3] * m), (float)(v[4] * m)};
@@ -1039,7 +1104,7 @@ int rlx_policy_loss(const float* logp, int64_t tokens, const rlx_policy_args* ar
                                                                                 partials, 0);
         RLX_HIP(hipGetLastError());
     }
-    policy_stats_kernel<<<dim3(1), dim3(1024), 0, s>>>(partials, blocks, a.kl_coef, a.entropy_coef, stats);
+    policy_stats_kernel<<<dim3(1), dim3(kStatsBlock), 0, s>>>(partials, blocks, a.kl_coef, a.entropy_coef, stats);
     RLX_HIP(hipGetLastError());
     return RLX_OK;
 }
@@ -1083,7 +1148,7 @@ int rlx_policy_loss_logits(const rlx_logits* x, const void* targets, int index_t
         });
         RLX_HIP(hipGetLastError());
     }
-    policy_stats_kernel<<<dim3(1), dim3(1024), 0, s>>>(partials, v.rows, a.kl_coef, a.entropy_coef, stats);
+    policy_stats_kernel<<<dim3(1), dim3(kStatsBlock), 0, s>>>(partials, v.rows, a.kl_coef, a.entropy_coef, stats);
     RLX_HIP(hipGetLastError());
     return RLX_OK;
 }
@@ -1123,7 +1188,7 @@ int rlx_preference_loss(const float* logp, int64_t tokens, const rlx_preference_
         preference_loss_kernel<<<dim3((unsigned)a.n_pairs), dim3(kPairBlock), 0, s>>>(a, logp, dlogp, rewards, partials);
         RLX_HIP(hipGetLastError());
     }
-    preference_stats_kernel<<<dim3(1), dim3(1024), 0, s>>>(partials, a.n_pairs, stats);
+    preference_stats_kernel<<<dim3(1), dim3(kStatsBlock), 0, s>>>(partials, a.n_pairs, stats);
     RLX_HIP(hipGetLastError());
     return RLX_OK;
 }
