@@ -38,6 +38,7 @@ constexpr float kLn2Hi = 0.693145751953125f;              // 15 bits: an integer
 constexpr float kLn2Lo = 1.42860682030941723212e-6f;
 constexpr float kRefMost = 536870912.0f;                  // 2^29
 constexpr float kLeastD = -1e30f;                         // keeps 0 * (-inf) out of sums of p log p
+constexpr float kLeastZ = -1e30f;                         // the same, of a logit
 
 struct Logits {             // rlx_logits as the kernels take it
     char* data;
@@ -54,8 +55,31 @@ __device__ __forceinline__ int64_t row_at(const Logits& x, uint32_t r) {
 
 // --- the three logit types: PER elements in 16 bytes -----------------------------------------------------------------
 
+__device__ __forceinline__ uint32_t max_f16x2(uint32_t a, uint32_t b) {       // of NaN and a number: the number
+    uint32_t r;
+    asm("v_pk_max_f16 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+    return r;
+}
+
 struct F16 {
     static constexpr int PER = 8, SIZE = 2;
+    static constexpr uint32_t kLeast = 0xfc00fc00u, kLowest = 0xfbfffbffu;      // -inf, -65504
+    typedef uint32_t Top;                                                       // two running maxima
+    static __device__ __forceinline__ Top no_top() { return kLeast; }
+    static __device__ __forceinline__ void add_top(Top& t, u32x4 v) {
+        t = max_f16x2(max_f16x2(t, max_f16x2(v[0], v[1])), max_f16x2(v[2], v[3]));
+    }
+    static __device__ __forceinline__ float top_of(Top t) {
+        const f16x2 h = __builtin_bit_cast(f16x2, t);
+        return fmaxf((float)h[0], (float)h[1]);
+    }
+    // the values with -inf as the lowest number (for sums of p log p)
+    static __device__ __forceinline__ void unpack_finite(u32x4 v, float (&f)[8]) {
+        u32x4 w;
+#pragma unroll
+        for (int i = 0; i < 4; i++) w[i] = max_f16x2(v[i], kLowest);
+        unpack(w, f);
+    }
     static __device__ __forceinline__ void unpack(u32x4 v, float (&f)[8]) {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -82,6 +106,21 @@ struct F16 {
 
 struct BF16 {
     static constexpr int PER = 8, SIZE = 2;
+    static constexpr uint32_t kLeast = 0xff80ff80u;
+    typedef float Top;
+    static __device__ __forceinline__ Top no_top() { return -INFINITY; }
+    static __device__ __forceinline__ void add_top(Top& t, u32x4 v) {
+        float f[PER];
+        unpack(v, f);
+#pragma unroll
+        for (int i = 0; i < PER; i++) t = fmaxf(t, f[i]);
+    }
+    static __device__ __forceinline__ float top_of(Top t) { return t; }
+    static __device__ __forceinline__ void unpack_finite(u32x4 v, float (&f)[PER]) {
+        unpack(v, f);
+#pragma unroll
+        for (int i = 0; i < PER; i++) f[i] = fmaxf(f[i], kLeastZ);
+    }
     static __device__ __forceinline__ void unpack(u32x4 v, float (&f)[8]) {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -109,6 +148,21 @@ struct BF16 {
 
 struct F32 {
     static constexpr int PER = 4, SIZE = 4;
+    static constexpr uint32_t kLeast = 0xff800000u;
+    typedef float Top;
+    static __device__ __forceinline__ Top no_top() { return -INFINITY; }
+    static __device__ __forceinline__ void add_top(Top& t, u32x4 v) {
+        float f[PER];
+        unpack(v, f);
+#pragma unroll
+        for (int i = 0; i < PER; i++) t = fmaxf(t, f[i]);
+    }
+    static __device__ __forceinline__ float top_of(Top t) { return t; }
+    static __device__ __forceinline__ void unpack_finite(u32x4 v, float (&f)[PER]) {
+        unpack(v, f);
+#pragma unroll
+        for (int i = 0; i < PER; i++) f[i] = fmaxf(f[i], kLeastZ);
+    }
     static __device__ __forceinline__ void unpack(u32x4 v, float (&f)[4]) {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -127,6 +181,12 @@ struct F32 {
 };
 
 __device__ __forceinline__ u32x4 load16(const char* p) { return *(const RLX_GLOBAL u32x4_any*)(const RLX_GLOBAL char*)p; }
+__device__ __forceinline__ u32x4 load16_once(const char* p) {            // data that is not read again
+    return __builtin_nontemporal_load((const RLX_GLOBAL u32x4_any*)(const RLX_GLOBAL char*)p);
+}
+__device__ __forceinline__ void store16_once(char* p, u32x4 v) {
+    __builtin_nontemporal_store(v, (RLX_GLOBAL u32x4_any*)(RLX_GLOBAL char*)p);
+}
 __device__ __forceinline__ void store16(char* p, u32x4 v) { *(RLX_GLOBAL u32x4_any*)(RLX_GLOBAL char*)p = v; }
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }     // 1 ulp
 
@@ -196,6 +256,10 @@ __device__ __forceinline__ T8 wave_sum8(T8 x) {
     const uint64_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), 63);
     return __builtin_bit_cast(T8, lo | (hi << 32));
 }
+
+// Makes the compiler forget what it knows about a value: without this it keeps the unpacked FP32 form of a held group
+// from one pass over the registers to the next, which takes twice the registers.
+__device__ __forceinline__ void forget(u32x4& v) { asm volatile("" : "+v"(v)); }
 
 // --- statistics of a row ---------------------------------------------------------------------------------------------
 
@@ -716,31 +780,35 @@ __global__ __launch_bounds__(kStatsBlock) void policy_stats_kernel(const Terms* 
     if (threadIdx.x == 0) write_stats(v, kl_coef, entropy_coef, stats);
 }
 
-// Policy loss from logits: one workgroup per row.
-template <typename T, bool DOT>
-__global__ __launch_bounds__(kRowBlock) void policy_loss_logits_kernel(
+// Policy loss from logits: one workgroup per row, the row held in registers between its statistics and its gradient
+// (NG 16-byte groups per lane; a vocabulary beyond BLOCK * NG groups has its rest read a second time, from the
+// last-level cache mostly).
+template <typename T, int BLOCK, int NG, bool DOT>
+__global__ __launch_bounds__(BLOCK) void policy_loss_row_kernel(
     Logits x, Logits dx, const void* __restrict__ targets, int wide, float k, float inv_t, Policy a,
     const int32_t* __restrict__ seq_counts, float* __restrict__ logp, float* __restrict__ entropy,
     Terms* __restrict__ partials, uint32_t first) {
-    __shared__ Stat shared[kRowBlock / 64];
-    __shared__ int64_t shared_n[kRowBlock / 64];
+    constexpr int PER = T::PER;
+    __shared__ Stat shared[BLOCK / 64];
+    __shared__ Stat shared_rare[BLOCK / 64];
+    __shared__ RowGrad shared_grad;
+    __shared__ int64_t shared_n[BLOCK / 64];
     const uint32_t r = first + blockIdx.x;
-    Terms p = {0.0, 0.0, 0.0, 0.0, 0.0, 0};
-    const int64_t s = sequence_of(a.batch, r);
     const char* row = x.data + row_at(x, r) * T::SIZE;
     char* out = dx.data + row_at(dx, r) * T::SIZE;
     const int64_t t = target_at(targets, wide, r);
+    const int64_t s = sequence_of(a.batch, r);
     if (s < 0 || !counts(a.batch, targets, wide, r)) {
-        fill_row<T, kRowBlock>(out, x.vocab, 0.0f);
+        fill_row<T, BLOCK>(out, x.vocab, 0.0f);
         if (threadIdx.x == 0) {
             logp[r] = 0.0f;
             if (entropy) entropy[r] = 0.0f;
-            partials[r] = p;
+            partials[r] = {0.0, 0.0, 0.0, 0.0, 0.0, 0};
         }
         return;
     }
     if (t >= x.vocab) {
-        fill_row<T, kRowBlock>(out, x.vocab, NAN);
+        fill_row<T, BLOCK>(out, x.vocab, NAN);
         if (threadIdx.x == 0) {
             logp[r] = NAN;
             if (entropy) entropy[r] = NAN;
@@ -748,22 +816,103 @@ __global__ __launch_bounds__(kRowBlock) void policy_loss_logits_kernel(
         }
         return;
     }
-    const float zt = T::one(row, t);
-    const int64_t m = a.reduction == RLX_LOSS_TOKEN_MEAN ? batch_count<kRowBlock>(a.batch, seq_counts, shared_n)
+    const int groups = x.vocab / PER, tid = threadIdx.x;
+    const int target = (int)t, last = groups * PER + tid;          // the elements behind the last whole group, one per lane
+    u32x4 held[NG];
+#pragma unroll
+    for (int n = 0; n < NG; n++) {
+        const int g = n * BLOCK + tid;
+        held[n] = u32x4{T::kLeast, T::kLeast, T::kLeast, T::kLeast};
+        if (g < groups) held[n] = load16_once(row + (int64_t)g * 16);
+    }
+    const float zt = T::one(row, target);
+    const float z_last = last < x.vocab ? T::one(row, last) : -INFINITY;
+
+    typename T::Top top = T::no_top();
+#pragma unroll
+    for (int n = 0; n < NG; n++) T::add_top(top, held[n]);
+    Stat st = {reference_of(fmaxf(T::top_of(top), z_last), k), 0.0f, 0.0f};
+#pragma unroll
+    for (int n = 0; n < NG; n++) {
+        float z[PER];
+        forget(held[n]);
+        T::unpack_finite(held[n], z);
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            const float d = __builtin_fmaf(z[i], k, -st.ref), e = exp2_of(d);
+            st.sum += e;
+            st.dot = __builtin_fmaf(e, d, st.dot);
+        }
+    }
+    {
+        const float d = __builtin_fmaf(z_last, k, -st.ref), e = exp2_of(d);
+        st.sum += e;
+        st.dot = __builtin_fmaf(e, fmaxf(d, kLeastD), st.dot);
+    }
+    for (int g = NG * BLOCK + tid; g < groups; g += BLOCK) {
+        float z[PER];
+        T::unpack(load16(row + (int64_t)g * 16), z);
+        add_logits<true>(st, z, k);
+    }
+    const int64_t m = a.reduction == RLX_LOSS_TOKEN_MEAN ? batch_count<BLOCK>(a.batch, seq_counts, shared_n)
                       : a.reduction == RLX_LOSS_SUM ? 1 : (int64_t)seq_counts[s];
-    const double w = weight_of(a, m);
-    const Row st = row_statistics<T, kRowBlock, true>(row, x.vocab, k, shared);
-    const RowValues v = row_values(st, zt, k, inv_t);
-    const TokenLoss o = token_loss(a, v.logp, a.advantages[a.per_token ? (int64_t)r : s], r);
-    const float ws = (float)w * (inv_t * a.grad_scale);
-    const float g = ws * o.slope, c = DOT ? -(ws * a.entropy_coef) : 0.0f;
-    const RowGrad q = row_gradient(st, v, g, c);
-    write_gradient<T, kRowBlock, DOT>(row, out, x.vocab, k, q, (int)t);
-    if (threadIdx.x == 0) {
-        logp[r] = v.logp;
-        if (entropy) entropy[r] = v.entropy;
-        partials[r] = {w * (double)o.policy, w * (double)o.kl, w * (double)v.entropy, o.clipped ? 1.0 : 0.0,
-                       (double)o.ratio, 1};
+    st = join_block<true, BLOCK>(st, shared);
+    Row rv = {0.0f, st.ref, st.sum, st.dot};
+    if (!ordinary(st.sum)) rv = row_by_maximum<T, BLOCK>(row, x.vocab, k, shared_rare);
+    // the row's few scalars by one wavefront: every wavefront doing the same would hold up the compute unit as long
+    if (tid < 64) {
+        const double w = weight_of(a, m);
+        const RowValues v = row_values(rv, zt, k, inv_t);
+        const TokenLoss o = token_loss(a, v.logp, a.advantages[a.per_token ? (int64_t)r : s], r);
+        const float ws = (float)w * (inv_t * a.grad_scale);
+        if (tid == 0) {
+            shared_grad = row_gradient(rv, v, ws * o.slope, DOT ? -(ws * a.entropy_coef) : 0.0f);
+            logp[r] = v.logp;
+            if (entropy) entropy[r] = v.entropy;
+            partials[r] = {w * (double)o.policy, w * (double)o.kl, w * (double)v.entropy, o.clipped ? 1.0 : 0.0,
+                           (double)o.ratio, 1};
+        }
+    }
+    __syncthreads();
+    const RowGrad q = shared_grad;
+    if (q.shift != 0.0f) {                    // a rare row: element by element
+        for (int j = tid; j < x.vocab; j += BLOCK) {
+            const float d = grad_by_maximum<DOT>(q, T::one(row, j), k);
+            T::put(out, j, j == target ? d + q.hot : d);
+        }
+        return;
+    }
+    const int hot_group = target / PER, hot_at = target % PER;
+#pragma unroll
+    for (int n = 0; n < NG; n++) {
+        const int g = n * BLOCK + tid;
+        float z[PER];
+        forget(held[n]);
+        T::unpack(held[n], z);
+#pragma unroll
+        for (int i = 0; i < PER; i++) z[i] = grad_of<DOT>(q, z[i], k);
+        if (g == hot_group) {
+#pragma unroll
+            for (int i = 0; i < PER; i++)
+                if (i == hot_at) z[i] += q.hot;
+        }
+        if (g < groups) store16_once(out + (int64_t)g * 16, T::pack(z));
+    }
+    for (int g = NG * BLOCK + tid; g < groups; g += BLOCK) {
+        float z[PER];
+        T::unpack(load16(row + (int64_t)g * 16), z);
+#pragma unroll
+        for (int i = 0; i < PER; i++) z[i] = grad_of<DOT>(q, z[i], k);
+        if (g == hot_group) {
+#pragma unroll
+            for (int i = 0; i < PER; i++)
+                if (i == hot_at) z[i] += q.hot;
+        }
+        store16_once(out + (int64_t)g * 16, T::pack(z));
+    }
+    if (last < x.vocab) {
+        const float d = grad_of<DOT>(q, z_last, k);
+        T::put(out, last, last == target ? d + q.hot : d);
     }
 }
 
@@ -1014,6 +1163,22 @@ void for_type(int dtype, Fn f) {
     else f(F32{});
 }
 
+template <int N>
+struct Int {
+    static constexpr int value = N;
+};
+
+// Calls f(lanes, 16-byte groups per lane) for the shape that holds a row of `groups` groups in registers.
+template <typename Fn>
+void for_row_shape(int groups, Fn f) {
+    if (groups <= 256 * 4) f(Int<256>{}, Int<4>{});
+    else if (groups <= 256 * 8) f(Int<256>{}, Int<8>{});
+    else if (groups <= 512 * 8) f(Int<512>{}, Int<8>{});
+    else if (groups <= 512 * 14) f(Int<512>{}, Int<14>{});
+    else if (groups <= 1024 * 12) f(Int<1024>{}, Int<12>{});
+    else f(Int<1024>{}, Int<19>{});
+}
+
 }  // namespace
 
 extern "C" {
@@ -1139,12 +1304,16 @@ int rlx_policy_loss_logits(const rlx_logits* x, const void* targets, int index_t
         const uint32_t here = v.rows - first < kRowsPerLaunch ? v.rows - first : kRowsPerLaunch;
         for_type(x->dtype, [&](auto type) {
             typedef decltype(type) T;
-            if (a.entropy_coef != 0.0f)
-                policy_loss_logits_kernel<T, true><<<dim3(here), dim3(kRowBlock), 0, s>>>(
-                    v, dv, targets, wide, k, inv_t, a, seq_counts, logp, entropy, partials, first);
-            else
-                policy_loss_logits_kernel<T, false><<<dim3(here), dim3(kRowBlock), 0, s>>>(
-                    v, dv, targets, wide, k, inv_t, a, seq_counts, logp, entropy, partials, first);
+            const int groups = v.vocab / T::PER;
+            for_row_shape(groups, [&](auto block, auto ng) {
+                constexpr int BLOCK = decltype(block)::value, NG = decltype(ng)::value;
+                if (a.entropy_coef != 0.0f)
+                    policy_loss_row_kernel<T, BLOCK, NG, true><<<dim3(here), dim3(BLOCK), 0, s>>>(
+                        v, dv, targets, wide, k, inv_t, a, seq_counts, logp, entropy, partials, first);
+                else
+                    policy_loss_row_kernel<T, BLOCK, NG, false><<<dim3(here), dim3(BLOCK), 0, s>>>(
+                        v, dv, targets, wide, k, inv_t, a, seq_counts, logp, entropy, partials, first);
+            });
         });
         RLX_HIP(hipGetLastError());
     }
