@@ -38,7 +38,6 @@ constexpr float kLn2Hi = 0.693145751953125f;              // 15 bits: an integer
 constexpr float kLn2Lo = 1.42860682030941723212e-6f;
 constexpr float kRefMost = 536870912.0f;                  // 2^29
 constexpr float kLeastD = -1e30f;                         // keeps 0 * (-inf) out of sums of p log p
-constexpr float kLeastZ = -1e30f;                         // the same, of a logit
 
 struct Logits {             // rlx_logits as the kernels take it
     char* data;
@@ -63,7 +62,7 @@ __device__ __forceinline__ uint32_t max_f16x2(uint32_t a, uint32_t b) {       //
 
 struct F16 {
     static constexpr int PER = 8, SIZE = 2;
-    static constexpr uint32_t kLeast = 0xfc00fc00u, kLowest = 0xfbfffbffu;      // -inf, -65504
+    static constexpr uint32_t kLeast = 0xfc00fc00u;                             // -inf, twice
     typedef uint32_t Top;                                                       // two running maxima
     static __device__ __forceinline__ Top no_top() { return kLeast; }
     static __device__ __forceinline__ void add_top(Top& t, u32x4 v) {
@@ -72,13 +71,6 @@ struct F16 {
     static __device__ __forceinline__ float top_of(Top t) {
         const f16x2 h = __builtin_bit_cast(f16x2, t);
         return fmaxf((float)h[0], (float)h[1]);
-    }
-    // the values with -inf as the lowest number (for sums of p log p)
-    static __device__ __forceinline__ void unpack_finite(u32x4 v, float (&f)[8]) {
-        u32x4 w;
-#pragma unroll
-        for (int i = 0; i < 4; i++) w[i] = max_f16x2(v[i], kLowest);
-        unpack(w, f);
     }
     static __device__ __forceinline__ void unpack(u32x4 v, float (&f)[8]) {
 #pragma unroll
@@ -116,11 +108,6 @@ struct BF16 {
         for (int i = 0; i < PER; i++) t = fmaxf(t, f[i]);
     }
     static __device__ __forceinline__ float top_of(Top t) { return t; }
-    static __device__ __forceinline__ void unpack_finite(u32x4 v, float (&f)[PER]) {
-        unpack(v, f);
-#pragma unroll
-        for (int i = 0; i < PER; i++) f[i] = fmaxf(f[i], kLeastZ);
-    }
     static __device__ __forceinline__ void unpack(u32x4 v, float (&f)[8]) {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -158,11 +145,6 @@ struct F32 {
         for (int i = 0; i < PER; i++) t = fmaxf(t, f[i]);
     }
     static __device__ __forceinline__ float top_of(Top t) { return t; }
-    static __device__ __forceinline__ void unpack_finite(u32x4 v, float (&f)[PER]) {
-        unpack(v, f);
-#pragma unroll
-        for (int i = 0; i < PER; i++) f[i] = fmaxf(f[i], kLeastZ);
-    }
     static __device__ __forceinline__ void unpack(u32x4 v, float (&f)[4]) {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -261,6 +243,32 @@ __device__ __forceinline__ T8 wave_sum8(T8 x) {
 // from one pass over the registers to the next, which takes twice the registers.
 __device__ __forceinline__ void forget(u32x4& v) { asm volatile("" : "+v"(v)); }
 
+// A row is its whole 16-byte groups, counted from its first element wherever that lies, and the fewer than PER elements
+// behind them, one per lane.  (Counting from the first 16-byte boundary instead was no faster: 93.0 against 89.5 us for the
+// policy loss of 2,250 rows of 50,257 BF16, and a sum's order would depend on the address.)
+
+// Loads N groups per lane, STEP apart; what lies behind the last group comes as -inf.  The loads are unconditional
+// (lanes without a group read the last one again): a load under a condition makes the compiler wait for it before it
+// issues the next, which took the policy loss of 8,000 rows of 32,000 FP16 from 136 to 246 us.  ONCE: past the
+// caches, for rows that start on a 16-byte boundary (statistics of 4,096 x 151,936 FP16: 187 against 199 us); groups of
+// other rows share cache lines, which would be fetched twice (2,250 rows of 50,257 BF16: 89.5 against 110 us).
+template <typename T, int N, int STEP, bool ONCE>
+__device__ __forceinline__ void load_groups(u32x4 (&held)[N], const char* row, int first, int groups) {
+    if (groups == 0) {                        // fewer elements than a group: nothing may be read
+#pragma unroll
+        for (int n = 0; n < N; n++) held[n] = u32x4{T::kLeast, T::kLeast, T::kLeast, T::kLeast};
+        return;
+    }
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+        const int g = first + n * STEP < groups ? first + n * STEP : groups - 1;
+        held[n] = ONCE ? load16_once(row + (int64_t)g * 16) : load16(row + (int64_t)g * 16);
+    }
+#pragma unroll
+    for (int n = 0; n < N; n++)
+        if (first + n * STEP >= groups) held[n] = u32x4{T::kLeast, T::kLeast, T::kLeast, T::kLeast};
+}
+
 // --- statistics of a row ---------------------------------------------------------------------------------------------
 
 struct Stat {
@@ -272,25 +280,11 @@ __device__ __forceinline__ float reference_of(float top, float k) {
     return fminf(fmaxf(__builtin_ceilf(top * k), -kRefMost), kRefMost);
 }
 
-// Adds N logits to a lane's statistics.
-template <bool DOT, int N>
-__device__ __forceinline__ void add_logits(Stat& s, const float (&z)[N], float k) {
-    float top = z[0];
-#pragma unroll
-    for (int i = 1; i < N; i++) top = fmaxf(top, z[i]);
-    // the reference follows the maximum at a distance of up to 16 powers of two: it moves a few times a row
-    if (top * k > s.ref + 16.0f && s.ref < kRefMost) {
-        const float ref = reference_of(top, k), d = s.ref - ref, f = exp2_of(d);
-        if constexpr (DOT) s.dot = f * (s.dot + d * s.sum);
-        s.sum *= f;
-        s.ref = ref;
-    }
-#pragma unroll
-    for (int i = 0; i < N; i++) {
-        const float d = __builtin_fmaf(z[i], k, -s.ref), e = exp2_of(d);
-        s.sum += e;
-        if constexpr (DOT) s.dot = __builtin_fmaf(e, fmaxf(d, kLeastD), s.dot);
-    }
+template <bool DOT>
+__device__ __forceinline__ Stat joined(Stat a, Stat b) {
+    const float ref = fmaxf(a.ref, b.ref), da = a.ref - ref, db = b.ref - ref;
+    const float fa = exp2_of(da), fb = exp2_of(db);
+    return {ref, a.sum * fa + b.sum * fb, DOT ? fa * (a.dot + da * a.sum) + fb * (b.dot + db * b.sum) : 0.0f};
 }
 
 // Joins the statistics of the first LANES lanes of a wavefront: the largest reference first, then plain sums.
@@ -380,25 +374,29 @@ __device__ __forceinline__ int64_t target_at(const void* targets, int wide, int6
     return wide ? ((const RLX_GLOBAL int64_t*)targets)[r] : (int64_t)((const RLX_GLOBAL int32_t*)targets)[r];
 }
 
-// Statistics of one row by a whole workgroup, streaming.
-template <typename T, int BLOCK, bool DOT>
-__device__ Row row_statistics(const char* row, int vocab, float k, Stat* shared) {
-    constexpr int PER = T::PER;
-    const int groups = vocab / PER;
-    Stat s = kNoStat;
-    for (int g = threadIdx.x; g < groups; g += BLOCK) {
-        float z[PER];
-        T::unpack(load16(row + (int64_t)g * 16), z);
-        add_logits<DOT>(s, z, k);
+// Statistics of up to N groups that a lane holds in registers, and of one loose logit (-inf: none).
+template <typename T, int N, bool DOT>
+__device__ __forceinline__ Stat held_statistics(u32x4 (&held)[N], float loose, float k) {
+    typename T::Top top = T::no_top();
+#pragma unroll
+    for (int n = 0; n < N; n++) T::add_top(top, held[n]);
+    Stat s = {reference_of(fmaxf(T::top_of(top), loose), k), 0.0f, 0.0f};
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+        float z[T::PER];
+        forget(held[n]);
+        T::unpack(held[n], z);
+#pragma unroll
+        for (int i = 0; i < T::PER; i++) {
+            const float d = __builtin_fmaf(z[i], k, -s.ref), e = exp2_of(d);
+            s.sum += e;
+            if constexpr (DOT) s.dot = __builtin_fmaf(e, fmaxf(d, kLeastD), s.dot);
+        }
     }
-    const int j = groups * PER + threadIdx.x;
-    if (j < vocab) {
-        float z[1] = {T::one(row, j)};
-        add_logits<DOT>(s, z, k);
-    }
-    s = join_block<DOT, BLOCK>(s, shared);
-    if (!ordinary(s.sum)) return row_by_maximum<T, BLOCK>(row, vocab, k, shared);
-    return {0.0f, s.ref, s.sum, s.dot};
+    const float d = __builtin_fmaf(loose, k, -s.ref), e = exp2_of(d);
+    s.sum += e;
+    if constexpr (DOT) s.dot = __builtin_fmaf(e, fmaxf(d, kLeastD), s.dot);
+    return s;
 }
 
 // The gradient of a row: -p (b0 + b1 d) with d = (z - shift) k - ref, plus `hot` at the target.
@@ -447,112 +445,149 @@ __device__ void fill_row(char* out, int vocab, float value) {
     if (j < vocab) T::put(out, j, value);
 }
 
+// The gradient of one group, `hot` added if the target is in it (at < 0 or >= PER: it is not).
+template <typename T, bool DOT>
+__device__ __forceinline__ u32x4 grad_group(const RowGrad& q, u32x4 v, float k, int at) {
+    float z[T::PER];
+    T::unpack(v, z);
+#pragma unroll
+    for (int i = 0; i < T::PER; i++) z[i] = grad_of<DOT>(q, z[i], k);
+    if ((unsigned)at < (unsigned)T::PER) {
+#pragma unroll
+        for (int i = 0; i < T::PER; i++)
+            if (i == at) z[i] += q.hot;
+    }
+    return T::pack(z);
+}
+
+// A rare row's gradient: elements from .. to, one at a time.
 template <typename T, int BLOCK, bool DOT>
-__device__ void write_gradient(const char* row, char* out, int vocab, float k, const RowGrad& q, int target) {
-    constexpr int PER = T::PER;
-    const int groups = vocab / PER;
-    if (q.shift != 0.0f) {                    // a rare row: element by element
-        for (int j = threadIdx.x; j < vocab; j += BLOCK) {
-            const float d = grad_by_maximum<DOT>(q, T::one(row, j), k);
-            T::put(out, j, j == target ? d + q.hot : d);
-        }
-        return;
-    }
-    for (int g = threadIdx.x; g < groups; g += BLOCK) {
-        float z[PER];
-        T::unpack(load16(row + (int64_t)g * 16), z);
-#pragma unroll
-        for (int i = 0; i < PER; i++) z[i] = grad_of<DOT>(q, z[i], k);
-        if (g == target / PER) {
-#pragma unroll
-            for (int i = 0; i < PER; i++)
-                if (i == target % PER) z[i] += q.hot;
-        }
-        store16(out + (int64_t)g * 16, T::pack(z));
-    }
-    const int j = groups * PER + threadIdx.x;
-    if (j < vocab) {
-        const float d = grad_of<DOT>(q, T::one(row, j), k);
+__device__ __attribute__((noinline)) void rare_gradient(RowGrad q, const char* row, char* out, int from, int to,
+                                                        float k, int target) {
+    for (int j = from + threadIdx.x; j < to; j += BLOCK) {
+        const float d = grad_by_maximum<DOT>(q, T::one(row, j), k);
         T::put(out, j, j == target ? d + q.hot : d);
     }
 }
 
 // --- kernels over logits ---------------------------------------------------------------------------------------------
 
-constexpr int kRowBlock = 512;
+constexpr int kChunkBlock = 256, kChunkGroups = 4;     // lanes, and 16-byte groups per lane, of a 16 KiB chunk of a row
 
-// One workgroup per row.
+template <typename T>
+__host__ __device__ constexpr int chunk_elems() { return kChunkBlock * kChunkGroups * T::PER; }
+
+// Statistics of one chunk of a row per workgroup: consecutive workgroups read consecutive 16 KiB, so that the addresses
+// in flight stay a narrow window, and a few rows still fill the chip.  The joining launch adds a row's chunks up.
+template <typename T, bool DOT, bool ONCE>
+__global__ __launch_bounds__(kChunkBlock) void chunk_statistics_kernel(Logits x, const void* __restrict__ targets, int wide,
+                                                                       const uint8_t* __restrict__ mask, float k,
+                                                                       Stat* __restrict__ partials,
+                                                                       uint32_t* __restrict__ ticket, uint32_t first) {
+    __shared__ Stat shared[kChunkBlock / 64];
+    const uint32_t r = first + blockIdx.y, c = blockIdx.x;
+    const int tid = threadIdx.x;
+    if (ticket && r == 0 && c == 0 && tid == 0) *ticket = 0;       // for the launch that follows
+    const int64_t t = target_at(targets, wide, r);
+    if (t < 0 || t >= x.vocab || (mask && mask[r] == 0)) return;
+    const char* row = x.data + row_at(x, r) * T::SIZE;
+    const int groups = x.vocab / T::PER, at = (int)c * kChunkBlock * kChunkGroups + tid, j = groups * T::PER + tid;
+    u32x4 held[kChunkGroups];
+    load_groups<T, kChunkGroups, kChunkBlock, ONCE>(held, row, at, groups);
+    const float loose = c == 0 && j < x.vocab ? T::one(row, j) : -INFINITY;
+    Stat s = held_statistics<T, kChunkGroups, DOT>(held, loose, k);
+    s = join_block<DOT, kChunkBlock>(s, shared);
+    if (tid == 0) partials[(int64_t)r * gridDim.x + c] = s;
+}
+
+// A row's statistics from its chunks, by every wavefront for itself.
+template <bool DOT>
+__device__ __forceinline__ Stat join_chunks(const Stat* __restrict__ partials, int chunks) {
+    const int lane = threadIdx.x & 63;
+    Stat s = lane < chunks ? partials[lane] : kNoStat;
+    for (int c = lane + 64; c < chunks; c += 64) s = joined<DOT>(s, partials[c]);
+    return join_wave<DOT, 64>(s);
+}
+
 template <typename T, bool DOT>
-__global__ __launch_bounds__(kRowBlock) void token_logprob_kernel(Logits x, const void* __restrict__ targets, int wide,
-                                                                  float k, float inv_t, float* __restrict__ logp,
-                                                                  float* __restrict__ lse, float* __restrict__ entropy,
-                                                                  uint32_t first) {
-    __shared__ Stat shared[kRowBlock / 64];
+__global__ __launch_bounds__(kChunkBlock) void token_logprob_join_kernel(
+    Logits x, const void* __restrict__ targets, int wide, float k, float inv_t, const Stat* __restrict__ partials, int chunks,
+    float* __restrict__ logp, float* __restrict__ lse, float* __restrict__ entropy, uint32_t first) {
+    __shared__ Stat shared[kChunkBlock / 64];
     const uint32_t r = first + blockIdx.x;
     const int64_t t = target_at(targets, wide, r);
+    RowValues v;
     if (t < 0 || t >= x.vocab) {
-        if (threadIdx.x == 0) {
-            const float v = t < 0 ? 0.0f : NAN;
-            logp[r] = v;
-            lse[r] = v;
-            if (entropy) entropy[r] = v;
-        }
-        return;
+        v.logp = v.lse = v.entropy = t < 0 ? 0.0f : NAN;
+    } else {
+        const char* row = x.data + row_at(x, r) * T::SIZE;
+        const float zt = T::one(row, t);
+        const Stat s = join_chunks<DOT>(partials + (int64_t)r * chunks, chunks);
+        Row rv = {0.0f, s.ref, s.sum, s.dot};
+        if (!ordinary(s.sum)) rv = row_by_maximum<T, kChunkBlock>(row, x.vocab, k, shared);
+        v = row_values(rv, zt, k, inv_t);
     }
-    const char* row = x.data + row_at(x, r) * T::SIZE;
-    const float zt = T::one(row, t);
-    const Row s = row_statistics<T, kRowBlock, DOT>(row, x.vocab, k, shared);
     if (threadIdx.x == 0) {
-        const RowValues v = row_values(s, zt, k, inv_t);
         logp[r] = v.logp;
         lse[r] = v.lse;
         if (entropy) entropy[r] = v.entropy;
     }
 }
 
-// One workgroup per row: dx from the saved lse (and entropy).  p = exp(z - lse) is formed as 2^((z/T - lse) log2 e), the
+// dx from the saved lse (and entropy), one chunk per workgroup.  p = exp(z - lse) is formed as 2^((z/T - lse) log2 e), the
 // difference first, so that the rounding is of the size of log p.
-template <typename T, bool DOT>
-__global__ __launch_bounds__(kRowBlock) void token_logprob_backward_kernel(
+template <typename T, bool DOT, bool ONCE>
+__global__ __launch_bounds__(kChunkBlock) void token_logprob_backward_kernel(
     Logits x, Logits dx, const void* __restrict__ targets, int wide, float inv_t, const float* __restrict__ lse,
     const float* __restrict__ entropy, const float* __restrict__ dlogp, const float* __restrict__ dentropy, uint32_t first) {
     constexpr int PER = T::PER;
-    const uint32_t r = first + blockIdx.x;
+    const uint32_t r = first + blockIdx.y;
+    const int tid = threadIdx.x;
     const int64_t t = target_at(targets, wide, r);
     const char* row = x.data + row_at(x, r) * T::SIZE;
     char* out = dx.data + row_at(dx, r) * T::SIZE;
-    const float g = t < 0 ? 0.0f : dlogp[r], c = (DOT && t >= 0) ? dentropy[r] : 0.0f;
-    if (t >= x.vocab) {
-        fill_row<T, kRowBlock>(out, x.vocab, NAN);
+    const float g = dlogp[r], c = DOT ? dentropy[r] : 0.0f, l = lse[r], h = DOT ? entropy[r] : 0.0f;
+    const bool bad = t >= x.vocab, none = t < 0 || (!bad && g == 0.0f && c == 0.0f);
+    const int groups = x.vocab / PER, at = (int)blockIdx.x * kChunkBlock * kChunkGroups + tid, j = groups * PER + tid;
+    const bool has_loose = blockIdx.x == 0 && j < x.vocab;
+    if (bad || none) {
+        const float value = bad ? NAN : 0.0f;
+        float f[PER];
+#pragma unroll
+        for (int i = 0; i < PER; i++) f[i] = value;
+        const u32x4 v = T::pack(f);
+#pragma unroll
+        for (int n = 0; n < kChunkGroups; n++)
+            if (at + n * kChunkBlock < groups) store16_once(out + (int64_t)(at + n * kChunkBlock) * 16, v);
+        if (has_loose) T::put(out, j, value);
         return;
     }
-    if (g == 0.0f && c == 0.0f) {
-        fill_row<T, kRowBlock>(out, x.vocab, 0.0f);
-        return;
-    }
-    const float l = lse[r], h = DOT ? entropy[r] : 0.0f;
     const float gs = g * inv_t, cs = c * inv_t;
-    const int target = (int)t, groups = x.vocab / PER;
+    const int target = (int)t;
     auto grad = [&](float z) {
         const float lp = __builtin_fmaf(z, inv_t, -l), p = exp2_of(lp * kLog2e);
         if constexpr (DOT) return -p * __builtin_fmaf(cs, fmaxf(lp, kLeastD) + h, gs);
         else return -p * gs;
     };
-    for (int i = threadIdx.x; i < groups; i += kRowBlock) {
+    u32x4 held[kChunkGroups];
+    load_groups<T, kChunkGroups, kChunkBlock, ONCE>(held, row, at, groups);
+    const float loose = has_loose ? T::one(row, j) : 0.0f;
+#pragma unroll
+    for (int n = 0; n < kChunkGroups; n++) {
         float z[PER];
-        T::unpack(load16(row + (int64_t)i * 16), z);
+        T::unpack(held[n], z);
 #pragma unroll
         for (int e = 0; e < PER; e++) z[e] = grad(z[e]);
-        if (i == target / PER) {
+        const int in = target - (at + n * kChunkBlock) * PER;
+        if ((unsigned)in < (unsigned)PER) {
 #pragma unroll
             for (int e = 0; e < PER; e++)
-                if (e == target % PER) z[e] += gs;
+                if (e == in) z[e] += gs;
         }
-        store16(out + (int64_t)i * 16, T::pack(z));
+        if (at + n * kChunkBlock < groups) store16_once(out + (int64_t)(at + n * kChunkBlock) * 16, T::pack(z));
     }
-    const int j = groups * PER + threadIdx.x;
-    if (j < x.vocab) {
-        const float d = grad(T::one(row, j));
+    if (has_loose) {
+        const float d = grad(loose);
         T::put(out, j, j == target ? d + gs : d);
     }
 }
@@ -698,26 +733,55 @@ __device__ __forceinline__ bool counts(const Batch& b, const void* targets, int 
     return !targets || target_at(targets, wide, t) >= 0;
 }
 
-// How many tokens of each sequence count.
+// How many tokens of each sequence count; with `info` also, per token, its sequence, or -1 if it is ignored.
 __global__ __launch_bounds__(kTokenBlock) void sequence_counts_kernel(Batch b, const void* __restrict__ targets, int wide,
-                                                                      int32_t* __restrict__ out) {
+                                                                      int32_t* __restrict__ out, int32_t* __restrict__ info) {
     __shared__ int64_t shared[kTokenBlock / 64];
     for (int64_t s = blockIdx.x; s < b.n_seqs; s += gridDim.x) {
         int64_t begin, end, n = 0;
         sequence_at(b, s, begin, end);
-        for (int64_t t = begin + threadIdx.x; t < end; t += kTokenBlock) n += counts(b, targets, wide, t) ? 1 : 0;
+        for (int64_t t = begin + threadIdx.x; t < end; t += kTokenBlock) {
+            const bool in = counts(b, targets, wide, t);
+            n += in ? 1 : 0;
+            if (info) info[t] = in ? (int32_t)s : -1;
+        }
         n = sum_block<kTokenBlock>(n, shared);
         if (threadIdx.x == 0) out[s] = (int32_t)n;
         __syncthreads();
     }
+    if (info && b.cu) {                       // in front of the first and behind the last sequence
+        int64_t lo, hi, unused;
+        sequence_at(b, 0, lo, unused);
+        sequence_at(b, b.n_seqs - 1, unused, hi);
+        const int64_t step = (int64_t)gridDim.x * kTokenBlock, at = (int64_t)blockIdx.x * kTokenBlock + threadIdx.x;
+        for (int64_t t = at; t < lo; t += step) info[t] = -1;
+        for (int64_t t = hi + at; t < b.tokens; t += step) info[t] = -1;
+    }
 }
 
-// The count that token weights divide by: the sequence's own, or the whole batch's.
-template <int BLOCK>
-__device__ int64_t batch_count(const Batch& b, const int32_t* __restrict__ seq_counts, int64_t* shared) {
+// The counts of all sequences, by one wavefront.
+__device__ __forceinline__ int64_t batch_count(const Batch& b, const int32_t* __restrict__ seq_counts) {
     int64_t n = 0;
-    for (int64_t s = threadIdx.x; s < b.n_seqs; s += BLOCK) n += seq_counts[s];
-    return sum_block<BLOCK>(n, shared);
+    for (int64_t s = threadIdx.x & 63; s < b.n_seqs; s += 64) n += seq_counts[s];
+    return wave_sum8(n);
+}
+
+constexpr int64_t kMostInline = 256;          // sequences whose counts a wavefront adds up by itself
+
+// Leaves the sum in place of the first count, for batches of more sequences.
+__global__ __launch_bounds__(1024) void total_count_kernel(int32_t* __restrict__ seq_counts, int64_t n_seqs) {
+    __shared__ int64_t shared[16];
+    int64_t n = 0;
+    for (int64_t s = threadIdx.x; s < n_seqs; s += 1024) n += seq_counts[s];
+    n = sum_block<1024>(n, shared);
+    if (threadIdx.x == 0) seq_counts[0] = (int32_t)n;
+}
+
+// What the weight of a token of sequence s divides by, by one wavefront.
+__device__ __forceinline__ int64_t count_for(const Policy& a, const int32_t* __restrict__ seq_counts, int64_t s) {
+    if (a.reduction == RLX_LOSS_SUM) return 1;
+    if (a.reduction == RLX_LOSS_SEQUENCE_MEAN) return seq_counts[s];
+    return a.batch.n_seqs > kMostInline ? (int64_t)seq_counts[0] : batch_count(a.batch, seq_counts);
 }
 
 // Policy loss over log-probabilities: a workgroup takes kTokenBlock tokens.
@@ -725,9 +789,9 @@ __global__ __launch_bounds__(kTokenBlock) void policy_loss_kernel(Policy a, cons
                                                                   const int32_t* __restrict__ seq_counts,
                                                                   float* __restrict__ dlogp, float* __restrict__ dentropy,
                                                                   Terms* __restrict__ partials, int64_t first) {
-    __shared__ int64_t shared_n[kTokenBlock / 64], shared_m[kTokenBlock / 64];
+    __shared__ int64_t shared_n[kTokenBlock / 64];
     __shared__ double shared[5 * kTokenBlock / 64];
-    const int64_t total = a.reduction == RLX_LOSS_TOKEN_MEAN ? batch_count<kTokenBlock>(a.batch, seq_counts, shared_n) : 0;
+    const int64_t total = a.reduction == RLX_LOSS_TOKEN_MEAN ? count_for(a, seq_counts, 0) : 0;
     const int64_t t = (first + blockIdx.x) * kTokenBlock + threadIdx.x;
     Terms v = {0.0, 0.0, 0.0, 0.0, 0.0, 0};
     const int64_t s = t < a.batch.tokens ? sequence_of(a.batch, t) : -1;
@@ -745,7 +809,7 @@ __global__ __launch_bounds__(kTokenBlock) void policy_loss_kernel(Policy a, cons
         dlogp[t] = g;
         if (dentropy) dentropy[t] = dh;
     }
-    v = sum_terms<kTokenBlock>(v, shared, shared_m);
+    v = sum_terms<kTokenBlock>(v, shared, shared_n);
     if (threadIdx.x == 0) partials[first + blockIdx.x] = v;
 }
 
@@ -780,139 +844,97 @@ __global__ __launch_bounds__(kStatsBlock) void policy_stats_kernel(const Terms* 
     if (threadIdx.x == 0) write_stats(v, kl_coef, entropy_coef, stats);
 }
 
+struct RowTerms {
+    RowGrad grad;
+    RowValues values;
+    Terms terms;
+};
+
+// Everything that a row's loss and gradient need besides its statistics.  m: count that the weight divides by.
+template <bool DOT>
+__device__ __forceinline__ RowTerms row_terms(const Policy& a, const Row& row, float zt, float advantage, int64_t m, uint32_t r,
+                                              float k, float inv_t) {
+    RowTerms o;
+    const double w = weight_of(a, m);
+    o.values = row_values(row, zt, k, inv_t);
+    const TokenLoss l = token_loss(a, o.values.logp, advantage, r);
+    const float ws = (float)w * (inv_t * a.grad_scale);
+    o.grad = row_gradient(row, o.values, ws * l.slope, DOT ? -(ws * a.entropy_coef) : 0.0f);
+    o.terms = {w * (double)l.policy, w * (double)l.kl, w * (double)o.values.entropy, l.clipped ? 1.0 : 0.0,
+               (double)l.ratio, 1};
+    return o;
+}
+
 // Policy loss from logits: one workgroup per row, the row held in registers between its statistics and its gradient
 // (NG 16-byte groups per lane; a vocabulary beyond BLOCK * NG groups has its rest read a second time, from the
 // last-level cache mostly).
-template <typename T, int BLOCK, int NG, bool DOT>
+template <typename T, int BLOCK, int NG, bool DOT, bool ONCE>
 __global__ __launch_bounds__(BLOCK) void policy_loss_row_kernel(
     Logits x, Logits dx, const void* __restrict__ targets, int wide, float k, float inv_t, Policy a,
-    const int32_t* __restrict__ seq_counts, float* __restrict__ logp, float* __restrict__ entropy,
-    Terms* __restrict__ partials, uint32_t first) {
-    constexpr int PER = T::PER;
+    const int32_t* __restrict__ seq_counts, const int32_t* __restrict__ info, float* __restrict__ logp,
+    float* __restrict__ entropy, Terms* __restrict__ partials, uint32_t first) {
     __shared__ Stat shared[BLOCK / 64];
     __shared__ Stat shared_rare[BLOCK / 64];
     __shared__ RowGrad shared_grad;
-    __shared__ int64_t shared_n[BLOCK / 64];
     const uint32_t r = first + blockIdx.x;
+    const int tid = threadIdx.x;
     const char* row = x.data + row_at(x, r) * T::SIZE;
     char* out = dx.data + row_at(dx, r) * T::SIZE;
+    int64_t s = info[r];
     const int64_t t = target_at(targets, wide, r);
-    const int64_t s = sequence_of(a.batch, r);
-    if (s < 0 || !counts(a.batch, targets, wide, r)) {
-        fill_row<T, BLOCK>(out, x.vocab, 0.0f);
-        if (threadIdx.x == 0) {
-            logp[r] = 0.0f;
-            if (entropy) entropy[r] = 0.0f;
-            partials[r] = {0.0, 0.0, 0.0, 0.0, 0.0, 0};
+    if (s < 0 || t >= x.vocab) {
+        const float value = s < 0 ? 0.0f : NAN;
+        fill_row<T, BLOCK>(out, x.vocab, value);
+        if (tid == 0) {
+            logp[r] = value;
+            if (entropy) entropy[r] = value;
+            partials[r] = {value, value, value, value, value, s < 0 ? 0 : 1};
         }
         return;
     }
-    if (t >= x.vocab) {
-        fill_row<T, BLOCK>(out, x.vocab, NAN);
-        if (threadIdx.x == 0) {
-            logp[r] = NAN;
-            if (entropy) entropy[r] = NAN;
-            partials[r] = {NAN, NAN, NAN, NAN, NAN, 1};
-        }
-        return;
-    }
-    const int groups = x.vocab / PER, tid = threadIdx.x;
-    const int target = (int)t, last = groups * PER + tid;          // the elements behind the last whole group, one per lane
+    s = s < a.batch.n_seqs ? s : a.batch.n_seqs - 1;
+    const int groups = x.vocab / T::PER, j = groups * T::PER + tid, target = (int)t;
     u32x4 held[NG];
-#pragma unroll
-    for (int n = 0; n < NG; n++) {
-        const int g = n * BLOCK + tid;
-        held[n] = u32x4{T::kLeast, T::kLeast, T::kLeast, T::kLeast};
-        if (g < groups) held[n] = load16_once(row + (int64_t)g * 16);
-    }
-    const float zt = T::one(row, target);
-    const float z_last = last < x.vocab ? T::one(row, last) : -INFINITY;
+    load_groups<T, NG, BLOCK, ONCE>(held, row, tid, groups);
+    const float loose = j < x.vocab ? T::one(row, j) : -INFINITY;
+    const float zt = T::one(row, t), advantage = a.advantages[a.per_token ? (int64_t)r : s];
 
-    typename T::Top top = T::no_top();
-#pragma unroll
-    for (int n = 0; n < NG; n++) T::add_top(top, held[n]);
-    Stat st = {reference_of(fmaxf(T::top_of(top), z_last), k), 0.0f, 0.0f};
-#pragma unroll
-    for (int n = 0; n < NG; n++) {
-        float z[PER];
-        forget(held[n]);
-        T::unpack_finite(held[n], z);
-#pragma unroll
-        for (int i = 0; i < PER; i++) {
-            const float d = __builtin_fmaf(z[i], k, -st.ref), e = exp2_of(d);
-            st.sum += e;
-            st.dot = __builtin_fmaf(e, d, st.dot);
-        }
-    }
-    {
-        const float d = __builtin_fmaf(z_last, k, -st.ref), e = exp2_of(d);
-        st.sum += e;
-        st.dot = __builtin_fmaf(e, fmaxf(d, kLeastD), st.dot);
-    }
+    Stat st = held_statistics<T, NG, true>(held, loose, k);
     for (int g = NG * BLOCK + tid; g < groups; g += BLOCK) {
-        float z[PER];
-        T::unpack(load16(row + (int64_t)g * 16), z);
-        add_logits<true>(st, z, k);
+        u32x4 more[1] = {load16(row + (int64_t)g * 16)};
+        st = joined<true>(st, held_statistics<T, 1, true>(more, -INFINITY, k));
     }
-    const int64_t m = a.reduction == RLX_LOSS_TOKEN_MEAN ? batch_count<BLOCK>(a.batch, seq_counts, shared_n)
-                      : a.reduction == RLX_LOSS_SUM ? 1 : (int64_t)seq_counts[s];
     st = join_block<true, BLOCK>(st, shared);
     Row rv = {0.0f, st.ref, st.sum, st.dot};
     if (!ordinary(st.sum)) rv = row_by_maximum<T, BLOCK>(row, x.vocab, k, shared_rare);
     // the row's few scalars by one wavefront: every wavefront doing the same would hold up the compute unit as long
     if (tid < 64) {
-        const double w = weight_of(a, m);
-        const RowValues v = row_values(rv, zt, k, inv_t);
-        const TokenLoss o = token_loss(a, v.logp, a.advantages[a.per_token ? (int64_t)r : s], r);
-        const float ws = (float)w * (inv_t * a.grad_scale);
+        const RowTerms o = row_terms<DOT>(a, rv, zt, advantage, count_for(a, seq_counts, s), r, k, inv_t);
         if (tid == 0) {
-            shared_grad = row_gradient(rv, v, ws * o.slope, DOT ? -(ws * a.entropy_coef) : 0.0f);
-            logp[r] = v.logp;
-            if (entropy) entropy[r] = v.entropy;
-            partials[r] = {w * (double)o.policy, w * (double)o.kl, w * (double)v.entropy, o.clipped ? 1.0 : 0.0,
-                           (double)o.ratio, 1};
+            shared_grad = o.grad;
+            logp[r] = o.values.logp;
+            if (entropy) entropy[r] = o.values.entropy;
+            partials[r] = o.terms;
         }
     }
     __syncthreads();
     const RowGrad q = shared_grad;
-    if (q.shift != 0.0f) {                    // a rare row: element by element
-        for (int j = tid; j < x.vocab; j += BLOCK) {
-            const float d = grad_by_maximum<DOT>(q, T::one(row, j), k);
-            T::put(out, j, j == target ? d + q.hot : d);
-        }
+    if (q.shift != 0.0f) {
+        rare_gradient<T, BLOCK, DOT>(q, row, out, 0, x.vocab, k, target);
         return;
     }
-    const int hot_group = target / PER, hot_at = target % PER;
 #pragma unroll
     for (int n = 0; n < NG; n++) {
         const int g = n * BLOCK + tid;
-        float z[PER];
         forget(held[n]);
-        T::unpack(held[n], z);
-#pragma unroll
-        for (int i = 0; i < PER; i++) z[i] = grad_of<DOT>(q, z[i], k);
-        if (g == hot_group) {
-#pragma unroll
-            for (int i = 0; i < PER; i++)
-                if (i == hot_at) z[i] += q.hot;
-        }
-        if (g < groups) store16_once(out + (int64_t)g * 16, T::pack(z));
+        const u32x4 v = grad_group<T, DOT>(q, held[n], k, target - g * T::PER);
+        if (g < groups) store16_once(out + (int64_t)g * 16, v);
     }
-    for (int g = NG * BLOCK + tid; g < groups; g += BLOCK) {
-        float z[PER];
-        T::unpack(load16(row + (int64_t)g * 16), z);
-#pragma unroll
-        for (int i = 0; i < PER; i++) z[i] = grad_of<DOT>(q, z[i], k);
-        if (g == hot_group) {
-#pragma unroll
-            for (int i = 0; i < PER; i++)
-                if (i == hot_at) z[i] += q.hot;
-        }
-        store16_once(out + (int64_t)g * 16, T::pack(z));
-    }
-    if (last < x.vocab) {
-        const float d = grad_of<DOT>(q, z_last, k);
-        T::put(out, last, last == target ? d + q.hot : d);
+    for (int g = NG * BLOCK + tid; g < groups; g += BLOCK)
+        store16_once(out + (int64_t)g * 16, grad_group<T, DOT>(q, load16(row + (int64_t)g * 16), k, target - g * T::PER));
+    if (j < x.vocab) {
+        const float d = grad_of<DOT>(q, loose, k);
+        T::put(out, j, j == target ? d + q.hot : d);
     }
 }
 
@@ -1086,6 +1108,20 @@ Logits view(const rlx_logits& x) {
     return v;
 }
 
+// 16 KiB chunks that a row is cut into; its loose elements go with the first.
+int64_t chunks_of(const rlx_logits& x) {
+    const int64_t elems = x.dtype == RLX_DTYPE_F32 ? chunk_elems<F32>() : chunk_elems<F16>();
+    return (x.vocab + elems - 1) / elems;
+}
+
+// Whether every row starts on a 16-byte boundary.
+bool rows_aligned(const rlx_logits& x) {
+    const int64_t es = (int64_t)elem_size(x.dtype);
+    const bool grouped = x.group_rows > 0 && x.group_rows < x.rows;
+    return rlx_is_aligned(x.data, 16) && (x.rows == 1 || x.row_stride * es % 16 == 0) &&
+           (!grouped || x.group_stride * es % 16 == 0);
+}
+
 int check_targets(const void* targets, int index_type) {
     if (index_type != RLX_INDEX_I32 && index_type != RLX_INDEX_I64) return RLX_ERR_INVALID_ARG;
     if (!targets) return RLX_ERR_INVALID_ARG;
@@ -1148,11 +1184,26 @@ int make_policy(const rlx_policy_args* p, int64_t tokens, Policy& a) {
     return RLX_OK;
 }
 
-hipError_t launch_counts(const Batch& b, const void* targets, int wide, int32_t* out, hipStream_t s) {
-    if (b.n_seqs == 0) return hipSuccess;
+// Counts of the sequences (and per token its sequence, if info); for the mean over all tokens of many sequences their sum.
+hipError_t launch_counts(const Policy& a, const void* targets, int wide, int32_t* out, int32_t* info, hipStream_t s) {
+    const Batch& b = a.batch;
     const int64_t grid = b.n_seqs < (1 << 20) ? b.n_seqs : (1 << 20);
-    sequence_counts_kernel<<<dim3((unsigned)grid), dim3(kTokenBlock), 0, s>>>(b, targets, wide, out);
+    sequence_counts_kernel<<<dim3((unsigned)grid), dim3(kTokenBlock), 0, s>>>(b, targets, wide, out, info);
+    if (a.reduction == RLX_LOSS_TOKEN_MEAN && b.n_seqs > kMostInline)
+        total_count_kernel<<<dim3(1), dim3(1024), 0, s>>>(out, b.n_seqs);
     return hipGetLastError();
+}
+
+constexpr uint32_t kMostGridY = 65535;
+
+// Calls f(first row, rows) for every launch of a kernel with a grid of (chunks, rows).
+template <typename Fn>
+int for_row_launches(uint32_t rows, uint32_t most, Fn f) {
+    for (uint32_t first = 0; first < rows; first += most) {
+        f(first, rows - first < most ? rows - first : most);
+        RLX_HIP(hipGetLastError());
+    }
+    return RLX_OK;
 }
 
 // Calls f(T{}) for the logit type.
@@ -1163,6 +1214,18 @@ void for_type(int dtype, Fn f) {
     else f(F32{});
 }
 
+template <bool V>
+struct Bool {
+    static constexpr bool value = V;
+};
+
+// Calls f with the two truth values as compile-time ones.
+template <typename Fn>
+void for_flags(bool a, bool b, Fn f) {
+    if (a) b ? f(Bool<true>{}, Bool<true>{}) : f(Bool<true>{}, Bool<false>{});
+    else b ? f(Bool<false>{}, Bool<true>{}) : f(Bool<false>{}, Bool<false>{});
+}
+
 template <int N>
 struct Int {
     static constexpr int value = N;
@@ -1171,7 +1234,9 @@ struct Int {
 // Calls f(lanes, 16-byte groups per lane) for the shape that holds a row of `groups` groups in registers.
 template <typename Fn>
 void for_row_shape(int groups, Fn f) {
-    if (groups <= 256 * 4) f(Int<256>{}, Int<4>{});
+    if (groups <= 64 * 4) f(Int<64>{}, Int<4>{});
+    else if (groups <= 64 * 8) f(Int<64>{}, Int<8>{});
+    else if (groups <= 128 * 8) f(Int<128>{}, Int<8>{});
     else if (groups <= 256 * 8) f(Int<256>{}, Int<8>{});
     else if (groups <= 512 * 8) f(Int<512>{}, Int<8>{});
     else if (groups <= 512 * 14) f(Int<512>{}, Int<14>{});
@@ -1183,7 +1248,10 @@ void for_row_shape(int groups, Fn f) {
 
 extern "C" {
 
-int64_t rlx_token_logprob_workspace(const rlx_logits* x) { return check_logits(x) == RLX_OK ? 0 : -1; }
+int64_t rlx_token_logprob_workspace(const rlx_logits* x) {
+    if (check_logits(x) != RLX_OK) return -1;
+    return x->rows * chunks_of(*x) * (int64_t)sizeof(Stat);
+}
 
 int rlx_token_logprob(const rlx_logits* x, const void* targets, int index_type, float temperature, float* logp,
                       float* lse, float* entropy, void* workspace, int64_t workspace_bytes, void* stream) {
@@ -1195,23 +1263,30 @@ int rlx_token_logprob(const rlx_logits* x, const void* targets, int index_type, 
     if (!logp || !lse) return RLX_ERR_INVALID_ARG;
     if (!floats_aligned({logp, lse, entropy})) return RLX_ERR_MISALIGNED;
     if ((st = check_workspace(workspace, workspace_bytes, rlx_token_logprob_workspace(x))) != RLX_OK) return st;
+    hipStream_t s = (hipStream_t)stream;
     const Logits v = view(*x);
     const float inv_t = 1.0f / temperature, k = kLog2e / temperature;
-    const int wide = index_type == RLX_INDEX_I64;
-    for (uint32_t first = 0; first < v.rows; first += kRowsPerLaunch) {
-        const uint32_t here = v.rows - first < kRowsPerLaunch ? v.rows - first : kRowsPerLaunch;
-        for_type(x->dtype, [&](auto type) {
-            typedef decltype(type) T;
-            if (entropy)
-                token_logprob_kernel<T, true><<<dim3(here), dim3(kRowBlock), 0, (hipStream_t)stream>>>(
-                    v, targets, wide, k, inv_t, logp, lse, entropy, first);
-            else
-                token_logprob_kernel<T, false><<<dim3(here), dim3(kRowBlock), 0, (hipStream_t)stream>>>(
-                    v, targets, wide, k, inv_t, logp, lse, entropy, first);
+    const int wide = index_type == RLX_INDEX_I64, chunks = (int)chunks_of(*x);
+    Stat* partials = (Stat*)workspace;
+    for_type(x->dtype, [&](auto type) {
+        typedef decltype(type) T;
+        for_flags(entropy != nullptr, rows_aligned(*x), [&](auto dot, auto once) {
+            st = for_row_launches(v.rows, kMostGridY, [&](uint32_t first, uint32_t here) {
+                chunk_statistics_kernel<T, decltype(dot)::value, decltype(once)::value>
+                    <<<dim3(chunks, here), dim3(kChunkBlock), 0, s>>>(v, targets, wide, nullptr, k, partials, nullptr, first);
+            });
         });
-        RLX_HIP(hipGetLastError());
-    }
-    return RLX_OK;
+        if (st != RLX_OK) return;
+        st = for_row_launches(v.rows, kRowsPerLaunch, [&](uint32_t first, uint32_t here) {
+            if (entropy)
+                token_logprob_join_kernel<T, true><<<dim3(here), dim3(kChunkBlock), 0, s>>>(
+                    v, targets, wide, k, inv_t, partials, chunks, logp, lse, entropy, first);
+            else
+                token_logprob_join_kernel<T, false><<<dim3(here), dim3(kChunkBlock), 0, s>>>(
+                    v, targets, wide, k, inv_t, partials, chunks, logp, lse, entropy, first);
+        });
+    });
+    return st;
 }
 
 int rlx_token_logprob_backward(const rlx_logits* x, const void* targets, int index_type, float temperature,
@@ -1228,20 +1303,17 @@ int rlx_token_logprob_backward(const rlx_logits* x, const void* targets, int ind
     const Logits v = view(*x), dv = view(*dx);
     const float inv_t = 1.0f / temperature;
     const int wide = index_type == RLX_INDEX_I64;
-    for (uint32_t first = 0; first < v.rows; first += kRowsPerLaunch) {
-        const uint32_t here = v.rows - first < kRowsPerLaunch ? v.rows - first : kRowsPerLaunch;
-        for_type(x->dtype, [&](auto type) {
-            typedef decltype(type) T;
-            if (dentropy)
-                token_logprob_backward_kernel<T, true><<<dim3(here), dim3(kRowBlock), 0, (hipStream_t)stream>>>(
-                    v, dv, targets, wide, inv_t, lse, entropy, dlogp, dentropy, first);
-            else
-                token_logprob_backward_kernel<T, false><<<dim3(here), dim3(kRowBlock), 0, (hipStream_t)stream>>>(
-                    v, dv, targets, wide, inv_t, lse, entropy, dlogp, dentropy, first);
+    for_type(x->dtype, [&](auto type) {
+        typedef decltype(type) T;
+        for_flags(dentropy != nullptr, rows_aligned(*x), [&](auto dot, auto once) {
+            st = for_row_launches(v.rows, kMostGridY, [&](uint32_t first, uint32_t here) {
+                token_logprob_backward_kernel<T, decltype(dot)::value, decltype(once)::value>
+                    <<<dim3((unsigned)chunks_of(*x), here), dim3(kChunkBlock), 0, (hipStream_t)stream>>>(
+                        v, dv, targets, wide, inv_t, lse, entropy, dlogp, dentropy, first);
+            });
         });
-        RLX_HIP(hipGetLastError());
-    }
-    return RLX_OK;
+    });
+    return st;
 }
 
 int64_t rlx_policy_loss_workspace(int64_t tokens, int64_t n_seqs) {
@@ -1262,7 +1334,7 @@ int rlx_policy_loss(const float* logp, int64_t tokens, const rlx_policy_args* ar
     hipStream_t s = (hipStream_t)stream;
     int32_t* seq_counts = (int32_t*)workspace;
     Terms* partials = (Terms*)((char*)workspace + round16(4 * a.batch.n_seqs));
-    if (tokens && a.reduction != RLX_LOSS_SUM) RLX_HIP(launch_counts(a.batch, nullptr, 0, seq_counts, s));
+    if (tokens && a.reduction != RLX_LOSS_SUM) RLX_HIP(launch_counts(a, nullptr, 0, seq_counts, nullptr, s));
     const int64_t blocks = token_blocks(tokens);
     if (blocks) {
         policy_loss_kernel<<<dim3((unsigned)blocks), dim3(kTokenBlock), 0, s>>>(a, logp, seq_counts, dlogp, dentropy,
@@ -1276,7 +1348,7 @@ int rlx_policy_loss(const float* logp, int64_t tokens, const rlx_policy_args* ar
 
 int64_t rlx_policy_loss_logits_workspace(const rlx_logits* x, int64_t n_seqs) {
     if (check_logits(x) != RLX_OK || n_seqs < 0 || n_seqs > kMaxRows) return -1;
-    return round16(4 * n_seqs) + x->rows * (int64_t)sizeof(Terms);
+    return round16(4 * n_seqs) + round16(4 * x->rows) + x->rows * (int64_t)sizeof(Terms);
 }
 
 int rlx_policy_loss_logits(const rlx_logits* x, const void* targets, int index_type, float temperature,
@@ -1298,25 +1370,23 @@ int rlx_policy_loss_logits(const rlx_logits* x, const void* targets, int index_t
     const float inv_t = 1.0f / temperature, k = kLog2e / temperature;
     const int wide = index_type == RLX_INDEX_I64;
     int32_t* seq_counts = (int32_t*)workspace;
-    Terms* partials = (Terms*)((char*)workspace + round16(4 * a.batch.n_seqs));
-    if (v.rows && a.reduction != RLX_LOSS_SUM) RLX_HIP(launch_counts(a.batch, targets, wide, seq_counts, s));
-    for (uint32_t first = 0; first < v.rows; first += kRowsPerLaunch) {
-        const uint32_t here = v.rows - first < kRowsPerLaunch ? v.rows - first : kRowsPerLaunch;
-        for_type(x->dtype, [&](auto type) {
-            typedef decltype(type) T;
-            const int groups = v.vocab / T::PER;
-            for_row_shape(groups, [&](auto block, auto ng) {
-                constexpr int BLOCK = decltype(block)::value, NG = decltype(ng)::value;
-                if (a.entropy_coef != 0.0f)
-                    policy_loss_row_kernel<T, BLOCK, NG, true><<<dim3(here), dim3(BLOCK), 0, s>>>(
-                        v, dv, targets, wide, k, inv_t, a, seq_counts, logp, entropy, partials, first);
-                else
-                    policy_loss_row_kernel<T, BLOCK, NG, false><<<dim3(here), dim3(BLOCK), 0, s>>>(
-                        v, dv, targets, wide, k, inv_t, a, seq_counts, logp, entropy, partials, first);
+    int32_t* info = (int32_t*)((char*)workspace + round16(4 * a.batch.n_seqs));
+    Terms* partials = (Terms*)((char*)info + round16(4 * x->rows));
+    if (v.rows) RLX_HIP(launch_counts(a, targets, wide, seq_counts, info, s));
+    for_type(x->dtype, [&](auto type) {
+        typedef decltype(type) T;
+        for_row_shape(v.vocab / T::PER, [&](auto block, auto ng) {
+            constexpr int BLOCK = decltype(block)::value, NG = decltype(ng)::value;
+            for_flags(a.entropy_coef != 0.0f, rows_aligned(*x), [&](auto dot, auto once) {
+                st = for_row_launches(v.rows, kRowsPerLaunch, [&](uint32_t first, uint32_t here) {
+                    policy_loss_row_kernel<T, BLOCK, NG, decltype(dot)::value, decltype(once)::value>
+                        <<<dim3(here), dim3(BLOCK), 0, s>>>(v, dv, targets, wide, k, inv_t, a, seq_counts, info, logp, entropy,
+                                                            partials, first);
+                });
             });
         });
-        RLX_HIP(hipGetLastError());
-    }
+    });
+    if (st != RLX_OK) return st;
     policy_stats_kernel<<<dim3(1), dim3(kStatsBlock), 0, s>>>(partials, v.rows, a.kl_coef, a.entropy_coef, stats);
     RLX_HIP(hipGetLastError());
     return RLX_OK;
