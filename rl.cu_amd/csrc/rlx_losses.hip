@@ -472,32 +472,49 @@ __device__ __attribute__((noinline)) void rare_gradient(RowGrad q, const char* r
 
 // --- kernels over logits ---------------------------------------------------------------------------------------------
 
-constexpr int kChunkBlock = 256, kChunkGroups = 4;     // lanes, and 16-byte groups per lane, of a 16 KiB chunk of a row
+struct RowOutputs {
+    float *logp, *lse, *entropy;
+};
 
-template <typename T>
-__host__ __device__ constexpr int chunk_elems() { return kChunkBlock * kChunkGroups * T::PER; }
+__device__ __forceinline__ void put_values(const RowOutputs& o, uint32_t r, const RowValues& v) {
+    o.logp[r] = v.logp;
+    o.lse[r] = v.lse;
+    if (o.entropy) o.entropy[r] = v.entropy;
+}
 
-// Statistics of one chunk of a row per workgroup: consecutive workgroups read consecutive 16 KiB, so that the addresses
-// in flight stay a narrow window, and a few rows still fill the chip.  The joining launch adds a row's chunks up.
-template <typename T, bool DOT, bool ONCE>
-__global__ __launch_bounds__(kChunkBlock) void chunk_statistics_kernel(Logits x, const void* __restrict__ targets, int wide,
-                                                                       const uint8_t* __restrict__ mask, float k,
-                                                                       Stat* __restrict__ partials,
-                                                                       uint32_t* __restrict__ ticket, uint32_t first) {
-    __shared__ Stat shared[kChunkBlock / 64];
+// Statistics of one chunk of a row (BLOCK * NG groups) per workgroup: consecutive workgroups read consecutive memory, so
+// that the addresses in flight stay a narrow window, and a few rows still fill the chip.  A row of one chunk is
+// finished here, with `o`; the chunks of longer rows are added up by the joining launch.
+template <typename T, int BLOCK, int NG, bool DOT, bool ONCE>
+__global__ __launch_bounds__(BLOCK) void chunk_statistics_kernel(Logits x, const void* __restrict__ targets, int wide,
+                                                                 const uint8_t* __restrict__ mask, float k, float inv_t,
+                                                                 RowOutputs o, Stat* __restrict__ partials,
+                                                                 uint32_t* __restrict__ ticket, uint32_t first) {
+    __shared__ Stat shared[BLOCK / 64];
     const uint32_t r = first + blockIdx.y, c = blockIdx.x;
     const int tid = threadIdx.x;
     if (ticket && r == 0 && c == 0 && tid == 0) *ticket = 0;       // for the launch that follows
     const int64_t t = target_at(targets, wide, r);
-    if (t < 0 || t >= x.vocab || (mask && mask[r] == 0)) return;
+    if (t < 0 || t >= x.vocab || (mask && mask[r] == 0)) {
+        const float v = t < 0 ? 0.0f : NAN;
+        if (o.logp && tid == 0) put_values(o, r, {v, v, v, v});
+        return;
+    }
     const char* row = x.data + row_at(x, r) * T::SIZE;
-    const int groups = x.vocab / T::PER, at = (int)c * kChunkBlock * kChunkGroups + tid, j = groups * T::PER + tid;
-    u32x4 held[kChunkGroups];
-    load_groups<T, kChunkGroups, kChunkBlock, ONCE>(held, row, at, groups);
+    const int groups = x.vocab / T::PER, at = (int)c * BLOCK * NG + tid, j = groups * T::PER + tid;
+    u32x4 held[NG];
+    load_groups<T, NG, BLOCK, ONCE>(held, row, at, groups);
     const float loose = c == 0 && j < x.vocab ? T::one(row, j) : -INFINITY;
-    Stat s = held_statistics<T, kChunkGroups, DOT>(held, loose, k);
-    s = join_block<DOT, kChunkBlock>(s, shared);
-    if (tid == 0) partials[(int64_t)r * gridDim.x + c] = s;
+    const float zt = o.logp ? T::one(row, t) : 0.0f;
+    Stat s = held_statistics<T, NG, DOT>(held, loose, k);
+    s = join_block<DOT, BLOCK>(s, shared);
+    if (o.logp) {
+        Row rv = {0.0f, s.ref, s.sum, s.dot};
+        if (!ordinary(s.sum)) rv = row_by_maximum<T, BLOCK>(row, x.vocab, k, shared);
+        if (tid == 0) put_values(o, r, row_values(rv, zt, k, inv_t));
+    } else if (tid == 0) {
+        partials[(int64_t)r * gridDim.x + c] = s;
+    }
 }
 
 // A row's statistics from its chunks, by every wavefront for itself.
@@ -509,11 +526,14 @@ __device__ __forceinline__ Stat join_chunks(const Stat* __restrict__ partials, i
     return join_wave<DOT, 64>(s);
 }
 
+constexpr int kJoinBlock = 256;
+
 template <typename T, bool DOT>
-__global__ __launch_bounds__(kChunkBlock) void token_logprob_join_kernel(
-    Logits x, const void* __restrict__ targets, int wide, float k, float inv_t, const Stat* __restrict__ partials, int chunks,
-    float* __restrict__ logp, float* __restrict__ lse, float* __restrict__ entropy, uint32_t first) {
-    __shared__ Stat shared[kChunkBlock / 64];
+__global__ __launch_bounds__(kJoinBlock) void token_logprob_join_kernel(Logits x, const void* __restrict__ targets, int wide,
+                                                                        float k, float inv_t,
+                                                                        const Stat* __restrict__ partials, int chunks,
+                                                                        RowOutputs o, uint32_t first) {
+    __shared__ Stat shared[kJoinBlock / 64];
     const uint32_t r = first + blockIdx.x;
     const int64_t t = target_at(targets, wide, r);
     RowValues v;
@@ -524,20 +544,16 @@ __global__ __launch_bounds__(kChunkBlock) void token_logprob_join_kernel(
         const float zt = T::one(row, t);
         const Stat s = join_chunks<DOT>(partials + (int64_t)r * chunks, chunks);
         Row rv = {0.0f, s.ref, s.sum, s.dot};
-        if (!ordinary(s.sum)) rv = row_by_maximum<T, kChunkBlock>(row, x.vocab, k, shared);
+        if (!ordinary(s.sum)) rv = row_by_maximum<T, kJoinBlock>(row, x.vocab, k, shared);
         v = row_values(rv, zt, k, inv_t);
     }
-    if (threadIdx.x == 0) {
-        logp[r] = v.logp;
-        lse[r] = v.lse;
-        if (entropy) entropy[r] = v.entropy;
-    }
+    if (threadIdx.x == 0) put_values(o, r, v);
 }
 
 // dx from the saved lse (and entropy), one chunk per workgroup.  p = exp(z - lse) is formed as 2^((z/T - lse) log2 e), the
 // difference first, so that the rounding is of the size of log p.
-template <typename T, bool DOT, bool ONCE>
-__global__ __launch_bounds__(kChunkBlock) void token_logprob_backward_kernel(
+template <typename T, int BLOCK, int NG, bool DOT, bool ONCE>
+__global__ __launch_bounds__(BLOCK) void token_logprob_backward_kernel(
     Logits x, Logits dx, const void* __restrict__ targets, int wide, float inv_t, const float* __restrict__ lse,
     const float* __restrict__ entropy, const float* __restrict__ dlogp, const float* __restrict__ dentropy, uint32_t first) {
     constexpr int PER = T::PER;
@@ -548,7 +564,7 @@ __global__ __launch_bounds__(kChunkBlock) void token_logprob_backward_kernel(
     char* out = dx.data + row_at(dx, r) * T::SIZE;
     const float g = dlogp[r], c = DOT ? dentropy[r] : 0.0f, l = lse[r], h = DOT ? entropy[r] : 0.0f;
     const bool bad = t >= x.vocab, none = t < 0 || (!bad && g == 0.0f && c == 0.0f);
-    const int groups = x.vocab / PER, at = (int)blockIdx.x * kChunkBlock * kChunkGroups + tid, j = groups * PER + tid;
+    const int groups = x.vocab / PER, at = (int)blockIdx.x * BLOCK * NG + tid, j = groups * PER + tid;
     const bool has_loose = blockIdx.x == 0 && j < x.vocab;
     if (bad || none) {
         const float value = bad ? NAN : 0.0f;
@@ -557,8 +573,8 @@ __global__ __launch_bounds__(kChunkBlock) void token_logprob_backward_kernel(
         for (int i = 0; i < PER; i++) f[i] = value;
         const u32x4 v = T::pack(f);
 #pragma unroll
-        for (int n = 0; n < kChunkGroups; n++)
-            if (at + n * kChunkBlock < groups) store16_once(out + (int64_t)(at + n * kChunkBlock) * 16, v);
+        for (int n = 0; n < NG; n++)
+            if (at + n * BLOCK < groups) store16_once(out + (int64_t)(at + n * BLOCK) * 16, v);
         if (has_loose) T::put(out, j, value);
         return;
     }
@@ -569,22 +585,22 @@ __global__ __launch_bounds__(kChunkBlock) void token_logprob_backward_kernel(
         if constexpr (DOT) return -p * __builtin_fmaf(cs, fmaxf(lp, kLeastD) + h, gs);
         else return -p * gs;
     };
-    u32x4 held[kChunkGroups];
-    load_groups<T, kChunkGroups, kChunkBlock, ONCE>(held, row, at, groups);
+    u32x4 held[NG];
+    load_groups<T, NG, BLOCK, ONCE>(held, row, at, groups);
     const float loose = has_loose ? T::one(row, j) : 0.0f;
 #pragma unroll
-    for (int n = 0; n < kChunkGroups; n++) {
+    for (int n = 0; n < NG; n++) {
         float z[PER];
         T::unpack(held[n], z);
 #pragma unroll
         for (int e = 0; e < PER; e++) z[e] = grad(z[e]);
-        const int in = target - (at + n * kChunkBlock) * PER;
+        const int in = target - (at + n * BLOCK) * PER;
         if ((unsigned)in < (unsigned)PER) {
 #pragma unroll
             for (int e = 0; e < PER; e++)
                 if (e == in) z[e] += gs;
         }
-        if (at + n * kChunkBlock < groups) store16_once(out + (int64_t)(at + n * kChunkBlock) * 16, T::pack(z));
+        if (at + n * BLOCK < groups) store16_once(out + (int64_t)(at + n * BLOCK) * 16, T::pack(z));
     }
     if (has_loose) {
         const float d = grad(loose);
@@ -1108,10 +1124,27 @@ Logits view(const rlx_logits& x) {
     return v;
 }
 
-// 16 KiB chunks that a row is cut into; its loose elements go with the first.
-int64_t chunks_of(const rlx_logits& x) {
-    const int64_t elems = x.dtype == RLX_DTYPE_F32 ? chunk_elems<F32>() : chunk_elems<F16>();
-    return (x.vocab + elems - 1) / elems;
+int row_groups(const rlx_logits& x) { return (int)(x.vocab / (x.dtype == RLX_DTYPE_F32 ? F32::PER : F16::PER)); }
+
+// How the statistics of rows are cut: lanes and groups per lane of a workgroup, workgroups per row (a row's few elements
+// behind its last whole group go with the first).
+struct Cut {
+    int block, per_lane, chunks;
+};
+
+Cut cut_of(const rlx_logits& x) {
+    const int groups = row_groups(x);
+    Cut c = {64, 8, 1};
+    if (groups <= 64 * 8) return c;
+    c.block = 128;
+    if (groups <= 128 * 8) return c;
+    c.block = 256;
+    c.chunks = (groups + 256 * 8 - 1) / (256 * 8);
+    if (x.rows * c.chunks < 512) {
+        c.per_lane = 2;
+        c.chunks = (groups + 256 * 2 - 1) / (256 * 2);
+    }
+    return c;
 }
 
 // Whether every row starts on a 16-byte boundary.
@@ -1231,6 +1264,14 @@ struct Int {
     static constexpr int value = N;
 };
 
+template <typename Fn>
+void for_cut(const Cut& c, Fn f) {
+    if (c.block == 64) f(Int<64>{}, Int<8>{});
+    else if (c.block == 128) f(Int<128>{}, Int<8>{});
+    else if (c.per_lane == 8) f(Int<256>{}, Int<8>{});
+    else f(Int<256>{}, Int<2>{});
+}
+
 // Calls f(lanes, 16-byte groups per lane) for the shape that holds a row of `groups` groups in registers.
 template <typename Fn>
 void for_row_shape(int groups, Fn f) {
@@ -1250,7 +1291,8 @@ extern "C" {
 
 int64_t rlx_token_logprob_workspace(const rlx_logits* x) {
     if (check_logits(x) != RLX_OK) return -1;
-    return x->rows * chunks_of(*x) * (int64_t)sizeof(Stat);
+    const Cut c = cut_of(*x);
+    return c.chunks > 1 ? x->rows * c.chunks * (int64_t)sizeof(Stat) : 0;
 }
 
 int rlx_token_logprob(const rlx_logits* x, const void* targets, int index_type, float temperature, float* logp,
@@ -1266,24 +1308,30 @@ int rlx_token_logprob(const rlx_logits* x, const void* targets, int index_type, 
     hipStream_t s = (hipStream_t)stream;
     const Logits v = view(*x);
     const float inv_t = 1.0f / temperature, k = kLog2e / temperature;
-    const int wide = index_type == RLX_INDEX_I64, chunks = (int)chunks_of(*x);
+    const int wide = index_type == RLX_INDEX_I64;
+    const Cut cut = cut_of(*x);
+    const RowOutputs o = {logp, lse, entropy}, none = {nullptr, nullptr, nullptr};
     Stat* partials = (Stat*)workspace;
     for_type(x->dtype, [&](auto type) {
         typedef decltype(type) T;
         for_flags(entropy != nullptr, rows_aligned(*x), [&](auto dot, auto once) {
-            st = for_row_launches(v.rows, kMostGridY, [&](uint32_t first, uint32_t here) {
-                chunk_statistics_kernel<T, decltype(dot)::value, decltype(once)::value>
-                    <<<dim3(chunks, here), dim3(kChunkBlock), 0, s>>>(v, targets, wide, nullptr, k, partials, nullptr, first);
+            for_cut(cut, [&](auto block, auto ng) {
+                constexpr int BLOCK = decltype(block)::value, NG = decltype(ng)::value;
+                st = for_row_launches(v.rows, kMostGridY, [&](uint32_t first, uint32_t here) {
+                    chunk_statistics_kernel<T, BLOCK, NG, decltype(dot)::value, decltype(once)::value>
+                        <<<dim3(cut.chunks, here), dim3(BLOCK), 0, s>>>(v, targets, wide, nullptr, k, inv_t,
+                                                                        cut.chunks == 1 ? o : none, partials, nullptr, first);
+                });
             });
         });
-        if (st != RLX_OK) return;
+        if (st != RLX_OK || cut.chunks == 1) return;
         st = for_row_launches(v.rows, kRowsPerLaunch, [&](uint32_t first, uint32_t here) {
             if (entropy)
-                token_logprob_join_kernel<T, true><<<dim3(here), dim3(kChunkBlock), 0, s>>>(
-                    v, targets, wide, k, inv_t, partials, chunks, logp, lse, entropy, first);
+                token_logprob_join_kernel<T, true><<<dim3(here), dim3(kJoinBlock), 0, s>>>(v, targets, wide, k, inv_t,
+                                                                                           partials, cut.chunks, o, first);
             else
-                token_logprob_join_kernel<T, false><<<dim3(here), dim3(kChunkBlock), 0, s>>>(
-                    v, targets, wide, k, inv_t, partials, chunks, logp, lse, entropy, first);
+                token_logprob_join_kernel<T, false><<<dim3(here), dim3(kJoinBlock), 0, s>>>(v, targets, wide, k, inv_t,
+                                                                                            partials, cut.chunks, o, first);
         });
     });
     return st;
@@ -1302,13 +1350,15 @@ int rlx_token_logprob_backward(const rlx_logits* x, const void* targets, int ind
     if (!floats_aligned({lse, entropy, dlogp, dentropy})) return RLX_ERR_MISALIGNED;
     const Logits v = view(*x), dv = view(*dx);
     const float inv_t = 1.0f / temperature;
-    const int wide = index_type == RLX_INDEX_I64;
+    const int wide = index_type == RLX_INDEX_I64, groups = row_groups(*x);
+    const unsigned chunks = groups ? (groups + 255) / 256 : 1;          // 4 KiB of a row per workgroup
     for_type(x->dtype, [&](auto type) {
         typedef decltype(type) T;
         for_flags(dentropy != nullptr, rows_aligned(*x), [&](auto dot, auto once) {
             st = for_row_launches(v.rows, kMostGridY, [&](uint32_t first, uint32_t here) {
-                token_logprob_backward_kernel<T, decltype(dot)::value, decltype(once)::value>
-                    <<<dim3((unsigned)chunks_of(*x), here), dim3(kChunkBlock), 0, (hipStream_t)stream>>>(
+                constexpr bool ONCE = decltype(once)::value;
+                token_logprob_backward_kernel<T, ONCE ? 256 : 128, ONCE ? 1 : 2, decltype(dot)::value, ONCE>
+                    <<<dim3(chunks, here), dim3(ONCE ? 256 : 128), 0, (hipStream_t)stream>>>(
                         v, dv, targets, wide, inv_t, lse, entropy, dlogp, dentropy, first);
             });
         });
