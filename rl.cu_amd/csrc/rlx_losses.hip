@@ -630,16 +630,15 @@ __device__ __forceinline__ void sequence_at(const Batch& b, int64_t s, int64_t& 
     }
 }
 
-// The sequence that token t belongs to, -1 if it lies in front of the first or behind the last.
-__device__ __forceinline__ int64_t sequence_of(const Batch& b, int64_t t) {
-    if (!b.cu) return t / (b.tokens / b.n_seqs);
-    int64_t lo = 0, hi = b.n_seqs + 1;                  // first index whose offset is greater than t
+// How many of the offsets lo .. hi - 1 (ascending) and all in front of them are at most t, given that it is lo .. hi.
+template <typename Ptr>
+__device__ __forceinline__ int64_t offsets_up_to(Ptr cu, int64_t lo, int64_t hi, int64_t t) {
     while (lo < hi) {
         const int64_t mid = (lo + hi) >> 1;
-        if (((const RLX_GLOBAL int32_t*)b.cu)[mid] <= t) lo = mid + 1;
+        if (cu[mid] <= t) lo = mid + 1;
         else hi = mid;
     }
-    return lo == 0 || lo > b.n_seqs ? -1 : lo - 1;
+    return lo;
 }
 
 struct Policy {             // rlx_policy_args as the kernels take it
@@ -685,10 +684,11 @@ struct TokenLoss {
     bool clipped;
 };
 
-__device__ __forceinline__ TokenLoss token_loss(const Policy& a, float logp, float advantage, int64_t t) {
+// old and ref are used only where the batch has them.
+__device__ __forceinline__ TokenLoss token_loss(const Policy& a, float logp, float old, float ref, float advantage) {
     TokenLoss o;
     // the side of the border is decided in FP64: the inputs' difference is exact there
-    const double lr = a.old_logp ? (double)logp - (double)((const RLX_GLOBAL float*)a.old_logp)[t] : 0.0;
+    const double lr = a.old_logp ? (double)logp - (double)old : 0.0;
     o.clipped = advantage >= 0.0f ? lr > a.log_high : lr < a.log_low;
     o.ratio = expf((float)lr);
     // min(rho A, clip(rho) A) without the product of an infinite rho and A = 0
@@ -697,7 +697,7 @@ __device__ __forceinline__ TokenLoss token_loss(const Policy& a, float logp, flo
     o.kl = 0.0f;
     if (a.ref_logp) {
         float em1;
-        kl_of((float)((double)((const RLX_GLOBAL float*)a.ref_logp)[t] - (double)logp), em1, o.kl);
+        kl_of((float)((double)ref - (double)logp), em1, o.kl);
         if (a.kl_coef != 0.0f) o.slope -= a.kl_coef * em1;
     }
     return o;
@@ -749,6 +749,22 @@ __device__ __forceinline__ bool counts(const Batch& b, const void* targets, int 
     return !targets || target_at(targets, wide, t) >= 0;
 }
 
+typedef uint32_t u32x4_bytes __attribute__((ext_vector_type(4), aligned(1)));
+typedef uint32_t u32_bytes __attribute__((aligned(1)));
+
+__device__ __forceinline__ u32x4 load_mask16(const uint8_t* p) { return *(const RLX_GLOBAL u32x4_bytes*)(const RLX_GLOBAL uint8_t*)p; }
+__device__ __forceinline__ uint32_t load_mask4(const uint8_t* p) { return *(const RLX_GLOBAL u32_bytes*)(const RLX_GLOBAL uint8_t*)p; }
+
+// Bytes of a word that are not 0, as their top bits.
+__device__ __forceinline__ uint32_t nonzero_bytes(uint32_t w) { return (((w & 0x7f7f7f7fu) + 0x7f7f7f7fu) | w) & 0x80808080u; }
+
+__device__ __forceinline__ int masked_in(u32x4 v) {
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) n += __builtin_popcount(nonzero_bytes(v[i]));
+    return n;
+}
+
 // How many tokens of each sequence count; with `info` also, per token, its sequence, or -1 if it is ignored.
 __global__ __launch_bounds__(kTokenBlock) void sequence_counts_kernel(Batch b, const void* __restrict__ targets, int wide,
                                                                       int32_t* __restrict__ out, int32_t* __restrict__ info) {
@@ -756,10 +772,18 @@ __global__ __launch_bounds__(kTokenBlock) void sequence_counts_kernel(Batch b, c
     for (int64_t s = blockIdx.x; s < b.n_seqs; s += gridDim.x) {
         int64_t begin, end, n = 0;
         sequence_at(b, s, begin, end);
-        for (int64_t t = begin + threadIdx.x; t < end; t += kTokenBlock) {
-            const bool in = counts(b, targets, wide, t);
-            n += in ? 1 : 0;
-            if (info) info[t] = in ? (int32_t)s : -1;
+        if (info) {
+            for (int64_t t = begin + threadIdx.x; t < end; t += kTokenBlock) {
+                const bool in = counts(b, targets, wide, t);
+                n += in ? 1 : 0;
+                info[t] = in ? (int32_t)s : -1;
+            }
+        } else if (!b.mask) {
+            n = threadIdx.x == 0 ? end - begin : 0;
+        } else {
+            int64_t t = begin + threadIdx.x * 16;
+            for (; t + 16 <= end; t += kTokenBlock * 16) n += masked_in(load_mask16(b.mask + t));
+            for (int64_t u = t; u < end && u < t + 16; u++) n += ((const RLX_GLOBAL uint8_t*)b.mask)[u] != 0;
         }
         n = sum_block<kTokenBlock>(n, shared);
         if (threadIdx.x == 0) out[s] = (int32_t)n;
@@ -782,7 +806,7 @@ __device__ __forceinline__ int64_t batch_count(const Batch& b, const int32_t* __
     return wave_sum8(n);
 }
 
-constexpr int64_t kMostInline = 256;          // sequences whose counts a wavefront adds up by itself
+constexpr int64_t kMostInline = 1024;         // sequences whose counts a wavefront adds up by itself
 
 // Leaves the sum in place of the first count, for batches of more sequences.
 __global__ __launch_bounds__(1024) void total_count_kernel(int32_t* __restrict__ seq_counts, int64_t n_seqs) {
@@ -800,33 +824,124 @@ __device__ __forceinline__ int64_t count_for(const Policy& a, const int32_t* __r
     return a.batch.n_seqs > kMostInline ? (int64_t)seq_counts[0] : batch_count(a.batch, seq_counts);
 }
 
-// Policy loss over log-probabilities: a workgroup takes kTokenBlock tokens.
+// Four consecutive floats at any 4-byte boundary.
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+__device__ __forceinline__ f32x4_any load4(const float* p) { return *(const RLX_GLOBAL f32x4_any*)(const RLX_GLOBAL float*)p; }
+__device__ __forceinline__ void store4(float* p, f32x4_any v) { *(RLX_GLOBAL f32x4_any*)(RLX_GLOBAL float*)p = v; }
+
+// Four consecutive tokens from t on (those at `tokens` and behind are left as zeros) of the per-token arrays.
+struct Tokens4 {
+    f32x4_any logp, old, ref, entropy, advantage;
+    uint32_t in;                   // top bit of byte i: token i is not masked
+};
+
+__device__ __forceinline__ Tokens4 load_tokens(const Policy& a, const float* logp, int64_t t) {
+    Tokens4 o;
+    o.old = o.ref = o.entropy = o.advantage = f32x4_any{0.0f, 0.0f, 0.0f, 0.0f};
+    const uint8_t* mask = a.batch.mask;
+    if (t + 4 <= a.batch.tokens) {
+        o.logp = load4(logp + t);
+        if (a.old_logp) o.old = load4(a.old_logp + t);
+        if (a.ref_logp) o.ref = load4(a.ref_logp + t);
+        if (a.entropy) o.entropy = load4(a.entropy + t);
+        if (a.per_token) o.advantage = load4(a.advantages + t);
+        o.in = mask ? nonzero_bytes(load_mask4(mask + t)) : 0x80808080u;
+    } else {
+        o.logp = f32x4_any{0.0f, 0.0f, 0.0f, 0.0f};
+        o.in = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (t + i >= a.batch.tokens) continue;
+            o.logp[i] = logp[t + i];
+            if (a.old_logp) o.old[i] = a.old_logp[t + i];
+            if (a.ref_logp) o.ref[i] = a.ref_logp[t + i];
+            if (a.entropy) o.entropy[i] = a.entropy[t + i];
+            if (a.per_token) o.advantage[i] = a.advantages[t + i];
+            if (!mask || mask[t + i]) o.in |= 0x80u << (8 * i);
+        }
+    }
+    return o;
+}
+
+// One token's share of the loss; returns its gradients (of logp, of the entropy).
+__device__ __forceinline__ f32x2 add_token(const Policy& a, double w, float logp, float old, float ref, float entropy,
+                                           float advantage, Terms& v) {
+    const TokenLoss o = token_loss(a, logp, old, ref, advantage);
+    v.policy += w * (double)o.policy;
+    v.kl += w * (double)o.kl;
+    v.entropy += w * (double)entropy;
+    v.clipped += o.clipped ? 1.0 : 0.0;
+    v.ratio += (double)o.ratio;
+    v.count++;
+    return f32x2{(float)(w * (double)o.slope) * a.grad_scale, (float)(w * -(double)a.entropy_coef) * a.grad_scale};
+}
+
+constexpr int kTokensPerBlock = 4 * kTokenBlock;
+
+// Policy loss over log-probabilities: a workgroup takes kTokensPerBlock tokens, a lane four in a row.  The sequences of
+// the workgroup's first and last token are searched once; only where they differ does a lane search between them.
 __global__ __launch_bounds__(kTokenBlock) void policy_loss_kernel(Policy a, const float* __restrict__ logp,
                                                                   const int32_t* __restrict__ seq_counts,
                                                                   float* __restrict__ dlogp, float* __restrict__ dentropy,
-                                                                  Terms* __restrict__ partials, int64_t first) {
+                                                                  Terms* __restrict__ partials) {
     __shared__ int64_t shared_n[kTokenBlock / 64];
     __shared__ double shared[5 * kTokenBlock / 64];
-    const int64_t total = a.reduction == RLX_LOSS_TOKEN_MEAN ? count_for(a, seq_counts, 0) : 0;
-    const int64_t t = (first + blockIdx.x) * kTokenBlock + threadIdx.x;
+    const RLX_GLOBAL int32_t* cu = (const RLX_GLOBAL int32_t*)a.batch.cu;
+    const int64_t n_seqs = a.batch.n_seqs, begin = (int64_t)blockIdx.x * kTokensPerBlock, t0 = begin + threadIdx.x * 4;
+    const int64_t last = begin + kTokensPerBlock < a.batch.tokens ? begin + kTokensPerBlock - 1 : a.batch.tokens - 1;
     Terms v = {0.0, 0.0, 0.0, 0.0, 0.0, 0};
-    const int64_t s = t < a.batch.tokens ? sequence_of(a.batch, t) : -1;
-    if (t < a.batch.tokens) {
-        float g = 0.0f, dh = 0.0f;
-        if (s >= 0 && counts(a.batch, nullptr, 0, t)) {
-            const double w = weight_of(a, a.reduction == RLX_LOSS_TOKEN_MEAN ? total
-                                          : a.reduction == RLX_LOSS_SUM ? 1 : (int64_t)seq_counts[s]);
-            const float h = a.entropy ? a.entropy[t] : 0.0f;
-            const TokenLoss o = token_loss(a, logp[t], a.advantages[a.per_token ? t : s], t);
-            g = (float)(w * (double)o.slope) * a.grad_scale;
-            dh = (float)(w * -(double)a.entropy_coef) * a.grad_scale;
-            v = {w * (double)o.policy, w * (double)o.kl, w * (double)h, o.clipped ? 1.0 : 0.0, (double)o.ratio, 1};
+    Tokens4 x;
+    x.in = 0;
+    if (t0 < a.batch.tokens) x = load_tokens(a, logp, t0);
+    // offsets up to a token: its sequence is one less (0: in front of the first, n_seqs + 1: behind the last)
+    int64_t lo, hi, len = 1;
+    if (cu) {
+        lo = offsets_up_to(cu, 0, n_seqs + 1, begin);
+        hi = offsets_up_to(cu, lo, n_seqs + 1, last);
+    } else {
+        len = a.batch.tokens / n_seqs;
+        lo = begin / len + 1;
+        hi = last / len + 1;
+    }
+    const int64_t total = a.reduction == RLX_LOSS_TOKEN_MEAN ? count_for(a, seq_counts, 0) : 1;
+    int64_t at = lo, weighed = -1;
+    if (lo != hi && t0 < a.batch.tokens) at = cu ? offsets_up_to(cu, lo, hi, t0) : t0 / len + 1;
+    double w = 0.0;
+    float advantage = 0.0f;
+    f32x4_any g = {0.0f, 0.0f, 0.0f, 0.0f}, dh = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int64_t t = t0 + i;
+        if (cu) {
+            while (at < hi && cu[at] <= t) at++;
+        } else if (lo != hi) {
+            at = t / len + 1;
         }
-        dlogp[t] = g;
-        if (dentropy) dentropy[t] = dh;
+        if ((x.in >> (8 * i) & 0x80u) && at >= 1 && at <= n_seqs) {
+            if (weighed != at) {
+                weighed = at;
+                w = weight_of(a, a.reduction == RLX_LOSS_SEQUENCE_MEAN ? (int64_t)seq_counts[at - 1] : total);
+                if (!a.per_token) advantage = a.advantages[at - 1];
+            }
+            const f32x2 d = add_token(a, w, x.logp[i], x.old[i], x.ref[i], x.entropy[i],
+                                      a.per_token ? x.advantage[i] : advantage, v);
+            g[i] = d[0];
+            dh[i] = d[1];
+        }
+    }
+    if (t0 + 4 <= a.batch.tokens) {
+        store4(dlogp + t0, g);
+        if (dentropy) store4(dentropy + t0, dh);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (t0 + i >= a.batch.tokens) continue;
+            dlogp[t0 + i] = g[i];
+            if (dentropy) dentropy[t0 + i] = dh[i];
+        }
     }
     v = sum_terms<kTokenBlock>(v, shared, shared_n);
-    if (threadIdx.x == 0) partials[first + blockIdx.x] = v;
+    if (threadIdx.x == 0) partials[blockIdx.x] = v;
 }
 
 __device__ void write_stats(const Terms& v, float kl_coef, float entropy_coef, rlx_policy_stats* stats) {
@@ -836,6 +951,61 @@ __device__ void write_stats(const Terms& v, float kl_coef, float entropy_coef, r
     const double m = v.count > 0 ? (double)v.count : 1.0;
     *stats = {(float)loss, (float)v.policy, (float)v.kl, (float)v.entropy, (float)(v.clipped / m), (float)(v.ratio / m),
               v.count};
+}
+
+// The whole of a small batch in one launch of one workgroup: counts in LDS (integers, so that the order of their
+// additions says nothing), then losses, gradients and statistics.
+constexpr int kSmallBlock = 1024, kSmallTokens = 4 * kSmallBlock, kSmallSeqs = 1024;
+
+__global__ __launch_bounds__(kSmallBlock) void policy_loss_small_kernel(Policy a, const float* __restrict__ logp,
+                                                                        float* __restrict__ dlogp,
+                                                                        float* __restrict__ dentropy,
+                                                                        rlx_policy_stats* __restrict__ stats) {
+    __shared__ double shared[5 * kSmallBlock / 64];
+    __shared__ int64_t shared_n[kSmallBlock / 64];
+    __shared__ int32_t offsets[kSmallSeqs + 1], in_seq[kSmallSeqs];
+    const int n_seqs = (int)a.batch.n_seqs, tid = threadIdx.x;
+    const int64_t t0 = tid * 4;
+    Tokens4 x;
+    x.in = 0;
+    if (t0 < a.batch.tokens) x = load_tokens(a, logp, t0);
+    const int32_t len = n_seqs ? (int32_t)(a.batch.tokens / n_seqs) : 0;
+    for (int s = tid; s <= n_seqs; s += kSmallBlock) offsets[s] = a.batch.cu ? ((const RLX_GLOBAL int32_t*)a.batch.cu)[s] : s * len;
+    for (int s = tid; s < n_seqs; s += kSmallBlock) in_seq[s] = 0;
+    __syncthreads();
+    int at[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        at[i] = -1;
+        if (x.in >> (8 * i) & 0x80u) {
+            const int s = (int)offsets_up_to(offsets, 0, n_seqs + 1, t0 + i) - 1;
+            if (s >= 0 && s < n_seqs) {
+                at[i] = s;
+                atomicAdd(&in_seq[s], 1);
+            }
+        }
+    }
+    __syncthreads();
+    int64_t total = 1;
+    if (a.reduction == RLX_LOSS_TOKEN_MEAN) {
+        total = tid < n_seqs ? in_seq[tid] : 0;
+        total = sum_block<kSmallBlock>(total, shared_n);
+    }
+    Terms v = {0.0, 0.0, 0.0, 0.0, 0.0, 0};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if (t0 + i >= a.batch.tokens) continue;
+        f32x2 d = {0.0f, 0.0f};
+        if (at[i] >= 0) {
+            const double w = weight_of(a, a.reduction == RLX_LOSS_SEQUENCE_MEAN ? (int64_t)in_seq[at[i]] : total);
+            d = add_token(a, w, x.logp[i], x.old[i], x.ref[i], x.entropy[i], a.per_token ? x.advantage[i] : a.advantages[at[i]], v);
+        }
+        dlogp[t0 + i] = d[0];
+        if (dentropy) dentropy[t0 + i] = d[1];
+    }
+    __syncthreads();                               // shared_n held the total
+    v = sum_terms<kSmallBlock>(v, shared, shared_n);
+    if (tid == 0) write_stats(v, a.kl_coef, a.entropy_coef, stats);
 }
 
 constexpr int kStatsBlock = 512;
@@ -868,12 +1038,12 @@ struct RowTerms {
 
 // Everything that a row's loss and gradient need besides its statistics.  m: count that the weight divides by.
 template <bool DOT>
-__device__ __forceinline__ RowTerms row_terms(const Policy& a, const Row& row, float zt, float advantage, int64_t m, uint32_t r,
-                                              float k, float inv_t) {
+__device__ __forceinline__ RowTerms row_terms(const Policy& a, const Row& row, float zt, float old, float ref, float advantage,
+                                              int64_t m, float k, float inv_t) {
     RowTerms o;
     const double w = weight_of(a, m);
     o.values = row_values(row, zt, k, inv_t);
-    const TokenLoss l = token_loss(a, o.values.logp, advantage, r);
+    const TokenLoss l = token_loss(a, o.values.logp, old, ref, advantage);
     const float ws = (float)w * (inv_t * a.grad_scale);
     o.grad = row_gradient(row, o.values, ws * l.slope, DOT ? -(ws * a.entropy_coef) : 0.0f);
     o.terms = {w * (double)l.policy, w * (double)l.kl, w * (double)o.values.entropy, l.clipped ? 1.0 : 0.0,
@@ -914,6 +1084,7 @@ __global__ __launch_bounds__(BLOCK) void policy_loss_row_kernel(
     load_groups<T, NG, BLOCK, ONCE>(held, row, tid, groups);
     const float loose = j < x.vocab ? T::one(row, j) : -INFINITY;
     const float zt = T::one(row, t), advantage = a.advantages[a.per_token ? (int64_t)r : s];
+    const float old = a.old_logp ? a.old_logp[r] : 0.0f, ref = a.ref_logp ? a.ref_logp[r] : 0.0f;
 
     Stat st = held_statistics<T, NG, true>(held, loose, k);
     for (int g = NG * BLOCK + tid; g < groups; g += BLOCK) {
@@ -925,7 +1096,7 @@ __global__ __launch_bounds__(BLOCK) void policy_loss_row_kernel(
     if (!ordinary(st.sum)) rv = row_by_maximum<T, BLOCK>(row, x.vocab, k, shared_rare);
     // the row's few scalars by one wavefront: every wavefront doing the same would hold up the compute unit as long
     if (tid < 64) {
-        const RowTerms o = row_terms<DOT>(a, rv, zt, advantage, count_for(a, seq_counts, s), r, k, inv_t);
+        const RowTerms o = row_terms<DOT>(a, rv, zt, old, ref, advantage, count_for(a, seq_counts, s), k, inv_t);
         if (tid == 0) {
             shared_grad = o.grad;
             logp[r] = o.values.logp;
@@ -992,6 +1163,54 @@ __device__ __forceinline__ PairValues pair_values(const Preference& a, const dou
     return {{loss, diff > 0.0 ? 1.0 : 0.0, diff, reward[0], reward[1]}, {(float)(slope * per[0]), (float)(-slope * per[1])}};
 }
 
+// Sum of the log ratios and number of the counted tokens of one sequence, by LANES lanes.
+struct RatioSum {
+    double sum;
+    int64_t n;
+};
+
+template <int LANES>
+__device__ __forceinline__ RatioSum sum_ratios(const Preference& a, const float* logp, int64_t begin, int64_t end, int lane) {
+    RatioSum o = {0.0, 0};
+    int64_t t = begin + lane * 4;
+    for (; t + 4 <= end; t += LANES * 4) {
+        const f32x4_any x = load4(logp + t), y = a.ref_logp ? load4(a.ref_logp + t) : f32x4_any{0.0f, 0.0f, 0.0f, 0.0f};
+        const uint32_t in = a.batch.mask ? nonzero_bytes(load_mask4(a.batch.mask + t)) : 0x80808080u;
+#pragma unroll
+        for (int i = 0; i < 4; i++) o.sum += in >> (8 * i) & 0x80u ? (double)x[i] - (double)y[i] : 0.0;
+        o.n += __builtin_popcount(in);
+    }
+    for (int64_t u = t; u < end && u < t + 4; u++) {
+        if (a.batch.mask && a.batch.mask[u] == 0) continue;
+        o.sum += (double)logp[u] - (a.ref_logp ? (double)a.ref_logp[u] : 0.0);
+        o.n++;
+    }
+    return o;
+}
+
+template <int LANES>
+__device__ __forceinline__ void put_gradients(const Preference& a, float* dlogp, int64_t begin, int64_t end, float g, int lane) {
+    int64_t t = begin + lane * 4;
+    for (; t + 4 <= end; t += LANES * 4) {
+        const uint32_t in = a.batch.mask ? nonzero_bytes(load_mask4(a.batch.mask + t)) : 0x80808080u;
+        f32x4_any d;
+#pragma unroll
+        for (int i = 0; i < 4; i++) d[i] = in >> (8 * i) & 0x80u ? g : 0.0f;
+        store4(dlogp + t, d);
+    }
+    for (int64_t u = t; u < end && u < t + 4; u++) dlogp[u] = !a.batch.mask || a.batch.mask[u] ? g : 0.0f;
+}
+
+// Zeros for the tokens in front of the first and behind the last sequence; lane `at` of `step`.
+__device__ __forceinline__ void clear_outside(const Preference& a, float* dlogp, int64_t at, int64_t step) {
+    if (!a.batch.cu) return;
+    int64_t lo, hi, unused;
+    sequence_at(a.batch, 0, lo, unused);
+    sequence_at(a.batch, 2 * a.n_pairs - 1, unused, hi);
+    for (int64_t t = at; t < lo; t += step) dlogp[t] = 0.0f;
+    for (int64_t t = hi + at; t < a.batch.tokens; t += step) dlogp[t] = 0.0f;
+}
+
 constexpr int kPairBlock = 512;
 
 // One workgroup per pair: both sums, the pair's loss, and the gradient of its tokens.
@@ -1006,30 +1225,16 @@ __global__ __launch_bounds__(kPairBlock) void preference_loss_kernel(Preference 
 #pragma unroll
     for (int side = 0; side < 2; side++) {
         sequence_at(a.batch, pair + side * a.n_pairs, begin[side], end[side]);
-        sum[side] = 0.0;
-        n[side] = 0;
-        for (int64_t t = begin[side] + threadIdx.x; t < end[side]; t += kPairBlock) {
-            if (!counts(a.batch, nullptr, 0, t)) continue;
-            sum[side] += (double)logp[t] - (a.ref_logp ? (double)((const RLX_GLOBAL float*)a.ref_logp)[t] : 0.0);
-            n[side]++;
-        }
+        const RatioSum o = sum_ratios<kPairBlock>(a, logp, begin[side], end[side], threadIdx.x);
+        sum[side] = o.sum;
+        n[side] = o.n;
     }
     sum_block<kPairBlock, 2>(sum, shared);
     sum_block<kPairBlock, 2>(n, shared_n);
     const PairValues v = pair_values(a, sum, n);
 #pragma unroll
-    for (int side = 0; side < 2; side++)
-        for (int64_t t = begin[side] + threadIdx.x; t < end[side]; t += kPairBlock)
-            dlogp[t] = counts(a.batch, nullptr, 0, t) ? v.grad[side] : 0.0f;
-    // tokens in front of the first and behind the last sequence
-    if (a.batch.cu) {
-        int64_t lo, hi, unused;
-        sequence_at(a.batch, 0, lo, unused);
-        sequence_at(a.batch, 2 * a.n_pairs - 1, unused, hi);
-        const int64_t step = (int64_t)gridDim.x * kPairBlock, at = pair * kPairBlock + threadIdx.x;
-        for (int64_t t = at; t < lo; t += step) dlogp[t] = 0.0f;
-        for (int64_t t = hi + at; t < a.batch.tokens; t += step) dlogp[t] = 0.0f;
-    }
+    for (int side = 0; side < 2; side++) put_gradients<kPairBlock>(a, dlogp, begin[side], end[side], v.grad[side], threadIdx.x);
+    clear_outside(a, dlogp, pair * kPairBlock + threadIdx.x, (int64_t)gridDim.x * kPairBlock);
     if (threadIdx.x == 0) {
         if (rewards) {
             rewards[pair] = (float)v.terms.chosen;
@@ -1037,6 +1242,50 @@ __global__ __launch_bounds__(kPairBlock) void preference_loss_kernel(Preference 
         }
         partials[pair] = v.terms;
     }
+}
+
+__device__ __forceinline__ void write_pair_stats(const double (&v)[5], int64_t n, rlx_preference_stats* stats) {
+    const double m = n > 0 ? 1.0 / (double)n : 0.0;
+    *stats = {(float)(v[0] * m), (float)(v[1] * m), (float)(v[2] * m), (float)(v[3] * m), (float)(v[4] * m)};
+}
+
+// The whole of a small batch in one launch of one workgroup, a wavefront per pair.
+constexpr int64_t kSmallPairs = 32, kSmallPairTokens = 16384;
+
+__global__ __launch_bounds__(1024) void preference_loss_small_kernel(Preference a, const float* __restrict__ logp,
+                                                                     float* __restrict__ dlogp, float* __restrict__ rewards,
+                                                                     rlx_preference_stats* __restrict__ stats) {
+    __shared__ double shared[5 * 16];
+    const int lane = threadIdx.x & 63;
+    double terms[5] = {0.0, 0.0, 0.0, 0.0, 0.0};
+    for (int64_t pair = threadIdx.x >> 6; pair < a.n_pairs; pair += 16) {
+        int64_t begin[2], end[2], n[2];
+        double sum[2];
+#pragma unroll
+        for (int side = 0; side < 2; side++) {
+            sequence_at(a.batch, pair + side * a.n_pairs, begin[side], end[side]);
+            const RatioSum o = sum_ratios<64>(a, logp, begin[side], end[side], lane);
+            sum[side] = wave_sum8(o.sum);
+            n[side] = wave_sum8(o.n);
+        }
+        const PairValues v = pair_values(a, sum, n);
+#pragma unroll
+        for (int side = 0; side < 2; side++) put_gradients<64>(a, dlogp, begin[side], end[side], v.grad[side], lane);
+        if (lane == 0) {
+            if (rewards) {
+                rewards[pair] = (float)v.terms.chosen;
+                rewards[a.n_pairs + pair] = (float)v.terms.rejected;
+            }
+            terms[0] += v.terms.loss;
+            terms[1] += v.terms.correct;
+            terms[2] += v.terms.diff;
+            terms[3] += v.terms.chosen;
+            terms[4] += v.terms.rejected;
+        }
+    }
+    if (a.n_pairs) clear_outside(a, dlogp, threadIdx.x, 1024);
+    sum_block<1024, 5>(terms, shared);
+    if (threadIdx.x == 0) write_pair_stats(terms, a.n_pairs, stats);
 }
 
 __global__ __launch_bounds__(kStatsBlock) void preference_stats_kernel(const PairTerms* __restrict__ partials, int64_t n,
@@ -1052,10 +1301,7 @@ __global__ __launch_bounds__(kStatsBlock) void preference_stats_kernel(const Pai
         v[4] += p.rejected;
     }
     sum_block<kStatsBlock, 5>(v, shared);
-    if (threadIdx.x == 0) {
-        const double m = n > 0 ? 1.0 / (double)n : 0.0;
-        *stats = {(float)(v[0] * m), (float)(v[1] * m), (float)(v[2] * m), (float)(v[3] * m), (float)(v[4] * m)};
-    }
+    if (threadIdx.x == 0) write_pair_stats(v, n, stats);
 }
 
 // --- host side -------------------------------------------------------------------------------------------------------
@@ -1186,7 +1432,10 @@ int check_batch(const Batch& b) {
 }
 
 int64_t round16(int64_t n) { return (n + 15) & ~(int64_t)15; }
-int64_t token_blocks(int64_t tokens) { return (tokens + kTokenBlock - 1) / kTokenBlock; }
+int64_t token_blocks(int64_t tokens) { return (tokens + kTokensPerBlock - 1) / kTokensPerBlock; }
+
+bool small_pairs(int64_t tokens, int64_t n_pairs) { return tokens <= kSmallPairTokens && n_pairs <= kSmallPairs; }
+bool small_batch(int64_t tokens, int64_t n_seqs) { return tokens <= kSmallTokens && n_seqs <= kSmallSeqs; }
 
 int make_policy(const rlx_policy_args* p, int64_t tokens, Policy& a) {
     if (!p) return RLX_ERR_INVALID_ARG;
@@ -1368,6 +1617,7 @@ int rlx_token_logprob_backward(const rlx_logits* x, const void* targets, int ind
 
 int64_t rlx_policy_loss_workspace(int64_t tokens, int64_t n_seqs) {
     if (tokens < 0 || n_seqs < 0 || tokens > kMaxRows || n_seqs > kMaxRows) return -1;
+    if (small_batch(tokens, n_seqs)) return 0;
     return round16(4 * n_seqs) + token_blocks(tokens) * (int64_t)sizeof(Terms);
 }
 
@@ -1382,13 +1632,18 @@ int rlx_policy_loss(const float* logp, int64_t tokens, const rlx_policy_args* ar
     if ((st = check_workspace(workspace, workspace_bytes, rlx_policy_loss_workspace(tokens, a.batch.n_seqs))) != RLX_OK)
         return st;
     hipStream_t s = (hipStream_t)stream;
+    if (small_batch(tokens, a.batch.n_seqs)) {
+        policy_loss_small_kernel<<<dim3(1), dim3(kSmallBlock), 0, s>>>(a, logp, dlogp, dentropy, stats);
+        RLX_HIP(hipGetLastError());
+        return RLX_OK;
+    }
     int32_t* seq_counts = (int32_t*)workspace;
     Terms* partials = (Terms*)((char*)workspace + round16(4 * a.batch.n_seqs));
     if (tokens && a.reduction != RLX_LOSS_SUM) RLX_HIP(launch_counts(a, nullptr, 0, seq_counts, nullptr, s));
     const int64_t blocks = token_blocks(tokens);
     if (blocks) {
         policy_loss_kernel<<<dim3((unsigned)blocks), dim3(kTokenBlock), 0, s>>>(a, logp, seq_counts, dlogp, dentropy,
-                                                                                partials, 0);
+                                                                                partials);
         RLX_HIP(hipGetLastError());
     }
     policy_stats_kernel<<<dim3(1), dim3(kStatsBlock), 0, s>>>(partials, blocks, a.kl_coef, a.entropy_coef, stats);
@@ -1444,7 +1699,7 @@ int rlx_policy_loss_logits(const rlx_logits* x, const void* targets, int index_t
 
 int64_t rlx_preference_loss_workspace(int64_t tokens, int64_t n_pairs) {
     if (tokens < 0 || n_pairs < 0 || tokens > kMaxRows || n_pairs > kMaxRows / 2) return -1;
-    return n_pairs * (int64_t)sizeof(PairTerms);
+    return small_pairs(tokens, n_pairs) ? 0 : n_pairs * (int64_t)sizeof(PairTerms);
 }
 
 int rlx_preference_loss(const float* logp, int64_t tokens, const rlx_preference_args* args, float* dlogp,
@@ -1472,6 +1727,11 @@ int rlx_preference_loss(const float* logp, int64_t tokens, const rlx_preference_
     a.grad_scale = args->grad_scale;
     a.average = args->average ? 1 : 0;
     hipStream_t s = (hipStream_t)stream;
+    if (small_pairs(tokens, a.n_pairs)) {
+        preference_loss_small_kernel<<<dim3(1), dim3(1024), 0, s>>>(a, logp, dlogp, rewards, stats);
+        RLX_HIP(hipGetLastError());
+        return RLX_OK;
+    }
     PairTerms* partials = (PairTerms*)workspace;
     if (a.n_pairs) {
         preference_loss_kernel<<<dim3((unsigned)a.n_pairs), dim3(kPairBlock), 0, s>>>(a, logp, dlogp, rewards, partials);

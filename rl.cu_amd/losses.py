@@ -29,6 +29,28 @@ _DTYPES = {torch.float16: B.DTYPE_F16, torch.float32: B.DTYPE_F32, torch.bfloat1
 _REDUCTIONS = {"sequence": B.LOSS_SEQUENCE_MEAN, "token": B.LOSS_TOKEN_MEAN, "sum": B.LOSS_SUM}
 
 
+# handle of a GPU's current stream; torch's own short cut where it has one (the public way costs 2 us a call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+class _Here:
+    """Stands for torch.cuda.device(...) where that device is the current one already."""
+
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return None
+
+
+_HERE = _Here()
+
+
+def _on(device):
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
 def _on_gpu(name, t):
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError("%s must be a tensor on a GPU" % name)
@@ -53,31 +75,35 @@ def _ptr(name, t, device, dtype, shape):
 def _logits(name, x):
     """The rows of a [..., vocab] tensor as the library takes them."""
     _on_gpu(name, x)
-    if x.dtype not in _DTYPES:
+    dtype = _DTYPES.get(x.dtype)
+    if dtype is None:
         raise ValueError("%s must be float16, bfloat16 or float32, not %s" % (name, x.dtype))
-    if x.dim() < 2 or x.shape[-1] < 1:
+    shape, strides = x.shape, x.stride()
+    if len(shape) < 2 or shape[-1] < 1:
         raise ValueError("%s must have the shape [..., vocab]" % name)
-    vocab = x.shape[-1]
-    if vocab > 1 and x.stride(-1) != 1:
+    vocab = shape[-1]
+    if vocab > 1 and strides[-1] != 1:
         raise ValueError("the last dimension of %s must be contiguous" % name)
+    if len(shape) == 2:
+        rows = shape[0]
+        return B.Logits(x.data_ptr(), rows, vocab, strides[0] if rows > 1 else vocab, 0, 0, dtype, 0)
     # leading dimensions from the last one outwards, merged where one continues the other
-    dims = []
-    for n, step in zip(reversed(x.shape[:-1]), reversed(x.stride()[:-1])):
+    dims, rows = [], 1
+    for n, step in zip(reversed(shape[:-1]), reversed(strides[:-1])):
+        rows *= n
         if n == 1:
             continue
         if dims and step == dims[-1][0] * dims[-1][1]:
             dims[-1][0] *= n
         else:
             dims.append([n, step])
-    rows = x.numel() // vocab
-    if rows == 0:
-        dims = []
+    if rows == 0 or not dims:
+        return B.Logits(x.data_ptr(), rows, vocab, vocab, 0, 0, dtype, 0)
     if len(dims) > 2:
         raise ValueError("the rows of %s lie in more than two strides: make it contiguous" % name)
-    inner = dims[0] if dims else [rows, vocab]
-    outer = dims[1] if len(dims) == 2 else [1, 0]
-    return B.Logits(x.data_ptr(), rows, vocab, inner[1], inner[0] if len(dims) == 2 else 0, outer[1],
-                    _DTYPES[x.dtype], 0)
+    if len(dims) == 1:
+        return B.Logits(x.data_ptr(), rows, vocab, dims[0][1], 0, 0, dtype, 0)
+    return B.Logits(x.data_ptr(), rows, vocab, dims[0][1], dims[0][0], dims[1][1], dtype, 0)
 
 
 def _targets(targets, device, shape):
@@ -87,8 +113,10 @@ def _targets(targets, device, shape):
             B.INDEX_I64 if targets.dtype == torch.int64 else B.INDEX_I32)
 
 
-def _gradient(logits, out):
-    """The gradient's tensor (a new one unless given) and its rows."""
+def _gradient(logits, x, out):
+    """The gradient's tensor (a new one unless given) and its rows; x: those of the logits."""
+    if out is logits:
+        return out, x
     if out is None:
         out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
     elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
@@ -97,13 +125,22 @@ def _gradient(logits, out):
 
 
 def _workspace(nbytes, device, where):
-    if nbytes < 0:
-        raise B.RlxError(B.ERR_INVALID_ARG, where)
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    """(tensor to keep alive, address) of scratch memory."""
+    if nbytes <= 0:
+        if nbytes < 0:
+            raise B.RlxError(B.ERR_INVALID_ARG, where)
+        return None, None
+    t = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return t, t.data_ptr()
 
 
 def _address(t):
     return None if t is None else t.data_ptr()
+
+
+def _floats(like):
+    """A contiguous FP32 tensor in the shape of a contiguous per-token tensor."""
+    return torch.empty_like(like, dtype=torch.float32)
 
 
 def _batch(shape, device, mask, cu_seqlens):
@@ -125,10 +162,6 @@ def _batch(shape, device, mask, cu_seqlens):
     return mask_ptr, _ptr("cu_seqlens", cu_seqlens, device, torch.int32, cu_seqlens.shape), cu_seqlens.numel() - 1
 
 
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
-
-
 def token_logprobs(logits, targets, temperature=1.0, with_entropy=False):
     """Log-probability of targets[...] under softmax(logits / temperature), the log-sum-exp and, if asked, the
     entropy of every row.  Rows with a negative target are ignored (outputs 0)."""
@@ -136,14 +169,12 @@ def token_logprobs(logits, targets, temperature=1.0, with_entropy=False):
     device, shape = logits.device, logits.shape[:-1]
     target_ptr, index_type = _targets(targets, device, shape)
     lib = B.load()
-    with torch.cuda.device(device):
-        logp = torch.empty(shape, dtype=torch.float32, device=device)
-        lse = torch.empty(shape, dtype=torch.float32, device=device)
-        entropy = torch.empty(shape, dtype=torch.float32, device=device) if with_entropy else None
+    with _on(device):
+        logp, lse, entropy = _floats(targets), _floats(targets), _floats(targets) if with_entropy else None
         nbytes = lib.rlx_token_logprob_workspace(C.byref(x))
-        ws = _workspace(nbytes, device, "rlx_token_logprob")
+        ws, ws_ptr = _workspace(nbytes, device, "rlx_token_logprob")
         B.check(lib.rlx_token_logprob(C.byref(x), target_ptr, index_type, temperature, logp.data_ptr(),
-                                      lse.data_ptr(), _address(entropy), _address(ws), nbytes, _stream(device)),
+                                      lse.data_ptr(), _address(entropy), ws_ptr, nbytes, _raw_stream(device.index)),
                 "rlx_token_logprob")
     return TokenLogprobs(logp, lse, entropy)
 
@@ -161,10 +192,10 @@ def token_logprobs_backward(logits, targets, lse, dlogp, temperature=1.0, entrop
     ent_p, dent_p = _ptr("entropy", entropy, device, f32, shape), _ptr("dentropy", dentropy, device, f32, shape)
     if lse_p is None or dlogp_p is None:
         raise ValueError("lse and dlogp are needed")
-    with torch.cuda.device(device):
-        out, dx = _gradient(logits, out)
+    with _on(device):
+        out, dx = _gradient(logits, x, out)
         B.check(B.load().rlx_token_logprob_backward(C.byref(x), target_ptr, index_type, temperature, lse_p, ent_p,
-                                                    dlogp_p, dent_p, C.byref(dx), _stream(device)),
+                                                    dlogp_p, dent_p, C.byref(dx), _raw_stream(device.index)),
                 "rlx_token_logprob_backward")
     return out
 
@@ -184,8 +215,9 @@ def _policy_args(shape, device, advantages, old_logp, ref_logp, entropy, mask, c
 
 
 def _policy_stats(device):
-    buf = torch.empty(8, dtype=torch.float32, device=device)
-    return buf, buf[:6], buf[6:].view(torch.int64)[0]
+    """An rlx_policy_stats on the device and its parts."""
+    buf = torch.empty(4, dtype=torch.int64, device=device)
+    return buf, buf.view(torch.float32)[:6], buf[3]
 
 
 def policy_loss(logp, advantages, old_logp=None, ref_logp=None, entropy=None, mask=None, cu_seqlens=None,
@@ -203,14 +235,13 @@ def policy_loss(logp, advantages, old_logp=None, ref_logp=None, entropy=None, ma
     logp_p = _ptr("logp", logp, device, torch.float32, shape)
     tokens = logp.numel()
     lib = B.load()
-    with torch.cuda.device(device):
-        dlogp = torch.empty(shape, dtype=torch.float32, device=device)
-        dentropy = torch.empty(shape, dtype=torch.float32, device=device) if entropy_coef != 0.0 else None
+    with _on(device):
+        dlogp, dentropy = _floats(logp), _floats(logp) if entropy_coef != 0.0 else None
         buf, stats, count = _policy_stats(device)
         nbytes = lib.rlx_policy_loss_workspace(tokens, args.n_seqs)
-        ws = _workspace(nbytes, device, "rlx_policy_loss")
+        ws, ws_ptr = _workspace(nbytes, device, "rlx_policy_loss")
         B.check(lib.rlx_policy_loss(logp_p, tokens, C.byref(args), dlogp.data_ptr(), _address(dentropy),
-                                    buf.data_ptr(), _address(ws), nbytes, _stream(device)), "rlx_policy_loss")
+                                    buf.data_ptr(), ws_ptr, nbytes, _raw_stream(device.index)), "rlx_policy_loss")
     return PolicyLoss(stats, count, dlogp, dentropy)
 
 
@@ -226,16 +257,15 @@ def policy_loss_logits(logits, targets, advantages, old_logp=None, ref_logp=None
     args = _policy_args(shape, device, advantages, old_logp, ref_logp, None, mask, cu_seqlens, clip_low, clip_high,
                         kl_coef, entropy_coef, reduction, norm, grad_scale)
     lib = B.load()
-    with torch.cuda.device(device):
-        logp = torch.empty(shape, dtype=torch.float32, device=device)
-        entropy = torch.empty(shape, dtype=torch.float32, device=device) if with_entropy else None
-        out, dx = _gradient(logits, out)
+    with _on(device):
+        logp, entropy = _floats(targets), _floats(targets) if with_entropy else None
+        out, dx = _gradient(logits, x, out)
         buf, stats, count = _policy_stats(device)
         nbytes = lib.rlx_policy_loss_logits_workspace(C.byref(x), args.n_seqs)
-        ws = _workspace(nbytes, device, "rlx_policy_loss_logits")
+        ws, ws_ptr = _workspace(nbytes, device, "rlx_policy_loss_logits")
         B.check(lib.rlx_policy_loss_logits(C.byref(x), target_ptr, index_type, temperature, C.byref(args),
                                            logp.data_ptr(), _address(entropy), C.byref(dx), buf.data_ptr(),
-                                           _address(ws), nbytes, _stream(device)), "rlx_policy_loss_logits")
+                                           ws_ptr, nbytes, _raw_stream(device.index)), "rlx_policy_loss_logits")
     return PolicyLossLogits(stats, count, logp, entropy, out)
 
 
@@ -253,13 +283,13 @@ def preference_loss(logp, ref_logp=None, mask=None, cu_seqlens=None, beta=0.1, l
     logp_p = _ptr("logp", logp, device, f32, shape)
     tokens = logp.numel()
     lib = B.load()
-    with torch.cuda.device(device):
-        dlogp = torch.empty(shape, dtype=f32, device=device)
+    with _on(device):
+        dlogp = _floats(logp)
         rewards = torch.empty(n_seqs, dtype=f32, device=device)
         stats = torch.empty(5, dtype=f32, device=device)
         nbytes = lib.rlx_preference_loss_workspace(tokens, args.n_pairs)
-        ws = _workspace(nbytes, device, "rlx_preference_loss")
+        ws, ws_ptr = _workspace(nbytes, device, "rlx_preference_loss")
         B.check(lib.rlx_preference_loss(logp_p, tokens, C.byref(args), dlogp.data_ptr(), rewards.data_ptr(),
-                                        stats.data_ptr(), _address(ws), nbytes, _stream(device)),
+                                        stats.data_ptr(), ws_ptr, nbytes, _raw_stream(device.index)),
                 "rlx_preference_loss")
     return PreferenceLoss(stats, rewards, dlogp)

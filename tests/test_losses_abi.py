@@ -112,7 +112,9 @@ def test_policy_arguments_are_checked(B):
     for kw in BAD_HYPER:
         assert policy(B, policy_args(B, **kw)) == B.ERR_BAD_HYPER, kw
     ok = policy_args(B)
-    for kw in (dict(logp=None), dict(dlogp=None), dict(stats=None), dict(tokens=-1), dict(nbytes=0), dict(ws=None)):
+    many = 100000                                          # tokens of a batch that needs scratch memory
+    for kw in (dict(logp=None), dict(dlogp=None), dict(stats=None), dict(tokens=-1), dict(tokens=many, nbytes=8),
+               dict(tokens=many, ws=None)):
         assert policy(B, ok, **kw) == bad, kw
     assert policy(B, policy_args(B, entropy_coef=0.1), dent=P) == bad            # needs entropy
     assert policy(B, policy_args(B, entropy_coef=0.1, entropy=P)) == bad         # needs dentropy
@@ -123,7 +125,7 @@ def test_policy_arguments_are_checked(B):
     assert policy(B, ok, tokens=1 << 31) == B.ERR_TOO_LARGE
     lib = B.load()
     assert lib.rlx_policy_loss_workspace(-1, 1) == -1 and lib.rlx_policy_loss_workspace(1, -1) == -1
-    assert lib.rlx_policy_loss_workspace(1000, 3) > 0
+    assert lib.rlx_policy_loss_workspace(many, 3) > 8
 
 
 def fused(B, args, x, dx, targets=P, index=0, temp=1.0, logp=P, ent=None, stats=P, ws=P, nbytes=1 << 40):
@@ -159,8 +161,8 @@ def test_preference_arguments_are_checked(B):
         args = B.PreferenceArgs(*[a[f[0]] for f in B.PreferenceArgs._fields_])
         return lib.rlx_preference_loss(logp, tokens, C.byref(args), dlogp, rewards, stats, ws, nbytes, None)
 
-    for kw in (dict(tokens=-1), dict(logp=None), dict(dlogp=None), dict(stats=None), dict(ws=None), dict(nbytes=0),
-               dict(n_pairs=-1), dict(n_pairs=0), dict(reserved=1), dict(cu_seqlens=None, tokens=7)):
+    for kw in (dict(tokens=-1), dict(logp=None), dict(dlogp=None), dict(stats=None), dict(tokens=100000, ws=None),
+               dict(tokens=100000, nbytes=8), dict(n_pairs=-1), dict(n_pairs=0), dict(reserved=1), dict(cu_seqlens=None, tokens=7)):
         assert call(**kw) == bad, kw
     for kw in (dict(beta=float("nan")), dict(label_smoothing=-0.1), dict(label_smoothing=1.5), dict(margin=float("inf")),
                dict(grad_scale=float("nan"))):
@@ -170,7 +172,7 @@ def test_preference_arguments_are_checked(B):
         assert call(**kw) == B.ERR_MISALIGNED, kw
     assert call(n_pairs=1 << 30) == B.ERR_TOO_LARGE
     assert lib.rlx_preference_loss(P, 8, None, P, P, P, P, 1 << 40, None) == bad
-    assert lib.rlx_preference_loss_workspace(-1, 1) == -1 and lib.rlx_preference_loss_workspace(10, 4) > 0
+    assert lib.rlx_preference_loss_workspace(-1, 1) == -1 and lib.rlx_preference_loss_workspace(100000, 4) > 8
 
 
 def test_python_functions_refuse_host_tensors(losses):
