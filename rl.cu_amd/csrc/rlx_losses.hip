@@ -489,6 +489,7 @@ template <typename T, int BLOCK, int NG, bool DOT, bool ONCE>
 __global__ __launch_bounds__(BLOCK) void chunk_statistics_kernel(Logits x, const void* __restrict__ targets, int wide,
                                                                  const uint8_t* __restrict__ mask, float k, float inv_t,
                                                                  RowOutputs o, Stat* __restrict__ partials,
+                                                                 float* __restrict__ target_logits,
                                                                  uint32_t* __restrict__ ticket, uint32_t first) {
     __shared__ Stat shared[BLOCK / 64];
     const uint32_t r = first + blockIdx.y, c = blockIdx.x;
@@ -505,15 +506,17 @@ __global__ __launch_bounds__(BLOCK) void chunk_statistics_kernel(Logits x, const
     u32x4 held[NG];
     load_groups<T, NG, BLOCK, ONCE>(held, row, at, groups);
     const float loose = c == 0 && j < x.vocab ? T::one(row, j) : -INFINITY;
-    const float zt = o.logp ? T::one(row, t) : 0.0f;
+    const bool finish = o.logp != nullptr;
+    const float zt = finish || (target_logits && c == 0) ? T::one(row, t) : 0.0f;
     Stat s = held_statistics<T, NG, DOT>(held, loose, k);
     s = join_block<DOT, BLOCK>(s, shared);
-    if (o.logp) {
+    if (finish) {
         Row rv = {0.0f, s.ref, s.sum, s.dot};
         if (!ordinary(s.sum)) rv = row_by_maximum<T, BLOCK>(row, x.vocab, k, shared);
         if (tid == 0) put_values(o, r, row_values(rv, zt, k, inv_t));
     } else if (tid == 0) {
         partials[(int64_t)r * gridDim.x + c] = s;
+        if (target_logits && c == 0) target_logits[r] = zt;
     }
 }
 
@@ -526,7 +529,7 @@ __device__ __forceinline__ Stat join_chunks(const Stat* __restrict__ partials, i
     return join_wave<DOT, 64>(s);
 }
 
-constexpr int kJoinBlock = 256;
+constexpr int kChunkBlock = 256, kJoinBlock = 256;
 
 template <typename T, bool DOT>
 __global__ __launch_bounds__(kJoinBlock) void token_logprob_join_kernel(Logits x, const void* __restrict__ targets, int wide,
@@ -637,6 +640,18 @@ __device__ __forceinline__ int64_t offsets_up_to(Ptr cu, int64_t lo, int64_t hi,
         const int64_t mid = (lo + hi) >> 1;
         if (cu[mid] <= t) lo = mid + 1;
         else hi = mid;
+    }
+    return lo;
+}
+
+// The same by a whole wavefront for one t: 64 offsets at a time, so two or three dependent loads instead of ten.
+__device__ __forceinline__ int64_t wave_offsets_up_to(const RLX_GLOBAL int32_t* cu, int64_t lo, int64_t hi, int64_t t) {
+    const int lane = threadIdx.x & 63;
+    while (lo < hi) {
+        const int64_t step = (hi - lo + 63) >> 6, at = lo + (lane + 1) * step - 1;
+        const int64_t n = __builtin_popcountll(__ballot(at < hi && cu[at < hi ? at : hi - 1] <= t));
+        lo = lo + n * step < hi ? lo + n * step : hi;
+        hi = lo + step - 1 < hi ? lo + step - 1 : hi;
     }
     return lo;
 }
@@ -829,38 +844,33 @@ typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 __device__ __forceinline__ f32x4_any load4(const float* p) { return *(const RLX_GLOBAL f32x4_any*)(const RLX_GLOBAL float*)p; }
 __device__ __forceinline__ void store4(float* p, f32x4_any v) { *(RLX_GLOBAL f32x4_any*)(RLX_GLOBAL float*)p = v; }
 
-// Four consecutive tokens from t on (those at `tokens` and behind are left as zeros) of the per-token arrays.
+// Four consecutive tokens of the per-token arrays.  Every load is unconditional (arrays that the batch does not have are
+// stood for by logp): one under a condition would be waited for before the next is issued.
 struct Tokens4 {
     f32x4_any logp, old, ref, entropy, advantage;
     uint32_t in;                   // top bit of byte i: token i is not masked
 };
 
+// Tokens t .. t + 3, which must lie in the arrays.
 __device__ __forceinline__ Tokens4 load_tokens(const Policy& a, const float* logp, int64_t t) {
     Tokens4 o;
-    o.old = o.ref = o.entropy = o.advantage = f32x4_any{0.0f, 0.0f, 0.0f, 0.0f};
-    const uint8_t* mask = a.batch.mask;
-    if (t + 4 <= a.batch.tokens) {
-        o.logp = load4(logp + t);
-        if (a.old_logp) o.old = load4(a.old_logp + t);
-        if (a.ref_logp) o.ref = load4(a.ref_logp + t);
-        if (a.entropy) o.entropy = load4(a.entropy + t);
-        if (a.per_token) o.advantage = load4(a.advantages + t);
-        o.in = mask ? nonzero_bytes(load_mask4(mask + t)) : 0x80808080u;
-    } else {
-        o.logp = f32x4_any{0.0f, 0.0f, 0.0f, 0.0f};
-        o.in = 0;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            if (t + i >= a.batch.tokens) continue;
-            o.logp[i] = logp[t + i];
-            if (a.old_logp) o.old[i] = a.old_logp[t + i];
-            if (a.ref_logp) o.ref[i] = a.ref_logp[t + i];
-            if (a.entropy) o.entropy[i] = a.entropy[t + i];
-            if (a.per_token) o.advantage[i] = a.advantages[t + i];
-            if (!mask || mask[t + i]) o.in |= 0x80u << (8 * i);
-        }
-    }
+    o.logp = load4(logp + t);
+    o.old = load4((a.old_logp ? a.old_logp : logp) + t);
+    o.ref = load4((a.ref_logp ? a.ref_logp : logp) + t);
+    o.entropy = load4((a.entropy ? a.entropy : logp) + t);
+    o.advantage = load4((a.per_token ? a.advantages : logp) + t);
+    const uint32_t in = load_mask4(a.batch.mask ? a.batch.mask + t : (const uint8_t*)(logp + t));
+    o.in = a.batch.mask ? nonzero_bytes(in) : 0x80808080u;
+    if (!a.entropy) o.entropy = f32x4_any{0.0f, 0.0f, 0.0f, 0.0f};
     return o;
+}
+
+// Bits of a quad at `at` whose tokens lie in from .. to - 1.
+__device__ __forceinline__ uint32_t tokens_within(int64_t at, int64_t from, int64_t to) {
+    uint32_t in = 0x80808080u;
+    if (from > at) in = from - at >= 4 ? 0 : in << (8 * (from - at));
+    if (to < at + 4) in &= to <= at ? 0 : 0x80808080u >> (8 * (at + 4 - to));
+    return in;
 }
 
 // One token's share of the loss; returns its gradients (of logp, of the entropy).
@@ -878,8 +888,9 @@ __device__ __forceinline__ f32x2 add_token(const Policy& a, double w, float logp
 
 constexpr int kTokensPerBlock = 4 * kTokenBlock;
 
-// Policy loss over log-probabilities: a workgroup takes kTokensPerBlock tokens, a lane four in a row.  The sequences of
-// the workgroup's first and last token are searched once; only where they differ does a lane search between them.
+// Policy loss over log-probabilities (of at least four tokens): a workgroup takes kTokensPerBlock tokens, a lane four in a
+// row; the quads of the lanes at the end of the arrays move back into them.  The sequences of a workgroup's first
+// and last token are searched once; only where they differ does a lane search between them.
 __global__ __launch_bounds__(kTokenBlock) void policy_loss_kernel(Policy a, const float* __restrict__ logp,
                                                                   const int32_t* __restrict__ seq_counts,
                                                                   float* __restrict__ dlogp, float* __restrict__ dentropy,
@@ -887,27 +898,27 @@ __global__ __launch_bounds__(kTokenBlock) void policy_loss_kernel(Policy a, cons
     __shared__ int64_t shared_n[kTokenBlock / 64];
     __shared__ double shared[5 * kTokenBlock / 64];
     const RLX_GLOBAL int32_t* cu = (const RLX_GLOBAL int32_t*)a.batch.cu;
-    const int64_t n_seqs = a.batch.n_seqs, begin = (int64_t)blockIdx.x * kTokensPerBlock, t0 = begin + threadIdx.x * 4;
-    const int64_t last = begin + kTokensPerBlock < a.batch.tokens ? begin + kTokensPerBlock - 1 : a.batch.tokens - 1;
-    Terms v = {0.0, 0.0, 0.0, 0.0, 0.0, 0};
-    Tokens4 x;
-    x.in = 0;
-    if (t0 < a.batch.tokens) x = load_tokens(a, logp, t0);
+    const int64_t n_seqs = a.batch.n_seqs, tokens = a.batch.tokens, begin = (int64_t)blockIdx.x * kTokensPerBlock;
+    const int64_t own = begin + threadIdx.x * 4, t0 = own + 4 <= tokens ? own : tokens - 4;
+    const int64_t end = begin + kTokensPerBlock < tokens ? begin + kTokensPerBlock : tokens;
+    Tokens4 x = load_tokens(a, logp, t0);
+    x.in &= tokens_within(t0, own, tokens);
     // offsets up to a token: its sequence is one less (0: in front of the first, n_seqs + 1: behind the last)
     int64_t lo, hi, len = 1;
     if (cu) {
-        lo = offsets_up_to(cu, 0, n_seqs + 1, begin);
-        hi = offsets_up_to(cu, lo, n_seqs + 1, last);
+        lo = wave_offsets_up_to(cu, 0, n_seqs + 1, begin);
+        hi = wave_offsets_up_to(cu, lo, n_seqs + 1, end - 1);
     } else {
-        len = a.batch.tokens / n_seqs;
+        len = tokens / n_seqs;
         lo = begin / len + 1;
-        hi = last / len + 1;
+        hi = (end - 1) / len + 1;
     }
     const int64_t total = a.reduction == RLX_LOSS_TOKEN_MEAN ? count_for(a, seq_counts, 0) : 1;
     int64_t at = lo, weighed = -1;
-    if (lo != hi && t0 < a.batch.tokens) at = cu ? offsets_up_to(cu, lo, hi, t0) : t0 / len + 1;
+    if (lo != hi) at = cu ? offsets_up_to(cu, lo, hi, t0) : t0 / len + 1;
     double w = 0.0;
     float advantage = 0.0f;
+    Terms v = {0.0, 0.0, 0.0, 0.0, 0.0, 0};
     f32x4_any g = {0.0f, 0.0f, 0.0f, 0.0f}, dh = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < 4; i++) {
@@ -929,13 +940,13 @@ __global__ __launch_bounds__(kTokenBlock) void policy_loss_kernel(Policy a, cons
             dh[i] = d[1];
         }
     }
-    if (t0 + 4 <= a.batch.tokens) {
+    if (t0 == own) {
         store4(dlogp + t0, g);
         if (dentropy) store4(dentropy + t0, dh);
     } else {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            if (t0 + i >= a.batch.tokens) continue;
+            if (t0 + i < own) continue;
             dlogp[t0 + i] = g[i];
             if (dentropy) dentropy[t0 + i] = dh[i];
         }
@@ -954,57 +965,82 @@ __device__ void write_stats(const Terms& v, float kl_coef, float entropy_coef, r
 }
 
 // The whole of a small batch in one launch of one workgroup: counts in LDS (integers, so that the order of their
-// additions says nothing), then losses, gradients and statistics.
-constexpr int kSmallBlock = 1024, kSmallTokens = 4 * kSmallBlock, kSmallSeqs = 1024;
+// additions says nothing), then losses, gradients and statistics.  A lane takes the tokens tid, tid + BLOCK, ...
+constexpr int kSmallPerLane = 4, kSmallTokens = 512 * kSmallPerLane, kSmallSeqs = 1024;
 
-__global__ __launch_bounds__(kSmallBlock) void policy_loss_small_kernel(Policy a, const float* __restrict__ logp,
-                                                                        float* __restrict__ dlogp,
-                                                                        float* __restrict__ dentropy,
-                                                                        rlx_policy_stats* __restrict__ stats) {
-    __shared__ double shared[5 * kSmallBlock / 64];
-    __shared__ int64_t shared_n[kSmallBlock / 64];
+template <int BLOCK>
+__global__ __launch_bounds__(BLOCK) void policy_loss_small_kernel(Policy a, const float* __restrict__ logp,
+                                                                  float* __restrict__ dlogp, float* __restrict__ dentropy,
+                                                                  rlx_policy_stats* __restrict__ stats) {
+    __shared__ double shared[5 * BLOCK / 64];
+    __shared__ int64_t shared_n[BLOCK / 64], shared_m[BLOCK / 64];
     __shared__ int32_t offsets[kSmallSeqs + 1], in_seq[kSmallSeqs];
-    const int n_seqs = (int)a.batch.n_seqs, tid = threadIdx.x;
-    const int64_t t0 = tid * 4;
-    Tokens4 x;
-    x.in = 0;
-    if (t0 < a.batch.tokens) x = load_tokens(a, logp, t0);
-    const int32_t len = n_seqs ? (int32_t)(a.batch.tokens / n_seqs) : 0;
-    for (int s = tid; s <= n_seqs; s += kSmallBlock) offsets[s] = a.batch.cu ? ((const RLX_GLOBAL int32_t*)a.batch.cu)[s] : s * len;
-    for (int s = tid; s < n_seqs; s += kSmallBlock) in_seq[s] = 0;
-    __syncthreads();
-    int at[4];
+    const int n_seqs = (int)a.batch.n_seqs, tokens = (int)a.batch.tokens, tid = threadIdx.x;
+    float lp[kSmallPerLane], old[kSmallPerLane], ref[kSmallPerLane], entropy[kSmallPerLane], adv[kSmallPerLane];
+    int at[kSmallPerLane];
+    bool in[kSmallPerLane];
+    if (tokens > 0) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
+        for (int i = 0; i < kSmallPerLane; i++) {           // unconditional loads, the last token's behind the end
+            const int t = tid + i * BLOCK < tokens ? tid + i * BLOCK : tokens - 1;
+            lp[i] = logp[t];
+            old[i] = (a.old_logp ? a.old_logp : logp)[t];
+            ref[i] = (a.ref_logp ? a.ref_logp : logp)[t];
+            entropy[i] = (a.entropy ? a.entropy : logp)[t];
+            adv[i] = (a.per_token ? a.advantages : logp)[t];
+            const uint8_t m = a.batch.mask ? a.batch.mask[t] : *(const uint8_t*)(logp + t);
+            in[i] = tid + i * BLOCK < tokens && (!a.batch.mask || m != 0);
+        }
+    }
+    // more sequences than fit (only with fewer than four tokens): counted by token, offsets left in place
+    const bool many = n_seqs > kSmallSeqs;
+    const int slots = many ? 4 : n_seqs, len = n_seqs ? tokens / n_seqs : 0;
+    if (!many)
+        for (int s = tid; s <= n_seqs; s += BLOCK) offsets[s] = a.batch.cu ? ((const RLX_GLOBAL int32_t*)a.batch.cu)[s] : s * len;
+    for (int s = tid; s < slots; s += BLOCK) in_seq[s] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kSmallPerLane; i++) {
         at[i] = -1;
-        if (x.in >> (8 * i) & 0x80u) {
-            const int s = (int)offsets_up_to(offsets, 0, n_seqs + 1, t0 + i) - 1;
+        if (tokens > 0 && in[i]) {
+            const int t = tid + i * BLOCK;
+            const int s = (int)(many ? offsets_up_to((const RLX_GLOBAL int32_t*)a.batch.cu, 0, n_seqs + 1, t)
+                                     : offsets_up_to(offsets, 0, n_seqs + 1, t)) - 1;
             if (s >= 0 && s < n_seqs) {
                 at[i] = s;
-                atomicAdd(&in_seq[s], 1);
+                if (!many) atomicAdd(&in_seq[s], 1);
+                if (!a.per_token) adv[i] = a.advantages[s];
             }
         }
     }
+    if (many) {                                     // the tokens are lanes 0 .. 2 of the first wavefront
+        if (tid < 64) {
+            const int s0 = __builtin_amdgcn_readlane(at[0], 0), s1 = __builtin_amdgcn_readlane(at[0], 1);
+            const int s2 = __builtin_amdgcn_readlane(at[0], 2);
+            if (tid < 4) in_seq[tid] = at[0] < 0 ? 0 : (s0 == at[0]) + (s1 == at[0]) + (s2 == at[0]);
+        }
+    }
     __syncthreads();
-    int64_t total = 1;
+    int64_t total = 0;
     if (a.reduction == RLX_LOSS_TOKEN_MEAN) {
-        total = tid < n_seqs ? in_seq[tid] : 0;
-        total = sum_block<kSmallBlock>(total, shared_n);
+        // of the few tokens of many sequences: each once
+        for (int s = tid; s < slots; s += BLOCK) total += many ? (in_seq[s] > 0 ? 1 : 0) : in_seq[s];
+        total = sum_block<BLOCK>(total, shared_m);
     }
     Terms v = {0.0, 0.0, 0.0, 0.0, 0.0, 0};
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        if (t0 + i >= a.batch.tokens) continue;
+    for (int i = 0; i < kSmallPerLane; i++) {
+        const int t = tid + i * BLOCK;
+        if (t >= tokens) continue;
         f32x2 d = {0.0f, 0.0f};
         if (at[i] >= 0) {
-            const double w = weight_of(a, a.reduction == RLX_LOSS_SEQUENCE_MEAN ? (int64_t)in_seq[at[i]] : total);
-            d = add_token(a, w, x.logp[i], x.old[i], x.ref[i], x.entropy[i], a.per_token ? x.advantage[i] : a.advantages[at[i]], v);
+            const double w = weight_of(a, a.reduction == RLX_LOSS_SEQUENCE_MEAN ? (int64_t)in_seq[many ? tid : at[i]] : total);
+            d = add_token(a, w, lp[i], old[i], ref[i], a.entropy ? entropy[i] : 0.0f, adv[i], v);
         }
-        dlogp[t0 + i] = d[0];
-        if (dentropy) dentropy[t0 + i] = d[1];
+        dlogp[t] = d[0];
+        if (dentropy) dentropy[t] = d[1];
     }
-    __syncthreads();                               // shared_n held the total
-    v = sum_terms<kSmallBlock>(v, shared, shared_n);
+    v = sum_terms<BLOCK>(v, shared, shared_n);
     if (tid == 0) write_stats(v, a.kl_coef, a.entropy_coef, stats);
 }
 
@@ -1125,6 +1161,137 @@ __global__ __launch_bounds__(BLOCK) void policy_loss_row_kernel(
     }
 }
 
+// --- the loss of few rows: chunks of a row in workgroups of their own ------------------------------------------------------
+
+constexpr int kFewGroups = 2;                // 16-byte groups per lane of such a chunk (8 KiB)
+
+// Loads from and stores to memory that other workgroups of the same launch share.
+__device__ __forceinline__ void publish8(void* p, double x) {
+    __hip_atomic_store((uint64_t*)p, __builtin_bit_cast(uint64_t, x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+__device__ __forceinline__ double published8(const void* p) {
+    return __builtin_bit_cast(double, __hip_atomic_load((const uint64_t*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
+
+// How many rows of begin .. end - 1 count, by one wavefront.
+__device__ __forceinline__ int64_t count_rows(const Batch& b, const void* targets, int wide, int64_t begin, int64_t end) {
+    int64_t n = 0;
+    for (int64_t t = begin; t < end; t += 64) {
+        const int64_t u = t + (threadIdx.x & 63);
+        n += __builtin_popcountll(__ballot(u < end && counts(b, targets, wide, u)));
+    }
+    return n;
+}
+
+// The launch behind chunk_statistics_kernel<256, kFewGroups>: every workgroup joins its row's chunks, works out the row's
+// loss for itself and writes its chunk of the gradient; the first chunk's workgroup also writes the row's values.
+// The last of those to finish (the launch in front has cleared the ticket) adds up the rows, in their order.
+// The logits of the targets come from the first launch: here another workgroup may have overwritten them.
+template <typename T, bool DOT>
+__global__ __launch_bounds__(kChunkBlock) void policy_loss_few_kernel(
+    Logits x, Logits dx, const void* __restrict__ targets, int wide, float k, float inv_t, Policy a,
+    const Stat* __restrict__ partials, const float* __restrict__ target_logits, float* __restrict__ logp,
+    float* __restrict__ entropy, Terms* __restrict__ terms, uint32_t* __restrict__ ticket,
+    rlx_policy_stats* __restrict__ stats) {
+    constexpr int PER = T::PER;
+    __shared__ Stat shared[kChunkBlock / 64];
+    __shared__ double sums[5 * kChunkBlock / 64];
+    __shared__ int64_t sums_n[kChunkBlock / 64];
+    __shared__ int last_shared;
+    const uint32_t r = blockIdx.y, c = blockIdx.x;
+    const int tid = threadIdx.x, groups = x.vocab / PER, at = (int)c * kChunkBlock * kFewGroups + tid;
+    const int j = groups * PER + tid;                        // the loose elements go with the first chunk
+    const bool has_loose = c == 0 && j < x.vocab;
+    const char* row = x.data + row_at(x, r) * T::SIZE;
+    char* out = dx.data + row_at(dx, r) * T::SIZE;
+    const RLX_GLOBAL int32_t* cu = (const RLX_GLOBAL int32_t*)a.batch.cu;
+    const int64_t t = target_at(targets, wide, r), n_seqs = a.batch.n_seqs, len = cu ? 1 : a.batch.tokens / n_seqs;
+    const int64_t s = (cu ? wave_offsets_up_to(cu, 0, n_seqs + 1, r) : r / len + 1) - 1;
+    const bool in = s >= 0 && s < n_seqs && counts(a.batch, targets, wide, r), bad = in && t >= x.vocab;
+    RowTerms o;
+    o.values.logp = o.values.entropy = bad ? NAN : 0.0f;
+    o.terms = {0.0, 0.0, 0.0, 0.0, 0.0, 0};
+    if (bad) o.terms = {NAN, NAN, NAN, NAN, NAN, 1};
+    if (!in || bad) {
+        float f[PER];
+#pragma unroll
+        for (int i = 0; i < PER; i++) f[i] = bad ? NAN : 0.0f;
+        const u32x4 v = T::pack(f);
+#pragma unroll
+        for (int n = 0; n < kFewGroups; n++)
+            if (at + n * kChunkBlock < groups) store16_once(out + (int64_t)(at + n * kChunkBlock) * 16, v);
+        if (has_loose) T::put(out, j, f[0]);
+    } else {
+        u32x4 held[kFewGroups];
+        load_groups<T, kFewGroups, kChunkBlock, false>(held, row, at, groups);
+        const float loose = has_loose ? T::one(row, j) : 0.0f;
+        int64_t m = 1;
+        if (a.reduction != RLX_LOSS_SUM) {
+            const bool all = a.reduction == RLX_LOSS_TOKEN_MEAN;
+            int64_t begin, end, unused;
+            sequence_at(a.batch, all ? 0 : s, begin, end);
+            if (all) sequence_at(a.batch, n_seqs - 1, unused, end);
+            m = count_rows(a.batch, targets, wide, begin, end);
+        }
+        const float advantage = a.advantages[a.per_token ? (int64_t)r : s];
+        const float old = a.old_logp ? a.old_logp[r] : 0.0f, ref = a.ref_logp ? a.ref_logp[r] : 0.0f;
+        const Stat st = join_chunks<true>(partials + (int64_t)r * gridDim.x, (int)gridDim.x);
+        const bool rare = !ordinary(st.sum);
+        if (rare && c != 0) return;                          // the first chunk's workgroup does a rare row by itself
+        Row rv = {0.0f, st.ref, st.sum, st.dot};
+        if (rare) rv = row_by_maximum<T, kChunkBlock>(row, x.vocab, k, shared);
+        o = row_terms<DOT>(a, rv, target_logits[r], old, ref, advantage, m, k, inv_t);
+        const int target = (int)t;
+        if (rare) {
+            __syncthreads();                                 // every lane has read what is overwritten now
+            rare_gradient<T, kChunkBlock, DOT>(o.grad, row, out, 0, x.vocab, k, target);
+        } else {
+#pragma unroll
+            for (int n = 0; n < kFewGroups; n++) {
+                const int g = at + n * kChunkBlock;
+                const u32x4 v = grad_group<T, DOT>(o.grad, held[n], k, target - g * PER);
+                if (g < groups) store16_once(out + (int64_t)g * 16, v);
+            }
+            if (has_loose) {
+                const float d = grad_of<DOT>(o.grad, loose, k);
+                T::put(out, j, j == target ? d + o.grad.hot : d);
+            }
+        }
+    }
+    if (c != 0) return;
+    if (tid < 64) {
+        if (tid == 0) {
+            logp[r] = o.values.logp;
+            if (entropy) entropy[r] = o.values.entropy;
+            publish8(&terms[r].policy, o.terms.policy);
+            publish8(&terms[r].kl, o.terms.kl);
+            publish8(&terms[r].entropy, o.terms.entropy);
+            publish8(&terms[r].clipped, o.terms.clipped);
+            publish8(&terms[r].ratio, o.terms.ratio);
+            publish8(&terms[r].count, __builtin_bit_cast(double, o.terms.count));
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // they have arrived before the ticket is taken
+        if (tid == 0)
+            last_shared = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == gridDim.y;
+    }
+    __syncthreads();
+    if (!last_shared) return;
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+    Terms v = {0.0, 0.0, 0.0, 0.0, 0.0, 0};
+    for (uint32_t i = tid; i < gridDim.y; i += kChunkBlock) {
+        v.policy += published8(&terms[i].policy);
+        v.kl += published8(&terms[i].kl);
+        v.entropy += published8(&terms[i].entropy);
+        v.clipped += published8(&terms[i].clipped);
+        v.ratio += published8(&terms[i].ratio);
+        v.count += __builtin_bit_cast(int64_t, published8(&terms[i].count));
+    }
+    v = sum_terms<kChunkBlock>(v, sums, sums_n);
+    if (tid == 0) write_stats(v, a.kl_coef, a.entropy_coef, stats);
+}
+
 // --- preference loss -------------------------------------------------------------------------------------------------
 
 struct Preference {
@@ -1213,27 +1380,83 @@ __device__ __forceinline__ void clear_outside(const Preference& a, float* dlogp,
 
 constexpr int kPairBlock = 512;
 
-// One workgroup per pair: both sums, the pair's loss, and the gradient of its tokens.
+// One workgroup per pair: both sums, the pair's loss, and the gradient of its
+// tokens.  Each lane has its first kPairQuads quads of both sequences on the way at once (that covers 4,096 tokens a
+// sequence) and keeps which of their tokens count for the gradient; the rest of longer sequences goes in a loop.
+constexpr int kPairQuads = 2;
+
 __global__ __launch_bounds__(kPairBlock) void preference_loss_kernel(Preference a, const float* __restrict__ logp,
                                                                      float* __restrict__ dlogp, float* __restrict__ rewards,
                                                                      PairTerms* __restrict__ partials) {
     __shared__ double shared[2 * kPairBlock / 64];
     __shared__ int64_t shared_n[2 * kPairBlock / 64];
     const int64_t pair = blockIdx.x;
+    const float* ref = a.ref_logp ? a.ref_logp : logp;
     int64_t begin[2], end[2], n[2];
     double sum[2];
+    f32x4_any x[2][kPairQuads], y[2][kPairQuads];
+    uint32_t in[2][kPairQuads];
+#pragma unroll
+    for (int side = 0; side < 2; side++) sequence_at(a.batch, pair + side * a.n_pairs, begin[side], end[side]);
+    const bool quads = a.batch.tokens >= 4;               // below that everything goes in the loop
+    const int64_t head = quads ? kPairQuads * kPairBlock * 4 : 0;
+    if (quads) {
+#pragma unroll
+        for (int side = 0; side < 2; side++) {
+#pragma unroll
+            for (int q = 0; q < kPairQuads; q++) {
+                const int64_t own = begin[side] + ((int64_t)q * kPairBlock + threadIdx.x) * 4;
+                const int64_t t = own + 4 <= a.batch.tokens ? own : a.batch.tokens - 4;
+                x[side][q] = load4(logp + t);
+                y[side][q] = load4(ref + t);
+                in[side][q] = load_mask4(a.batch.mask ? a.batch.mask + t : (const uint8_t*)(logp + t));
+            }
+        }
+    }
 #pragma unroll
     for (int side = 0; side < 2; side++) {
-        sequence_at(a.batch, pair + side * a.n_pairs, begin[side], end[side]);
-        const RatioSum o = sum_ratios<kPairBlock>(a, logp, begin[side], end[side], threadIdx.x);
-        sum[side] = o.sum;
-        n[side] = o.n;
+        sum[side] = 0.0;
+        n[side] = 0;
+#pragma unroll
+        for (int q = 0; q < kPairQuads; q++) {
+            if (!quads) continue;
+            const int64_t own = begin[side] + ((int64_t)q * kPairBlock + threadIdx.x) * 4;
+            const int64_t t = own + 4 <= a.batch.tokens ? own : a.batch.tokens - 4;
+            in[side][q] = (a.batch.mask ? nonzero_bytes(in[side][q]) : 0x80808080u) & tokens_within(t, own, end[side]);
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                sum[side] += in[side][q] >> (8 * i) & 0x80u
+                                 ? (double)x[side][q][i] - (a.ref_logp ? (double)y[side][q][i] : 0.0) : 0.0;
+            n[side] += __builtin_popcount(in[side][q]);
+        }
+        const RatioSum o = sum_ratios<kPairBlock>(a, logp, begin[side] + head, end[side], threadIdx.x);
+        sum[side] += o.sum;
+        n[side] += o.n;
     }
     sum_block<kPairBlock, 2>(sum, shared);
     sum_block<kPairBlock, 2>(n, shared_n);
     const PairValues v = pair_values(a, sum, n);
 #pragma unroll
-    for (int side = 0; side < 2; side++) put_gradients<kPairBlock>(a, dlogp, begin[side], end[side], v.grad[side], threadIdx.x);
+    for (int side = 0; side < 2; side++) {
+        const float g = v.grad[side];
+#pragma unroll
+        for (int q = 0; q < kPairQuads; q++) {
+            if (!quads) continue;
+            const int64_t own = begin[side] + ((int64_t)q * kPairBlock + threadIdx.x) * 4;
+            const int64_t t = own + 4 <= a.batch.tokens ? own : a.batch.tokens - 4;
+            f32x4_any d;
+#pragma unroll
+            for (int i = 0; i < 4; i++) d[i] = in[side][q] >> (8 * i) & 0x80u ? g : 0.0f;
+            if (own + 4 <= end[side]) {
+                store4(dlogp + own, d);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (t + i >= own && t + i < end[side]) dlogp[t + i] = d[i];
+            }
+        }
+        put_gradients<kPairBlock>(a, dlogp, begin[side] + head, end[side], g, threadIdx.x);
+    }
     clear_outside(a, dlogp, pair * kPairBlock + threadIdx.x, (int64_t)gridDim.x * kPairBlock);
     if (threadIdx.x == 0) {
         if (rewards) {
@@ -1252,13 +1475,13 @@ __device__ __forceinline__ void write_pair_stats(const double (&v)[5], int64_t n
 // The whole of a small batch in one launch of one workgroup, a wavefront per pair.
 constexpr int64_t kSmallPairs = 32, kSmallPairTokens = 16384;
 
-__global__ __launch_bounds__(1024) void preference_loss_small_kernel(Preference a, const float* __restrict__ logp,
+__global__ __launch_bounds__(kPairBlock) void preference_loss_small_kernel(Preference a, const float* __restrict__ logp,
                                                                      float* __restrict__ dlogp, float* __restrict__ rewards,
                                                                      rlx_preference_stats* __restrict__ stats) {
-    __shared__ double shared[5 * 16];
+    __shared__ double shared[5 * kPairBlock / 64];
     const int lane = threadIdx.x & 63;
     double terms[5] = {0.0, 0.0, 0.0, 0.0, 0.0};
-    for (int64_t pair = threadIdx.x >> 6; pair < a.n_pairs; pair += 16) {
+    for (int64_t pair = threadIdx.x >> 6; pair < a.n_pairs; pair += kPairBlock / 64) {
         int64_t begin[2], end[2], n[2];
         double sum[2];
 #pragma unroll
@@ -1283,8 +1506,8 @@ __global__ __launch_bounds__(1024) void preference_loss_small_kernel(Preference 
             terms[4] += v.terms.rejected;
         }
     }
-    if (a.n_pairs) clear_outside(a, dlogp, threadIdx.x, 1024);
-    sum_block<1024, 5>(terms, shared);
+    if (a.n_pairs) clear_outside(a, dlogp, threadIdx.x, kPairBlock);
+    sum_block<kPairBlock, 5>(terms, shared);
     if (threadIdx.x == 0) write_pair_stats(terms, a.n_pairs, stats);
 }
 
@@ -1393,6 +1616,12 @@ Cut cut_of(const rlx_logits& x) {
     return c;
 }
 
+// Whether the loss from logits is better off with its rows in chunks, read twice, than with a workgroup per row: long rows
+// that would leave compute units idle.
+constexpr int64_t kFewRows = 128;
+bool few_rows(const rlx_logits& x) { return x.rows > 0 && x.rows <= kFewRows && row_groups(x) > 512 * 8; }
+int64_t few_chunks(const rlx_logits& x) { return (row_groups(x) + kChunkBlock * kFewGroups - 1) / (kChunkBlock * kFewGroups); }
+
 // Whether every row starts on a 16-byte boundary.
 bool rows_aligned(const rlx_logits& x) {
     const int64_t es = (int64_t)elem_size(x.dtype);
@@ -1435,7 +1664,7 @@ int64_t round16(int64_t n) { return (n + 15) & ~(int64_t)15; }
 int64_t token_blocks(int64_t tokens) { return (tokens + kTokensPerBlock - 1) / kTokensPerBlock; }
 
 bool small_pairs(int64_t tokens, int64_t n_pairs) { return tokens <= kSmallPairTokens && n_pairs <= kSmallPairs; }
-bool small_batch(int64_t tokens, int64_t n_seqs) { return tokens <= kSmallTokens && n_seqs <= kSmallSeqs; }
+bool small_batch(int64_t tokens, int64_t n_seqs) { return tokens < 4 || (tokens <= kSmallTokens && n_seqs <= kSmallSeqs); }
 
 int make_policy(const rlx_policy_args* p, int64_t tokens, Policy& a) {
     if (!p) return RLX_ERR_INVALID_ARG;
@@ -1569,7 +1798,8 @@ int rlx_token_logprob(const rlx_logits* x, const void* targets, int index_type, 
                 st = for_row_launches(v.rows, kMostGridY, [&](uint32_t first, uint32_t here) {
                     chunk_statistics_kernel<T, BLOCK, NG, decltype(dot)::value, decltype(once)::value>
                         <<<dim3(cut.chunks, here), dim3(BLOCK), 0, s>>>(v, targets, wide, nullptr, k, inv_t,
-                                                                        cut.chunks == 1 ? o : none, partials, nullptr, first);
+                                                                        cut.chunks == 1 ? o : none, partials, nullptr, nullptr,
+                                                                        first);
                 });
             });
         });
@@ -1633,7 +1863,12 @@ int rlx_policy_loss(const float* logp, int64_t tokens, const rlx_policy_args* ar
         return st;
     hipStream_t s = (hipStream_t)stream;
     if (small_batch(tokens, a.batch.n_seqs)) {
-        policy_loss_small_kernel<<<dim3(1), dim3(kSmallBlock), 0, s>>>(a, logp, dlogp, dentropy, stats);
+        if (tokens <= 128 * kSmallPerLane)
+            policy_loss_small_kernel<128><<<dim3(1), dim3(128), 0, s>>>(a, logp, dlogp, dentropy, stats);
+        else if (tokens <= 256 * kSmallPerLane)
+            policy_loss_small_kernel<256><<<dim3(1), dim3(256), 0, s>>>(a, logp, dlogp, dentropy, stats);
+        else
+            policy_loss_small_kernel<512><<<dim3(1), dim3(512), 0, s>>>(a, logp, dlogp, dentropy, stats);
         RLX_HIP(hipGetLastError());
         return RLX_OK;
     }
@@ -1653,6 +1888,9 @@ int rlx_policy_loss(const float* logp, int64_t tokens, const rlx_policy_args* ar
 
 int64_t rlx_policy_loss_logits_workspace(const rlx_logits* x, int64_t n_seqs) {
     if (check_logits(x) != RLX_OK || n_seqs < 0 || n_seqs > kMaxRows) return -1;
+    if (few_rows(*x))
+        return round16(x->rows * few_chunks(*x) * (int64_t)sizeof(Stat)) + round16(4 * x->rows) +
+               x->rows * (int64_t)sizeof(Terms) + 16;
     return round16(4 * n_seqs) + round16(4 * x->rows) + x->rows * (int64_t)sizeof(Terms);
 }
 
@@ -1674,6 +1912,28 @@ int rlx_policy_loss_logits(const rlx_logits* x, const void* targets, int index_t
     const Logits v = view(*x), dv = view(*dx);
     const float inv_t = 1.0f / temperature, k = kLog2e / temperature;
     const int wide = index_type == RLX_INDEX_I64;
+    if (few_rows(*x)) {
+        const unsigned chunks = (unsigned)few_chunks(*x);
+        Stat* partials = (Stat*)workspace;
+        float* target_logits = (float*)((char*)workspace + round16(x->rows * chunks * (int64_t)sizeof(Stat)));
+        Terms* terms = (Terms*)((char*)target_logits + round16(4 * x->rows));
+        uint32_t* ticket = (uint32_t*)(terms + x->rows);
+        const RowOutputs none = {nullptr, nullptr, nullptr};
+        for_type(x->dtype, [&](auto type) {
+            typedef decltype(type) T;
+            const dim3 grid(chunks, v.rows);
+            chunk_statistics_kernel<T, kChunkBlock, kFewGroups, true, false><<<grid, dim3(kChunkBlock), 0, s>>>(
+                v, targets, wide, a.batch.mask, k, inv_t, none, partials, target_logits, ticket, 0);
+            if (a.entropy_coef != 0.0f)
+                policy_loss_few_kernel<T, true><<<grid, dim3(kChunkBlock), 0, s>>>(
+                    v, dv, targets, wide, k, inv_t, a, partials, target_logits, logp, entropy, terms, ticket, stats);
+            else
+                policy_loss_few_kernel<T, false><<<grid, dim3(kChunkBlock), 0, s>>>(
+                    v, dv, targets, wide, k, inv_t, a, partials, target_logits, logp, entropy, terms, ticket, stats);
+        });
+        RLX_HIP(hipGetLastError());
+        return RLX_OK;
+    }
     int32_t* seq_counts = (int32_t*)workspace;
     int32_t* info = (int32_t*)((char*)workspace + round16(4 * a.batch.n_seqs));
     Terms* partials = (Terms*)((char*)info + round16(4 * x->rows));
@@ -1728,7 +1988,7 @@ int rlx_preference_loss(const float* logp, int64_t tokens, const rlx_preference_
     a.average = args->average ? 1 : 0;
     hipStream_t s = (hipStream_t)stream;
     if (small_pairs(tokens, a.n_pairs)) {
-        preference_loss_small_kernel<<<dim3(1), dim3(1024), 0, s>>>(a, logp, dlogp, rewards, stats);
+        preference_loss_small_kernel<<<dim3(1), dim3(kPairBlock), 0, s>>>(a, logp, dlogp, rewards, stats);
         RLX_HIP(hipGetLastError());
         return RLX_OK;
     }

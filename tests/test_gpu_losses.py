@@ -318,6 +318,35 @@ def test_policy_loss(losses, T, cu, reduction):
         assert T.equal(again.stats, r.stats) and T.equal(again.dlogp, r.dlogp)
 
 
+@pytest.mark.parametrize("tokens", [1, 2, 3, 5, 2047, 2049])
+@pytest.mark.parametrize("n_seqs", [1, 3, 1024, 5000])
+@pytest.mark.parametrize("reduction", ["sequence", "token"])
+def test_policy_loss_of_few_tokens_and_many_sequences(losses, T, tokens, n_seqs, reduction):
+    rng = np.random.default_rng(tokens + n_seqs)
+    cu = np.sort(rng.integers(0, tokens + 1, n_seqs + 1))
+    cu[0], cu[-1] = 0, tokens
+    h, d, rng = policy_inputs(T, tokens, n_seqs, False, 7)
+    mask = rng.random(tokens) < 0.9
+    kw = dict(kl_coef=0.1, reduction=reduction)
+    r = losses.policy_loss(d["logp"], d["advantages"], old_logp=d["old_logp"], ref_logp=d["ref_logp"],
+                           mask=T.tensor(mask).cuda(), cu_seqlens=T.tensor(cu.astype(np.int32)).cuda(), **kw)
+    seq = LO.sequences(tokens, cu)
+    # the oracle tells advantages per token and per sequence apart by their number
+    adv = h["advantages"] if n_seqs == tokens else h["advantages"][seq]
+    want = LO.policy(h["logp"], adv, seq, n_seqs, mask, old=h["old_logp"], ref=h["ref_logp"], **kw)
+    dlogp, _, size = check_policy(r, want, tokens, "few tokens")
+    check(r.dlogp, dlogp, size * 12 * U + 1e-37, "dlogp")
+    if n_seqs > 1:                                             # the same offsets as pairs
+        cu2 = cu if n_seqs % 2 == 0 else np.append(cu, tokens)
+        p = losses.preference_loss(d["logp"], ref_logp=d["ref_logp"], mask=T.tensor(mask).cuda(),
+                                   cu_seqlens=T.tensor(cu2.astype(np.int32)).cuda(), beta=0.3)
+        stats, rewards, dl = LO.preference(h["logp"], LO.sequences(tokens, cu2), (len(cu2) - 1) // 2, mask,
+                                           ref=h["ref_logp"], beta=0.3)
+        check(p.rewards, rewards, np.abs(rewards) * 2 * U + 1e-12, "rewards")
+        check(p.dlogp, dl, np.abs(dl) * 2 * U + 1e-37, "pairs dlogp")
+        check(p.stats, stats, np.abs(stats) * 2 * U + 1e-12, "pairs stats")
+
+
 def test_policy_loss_padded_batch(losses, T):
     h, d, rng = policy_inputs(T, 6 * 111, 6, False, 4)
     mask = rng.random((6, 111)) < 0.6
