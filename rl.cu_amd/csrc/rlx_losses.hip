@@ -659,7 +659,7 @@ __device__ __forceinline__ int64_t wave_offsets_up_to(const RLX_GLOBAL int32_t* 
 struct Policy {             // rlx_policy_args as the kernels take it
     const float *old_logp, *ref_logp, *advantages, *entropy;
     Batch batch;
-    double log_high, log_low;      // borders of the clip
+    float log_high[2], log_low[2]; // borders of the clip, each as a sum of two
     double norm;
     float high, low;               // 1 + clip_high, 1 - clip_low
     float kl_coef, entropy_coef, grad_scale;
@@ -702,17 +702,26 @@ struct TokenLoss {
 // old and ref are used only where the batch has them.
 __device__ __forceinline__ TokenLoss token_loss(const Policy& a, float logp, float old, float ref, float advantage) {
     TokenLoss o;
-    // the side of the border is decided in FP64: the inputs' difference is exact there
-    const double lr = a.old_logp ? (double)logp - (double)old : 0.0;
-    o.clipped = advantage >= 0.0f ? lr > a.log_high : lr < a.log_low;
-    o.ratio = expf((float)lr);
+    // The side of the border is decided as if in 48 bits: lr + rest is the inputs' difference exactly, and near the border
+    // its difference from the border's upper part is exact too.  (1.6 M tokens: 15.6 us, and 16.0 with this and the weighted
+    // terms in FP64.)
+    float lr = 0.0f, rest = 0.0f;
+    if (a.old_logp) {
+        lr = logp - old;
+        const float back = lr - logp;
+        rest = (logp - (lr - back)) - (old + back);
+        if (!(fabsf(rest) < INFINITY)) rest = 0.0f;          // of infinities
+    }
+    o.clipped = advantage >= 0.0f ? (lr - a.log_high[0]) + (rest - a.log_high[1]) > 0.0f
+                                  : (lr - a.log_low[0]) + (rest - a.log_low[1]) < 0.0f;
+    o.ratio = expf(lr);
     // min(rho A, clip(rho) A) without the product of an infinite rho and A = 0
     o.policy = -(advantage * (o.clipped ? (advantage >= 0.0f ? a.high : a.low) : o.ratio));
     o.slope = o.clipped ? 0.0f : -(advantage * o.ratio);
     o.kl = 0.0f;
     if (a.ref_logp) {
         float em1;
-        kl_of((float)((double)ref - (double)logp), em1, o.kl);
+        kl_of(ref - logp, em1, o.kl);
         if (a.kl_coef != 0.0f) o.slope -= a.kl_coef * em1;
     }
     return o;
@@ -780,6 +789,8 @@ __device__ __forceinline__ int masked_in(u32x4 v) {
     return n;
 }
 
+constexpr int64_t kMostInline = 1024;         // sequences whose counts a wavefront adds up by itself
+
 // How many tokens of each sequence count; with `info` also, per token, its sequence, or -1 if it is ignored.
 __global__ __launch_bounds__(kTokenBlock) void sequence_counts_kernel(Batch b, const void* __restrict__ targets, int wide,
                                                                       int32_t* __restrict__ out, int32_t* __restrict__ info) {
@@ -804,6 +815,7 @@ __global__ __launch_bounds__(kTokenBlock) void sequence_counts_kernel(Batch b, c
         if (threadIdx.x == 0) out[s] = (int32_t)n;
         __syncthreads();
     }
+    for (int64_t s = b.n_seqs + threadIdx.x; blockIdx.x == 0 && s < kMostInline; s += kTokenBlock) out[s] = 0;
     if (info && b.cu) {                       // in front of the first and behind the last sequence
         int64_t lo, hi, unused;
         sequence_at(b, 0, lo, unused);
@@ -814,14 +826,16 @@ __global__ __launch_bounds__(kTokenBlock) void sequence_counts_kernel(Batch b, c
     }
 }
 
-// The counts of all sequences, by one wavefront.
-__device__ __forceinline__ int64_t batch_count(const Batch& b, const int32_t* __restrict__ seq_counts) {
-    int64_t n = 0;
-    for (int64_t s = threadIdx.x & 63; s < b.n_seqs; s += 64) n += seq_counts[s];
-    return wave_sum8(n);
+// The counts of all sequences, by one wavefront: kMostInline of them, those behind the last sequence 0, in one go (a loop
+// over 512 counts, a load at a time, took 6 us).
+__device__ __forceinline__ int64_t batch_count(const int32_t* __restrict__ seq_counts) {
+    const RLX_GLOBAL u32x4* at = (const RLX_GLOBAL u32x4*)seq_counts + (threadIdx.x & 63);
+    const u32x4 a = at[0], b = at[64], c = at[128], d = at[192];
+    uint32_t n = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) n += a[i] + b[i] + c[i] + d[i];
+    return wave_sum8((int64_t)n);
 }
-
-constexpr int64_t kMostInline = 1024;         // sequences whose counts a wavefront adds up by itself
 
 // Leaves the sum in place of the first count, for batches of more sequences.
 __global__ __launch_bounds__(1024) void total_count_kernel(int32_t* __restrict__ seq_counts, int64_t n_seqs) {
@@ -836,7 +850,7 @@ __global__ __launch_bounds__(1024) void total_count_kernel(int32_t* __restrict__
 __device__ __forceinline__ int64_t count_for(const Policy& a, const int32_t* __restrict__ seq_counts, int64_t s) {
     if (a.reduction == RLX_LOSS_SUM) return 1;
     if (a.reduction == RLX_LOSS_SEQUENCE_MEAN) return seq_counts[s];
-    return a.batch.n_seqs > kMostInline ? (int64_t)seq_counts[0] : batch_count(a.batch, seq_counts);
+    return a.batch.n_seqs > kMostInline ? (int64_t)seq_counts[0] : batch_count(seq_counts);
 }
 
 // Four consecutive floats at any 4-byte boundary.
@@ -873,17 +887,37 @@ __device__ __forceinline__ uint32_t tokens_within(int64_t at, int64_t from, int6
     return in;
 }
 
-// One token's share of the loss; returns its gradients (of logp, of the entropy).
-__device__ __forceinline__ f32x2 add_token(const Policy& a, double w, float logp, float old, float ref, float entropy,
-                                           float advantage, Terms& v) {
+// What a lane adds up over its few tokens.
+struct LaneTerms {
+    float policy, kl, entropy, ratio;      // the first three weighted
+    int clipped, count;
+};
+
+// A token's weight as it is used: in the loss, in the gradients of logp and of the entropy.
+struct Weight {
+    float loss, logp, entropy;
+};
+
+__device__ __forceinline__ Weight weights(const Policy& a, int64_t count) {
+    const double w = weight_of(a, count), g = w * (double)a.grad_scale;
+    return {(float)w, (float)g, (float)(g * -(double)a.entropy_coef)};
+}
+
+// One token's share of the loss; returns its gradient.
+__device__ __forceinline__ float add_token(const Policy& a, const Weight& w, float logp, float old, float ref, float entropy,
+                                           float advantage, LaneTerms& v) {
     const TokenLoss o = token_loss(a, logp, old, ref, advantage);
-    v.policy += w * (double)o.policy;
-    v.kl += w * (double)o.kl;
-    v.entropy += w * (double)entropy;
-    v.clipped += o.clipped ? 1.0 : 0.0;
-    v.ratio += (double)o.ratio;
+    v.policy += w.loss * o.policy;
+    v.kl += w.loss * o.kl;
+    v.entropy += w.loss * entropy;
+    v.ratio += o.ratio;
+    v.clipped += o.clipped ? 1 : 0;
     v.count++;
-    return f32x2{(float)(w * (double)o.slope) * a.grad_scale, (float)(w * -(double)a.entropy_coef) * a.grad_scale};
+    return w.logp * o.slope;
+}
+
+__device__ __forceinline__ Terms terms_of(const LaneTerms& v) {
+    return {(double)v.policy, (double)v.kl, (double)v.entropy, (double)v.clipped, (double)v.ratio, v.count};
 }
 
 constexpr int kTokensPerBlock = 4 * kTokenBlock;
@@ -916,9 +950,9 @@ __global__ __launch_bounds__(kTokenBlock) void policy_loss_kernel(Policy a, cons
     const int64_t total = a.reduction == RLX_LOSS_TOKEN_MEAN ? count_for(a, seq_counts, 0) : 1;
     int64_t at = lo, weighed = -1;
     if (lo != hi) at = cu ? offsets_up_to(cu, lo, hi, t0) : t0 / len + 1;
-    double w = 0.0;
+    Weight w = {0.0f, 0.0f, 0.0f};
     float advantage = 0.0f;
-    Terms v = {0.0, 0.0, 0.0, 0.0, 0.0, 0};
+    LaneTerms v = {0.0f, 0.0f, 0.0f, 0.0f, 0, 0};
     f32x4_any g = {0.0f, 0.0f, 0.0f, 0.0f}, dh = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < 4; i++) {
@@ -931,13 +965,11 @@ __global__ __launch_bounds__(kTokenBlock) void policy_loss_kernel(Policy a, cons
         if ((x.in >> (8 * i) & 0x80u) && at >= 1 && at <= n_seqs) {
             if (weighed != at) {
                 weighed = at;
-                w = weight_of(a, a.reduction == RLX_LOSS_SEQUENCE_MEAN ? (int64_t)seq_counts[at - 1] : total);
+                w = weights(a, a.reduction == RLX_LOSS_SEQUENCE_MEAN ? (int64_t)seq_counts[at - 1] : total);
                 if (!a.per_token) advantage = a.advantages[at - 1];
             }
-            const f32x2 d = add_token(a, w, x.logp[i], x.old[i], x.ref[i], x.entropy[i],
-                                      a.per_token ? x.advantage[i] : advantage, v);
-            g[i] = d[0];
-            dh[i] = d[1];
+            g[i] = add_token(a, w, x.logp[i], x.old[i], x.ref[i], x.entropy[i], a.per_token ? x.advantage[i] : advantage, v);
+            dh[i] = w.entropy;
         }
     }
     if (t0 == own) {
@@ -951,8 +983,8 @@ __global__ __launch_bounds__(kTokenBlock) void policy_loss_kernel(Policy a, cons
             if (dentropy) dentropy[t0 + i] = dh[i];
         }
     }
-    v = sum_terms<kTokenBlock>(v, shared, shared_n);
-    if (threadIdx.x == 0) partials[blockIdx.x] = v;
+    const Terms sum = sum_terms<kTokenBlock>(terms_of(v), shared, shared_n);
+    if (threadIdx.x == 0) partials[blockIdx.x] = sum;
 }
 
 __device__ void write_stats(const Terms& v, float kl_coef, float entropy_coef, rlx_policy_stats* stats) {
@@ -1027,21 +1059,22 @@ __global__ __launch_bounds__(BLOCK) void policy_loss_small_kernel(Policy a, cons
         for (int s = tid; s < slots; s += BLOCK) total += many ? (in_seq[s] > 0 ? 1 : 0) : in_seq[s];
         total = sum_block<BLOCK>(total, shared_m);
     }
-    Terms v = {0.0, 0.0, 0.0, 0.0, 0.0, 0};
+    LaneTerms v = {0.0f, 0.0f, 0.0f, 0.0f, 0, 0};
 #pragma unroll
     for (int i = 0; i < kSmallPerLane; i++) {
         const int t = tid + i * BLOCK;
         if (t >= tokens) continue;
         f32x2 d = {0.0f, 0.0f};
         if (at[i] >= 0) {
-            const double w = weight_of(a, a.reduction == RLX_LOSS_SEQUENCE_MEAN ? (int64_t)in_seq[many ? tid : at[i]] : total);
-            d = add_token(a, w, lp[i], old[i], ref[i], a.entropy ? entropy[i] : 0.0f, adv[i], v);
+            const Weight w = weights(a, a.reduction == RLX_LOSS_SEQUENCE_MEAN ? (int64_t)in_seq[many ? tid : at[i]] : total);
+            d[0] = add_token(a, w, lp[i], old[i], ref[i], a.entropy ? entropy[i] : 0.0f, adv[i], v);
+            d[1] = w.entropy;
         }
         dlogp[t] = d[0];
         if (dentropy) dentropy[t] = d[1];
     }
-    v = sum_terms<BLOCK>(v, shared, shared_n);
-    if (tid == 0) write_stats(v, a.kl_coef, a.entropy_coef, stats);
+    const Terms sum = sum_terms<BLOCK>(terms_of(v), shared, shared_n);
+    if (tid == 0) write_stats(sum, a.kl_coef, a.entropy_coef, stats);
 }
 
 constexpr int kStatsBlock = 512;
@@ -1306,9 +1339,6 @@ struct PairTerms {
     double loss, correct, diff, chosen, rejected;
 };
 
-// log(1 / (1 + e^-x))
-__device__ __forceinline__ double log_sigmoid(double x) { return fmin(x, 0.0) - log1p(exp(-fabs(x))); }
-
 struct PairValues {
     PairTerms terms;
     float grad[2];               // of each counted token of the chosen and of the rejected sequence
@@ -1323,8 +1353,11 @@ __device__ __forceinline__ PairValues pair_values(const Preference& a, const dou
         reward[i] = sum[i] * per[i];
     }
     const double diff = reward[0] - reward[1], x = diff - (double)a.margin, ls = (double)a.smoothing;
-    const double log_s = log_sigmoid(x), log_n = log_sigmoid(-x);
-    const double slope = (ls * exp(log_s) - (1.0 - ls) * exp(log_n)) / (double)a.n_pairs * (double)a.grad_scale;
+    // with e = exp(-|x|): log sigmoid(x) = min(x, 0) - log(1 + e), sigmoid(|x|) = 1 / (1 + e), sigmoid(-|x|) = e / (1 + e)
+    const double e = exp(-fabs(x)), l = log1p(e), inv = 1.0 / (1.0 + e);
+    const double log_s = fmin(x, 0.0) - l, log_n = fmin(-x, 0.0) - l;
+    const double s = x >= 0.0 ? inv : e * inv, s_neg = x >= 0.0 ? e * inv : inv;
+    const double slope = (ls * s - (1.0 - ls) * s_neg) / (double)a.n_pairs * (double)a.grad_scale;
     // 0 * (-inf) of a label that is not smoothed is 0
     const double loss = -(1.0 - ls) * (ls < 1.0 ? log_s : 0.0) - ls * (ls > 0.0 ? log_n : 0.0);
     return {{loss, diff > 0.0 ? 1.0 : 0.0, diff, reward[0], reward[1]}, {(float)(slope * per[0]), (float)(-slope * per[1])}};
@@ -1390,6 +1423,7 @@ __global__ __launch_bounds__(kPairBlock) void preference_loss_kernel(Preference 
                                                                      PairTerms* __restrict__ partials) {
     __shared__ double shared[2 * kPairBlock / 64];
     __shared__ int64_t shared_n[2 * kPairBlock / 64];
+    __shared__ float grads[2];
     const int64_t pair = blockIdx.x;
     const float* ref = a.ref_logp ? a.ref_logp : logp;
     int64_t begin[2], end[2], n[2];
@@ -1435,10 +1469,23 @@ __global__ __launch_bounds__(kPairBlock) void preference_loss_kernel(Preference 
     }
     sum_block<kPairBlock, 2>(sum, shared);
     sum_block<kPairBlock, 2>(n, shared_n);
-    const PairValues v = pair_values(a, sum, n);
+    // by one wavefront: its few hundred FP64 instructions in all eight would hold up the compute unit
+    if (threadIdx.x < 64) {
+        const PairValues v = pair_values(a, sum, n);
+        if (threadIdx.x == 0) {
+            grads[0] = v.grad[0];
+            grads[1] = v.grad[1];
+            if (rewards) {
+                rewards[pair] = (float)v.terms.chosen;
+                rewards[a.n_pairs + pair] = (float)v.terms.rejected;
+            }
+            partials[pair] = v.terms;
+        }
+    }
+    __syncthreads();
 #pragma unroll
     for (int side = 0; side < 2; side++) {
-        const float g = v.grad[side];
+        const float g = grads[side];
 #pragma unroll
         for (int q = 0; q < kPairQuads; q++) {
             if (!quads) continue;
@@ -1458,13 +1505,6 @@ __global__ __launch_bounds__(kPairBlock) void preference_loss_kernel(Preference 
         put_gradients<kPairBlock>(a, dlogp, begin[side] + head, end[side], g, threadIdx.x);
     }
     clear_outside(a, dlogp, pair * kPairBlock + threadIdx.x, (int64_t)gridDim.x * kPairBlock);
-    if (threadIdx.x == 0) {
-        if (rewards) {
-            rewards[pair] = (float)v.terms.chosen;
-            rewards[a.n_pairs + pair] = (float)v.terms.rejected;
-        }
-        partials[pair] = v.terms;
-    }
 }
 
 __device__ __forceinline__ void write_pair_stats(const double (&v)[5], int64_t n, rlx_preference_stats* stats) {
@@ -1616,10 +1656,12 @@ Cut cut_of(const rlx_logits& x) {
     return c;
 }
 
-// Whether the loss from logits is better off with its rows in chunks, read twice, than with a workgroup per row: long rows
-// that would leave compute units idle.
-constexpr int64_t kFewRows = 128;
-bool few_rows(const rlx_logits& x) { return x.rows > 0 && x.rows <= kFewRows && row_groups(x) > 512 * 8; }
+// Whether the loss from logits is better off with its rows in chunks, read twice, than with a workgroup per row: long rows,
+// too few of them to fill the chip.  Time on the GPU, chunks / workgroup per row: 14 rows of 151,936 FP16 11.1 / 23.8 us,
+// 85 rows 20.7 / 24.6, 145 rows 32.9 / 26.0; 85 rows of 151,936 FP32 33.1 / 36.1, 145 rows 53.8 / 43.4; 57 rows of 50,257
+// BF16 12.5 / 17.0, 164 rows 18.6 / 17.5; 57 rows of 32,000 11.1 / 12.8, 145 rows 14.4 / 13.4; rows of 16,000 gain nothing.
+constexpr int64_t kFewRows = 96;
+bool few_rows(const rlx_logits& x) { return x.rows > 0 && x.rows <= kFewRows && row_groups(x) > 256 * 8; }
 int64_t few_chunks(const rlx_logits& x) { return (row_groups(x) + kChunkBlock * kFewGroups - 1) / (kChunkBlock * kFewGroups); }
 
 // Whether every row starts on a 16-byte boundary.
@@ -1661,6 +1703,7 @@ int check_batch(const Batch& b) {
 }
 
 int64_t round16(int64_t n) { return (n + 15) & ~(int64_t)15; }
+int64_t counts_bytes(int64_t n_seqs) { return round16(4 * (n_seqs > kMostInline ? n_seqs : kMostInline)); }
 int64_t token_blocks(int64_t tokens) { return (tokens + kTokensPerBlock - 1) / kTokensPerBlock; }
 
 bool small_pairs(int64_t tokens, int64_t n_pairs) { return tokens <= kSmallPairTokens && n_pairs <= kSmallPairs; }
@@ -1682,8 +1725,11 @@ int make_policy(const rlx_policy_args* p, int64_t tokens, Policy& a) {
     if (p->clip_low < 0.0f || p->clip_low > 1.0f || p->clip_high < 0.0f) return RLX_ERR_BAD_HYPER;
     if (tokens > 0 && !p->advantages) return RLX_ERR_INVALID_ARG;
     if (!floats_aligned({p->old_logp, p->ref_logp, p->advantages, p->entropy})) return RLX_ERR_MISALIGNED;
-    a.log_high = std::log1p((double)p->clip_high);
-    a.log_low = std::log1p(-(double)p->clip_low);
+    const double high = std::log1p((double)p->clip_high), low = std::log1p(-(double)p->clip_low);
+    a.log_high[0] = (float)high;
+    a.log_high[1] = (float)(high - (double)a.log_high[0]);
+    a.log_low[0] = (float)low;                              // -inf for clip_low = 1: nothing is below it
+    a.log_low[1] = std::isfinite(low) ? (float)(low - (double)a.log_low[0]) : 0.0f;
     a.high = (float)(1.0 + (double)p->clip_high);
     a.low = (float)(1.0 - (double)p->clip_low);
     a.norm = (double)p->norm;
@@ -1848,7 +1894,7 @@ int rlx_token_logprob_backward(const rlx_logits* x, const void* targets, int ind
 int64_t rlx_policy_loss_workspace(int64_t tokens, int64_t n_seqs) {
     if (tokens < 0 || n_seqs < 0 || tokens > kMaxRows || n_seqs > kMaxRows) return -1;
     if (small_batch(tokens, n_seqs)) return 0;
-    return round16(4 * n_seqs) + token_blocks(tokens) * (int64_t)sizeof(Terms);
+    return counts_bytes(n_seqs) + token_blocks(tokens) * (int64_t)sizeof(Terms);
 }
 
 int rlx_policy_loss(const float* logp, int64_t tokens, const rlx_policy_args* args, float* dlogp, float* dentropy,
@@ -1873,7 +1919,7 @@ int rlx_policy_loss(const float* logp, int64_t tokens, const rlx_policy_args* ar
         return RLX_OK;
     }
     int32_t* seq_counts = (int32_t*)workspace;
-    Terms* partials = (Terms*)((char*)workspace + round16(4 * a.batch.n_seqs));
+    Terms* partials = (Terms*)((char*)workspace + counts_bytes(a.batch.n_seqs));
     if (tokens && a.reduction != RLX_LOSS_SUM) RLX_HIP(launch_counts(a, nullptr, 0, seq_counts, nullptr, s));
     const int64_t blocks = token_blocks(tokens);
     if (blocks) {
@@ -1891,7 +1937,7 @@ int64_t rlx_policy_loss_logits_workspace(const rlx_logits* x, int64_t n_seqs) {
     if (few_rows(*x))
         return round16(x->rows * few_chunks(*x) * (int64_t)sizeof(Stat)) + round16(4 * x->rows) +
                x->rows * (int64_t)sizeof(Terms) + 16;
-    return round16(4 * n_seqs) + round16(4 * x->rows) + x->rows * (int64_t)sizeof(Terms);
+    return counts_bytes(n_seqs) + round16(4 * x->rows) + x->rows * (int64_t)sizeof(Terms);
 }
 
 int rlx_policy_loss_logits(const rlx_logits* x, const void* targets, int index_type, float temperature,
@@ -1935,7 +1981,7 @@ int rlx_policy_loss_logits(const rlx_logits* x, const void* targets, int index_t
         return RLX_OK;
     }
     int32_t* seq_counts = (int32_t*)workspace;
-    int32_t* info = (int32_t*)((char*)workspace + round16(4 * a.batch.n_seqs));
+    int32_t* info = (int32_t*)((char*)workspace + counts_bytes(a.batch.n_seqs));
     Terms* partials = (Terms*)((char*)info + round16(4 * x->rows));
     if (v.rows) RLX_HIP(launch_counts(a, targets, wide, seq_counts, info, s));
     for_type(x->dtype, [&](auto type) {

@@ -61,15 +61,15 @@ def _ptr(name, t, device, dtype, shape):
     """Address of a contiguous tensor of the given type and shape; None for None."""
     if t is None:
         return None
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.device == device and t.is_contiguous():
+        return t.data_ptr()
     if _on_gpu(name, t) != device:
         raise ValueError("%s is on %s, the other tensors on %s" % (name, t.device, device))
     if t.dtype != dtype:
         raise ValueError("%s must be %s, not %s" % (name, dtype, t.dtype))
     if t.shape != shape:
         raise ValueError("%s must have the shape %s, not %s" % (name, tuple(shape), tuple(t.shape)))
-    if not t.is_contiguous():
-        raise ValueError("%s must be contiguous" % name)
-    return t.data_ptr()
+    raise ValueError("%s must be contiguous" % name)
 
 
 def _logits(name, x):
