@@ -25,8 +25,7 @@
 namespace {
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-// 16 bytes at any 2-byte boundary: rows of an odd vocabulary start anywhere (gfx950 reads and writes these as one
-// 128-bit access)
+// 16 bytes at any 2-byte boundary: rows of an odd vocabulary start anywhere (gfx950 writes these as one 128-bit access)
 typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
@@ -244,14 +243,13 @@ __device__ __forceinline__ T8 wave_sum8(T8 x) {
 __device__ __forceinline__ void forget(u32x4& v) { asm volatile("" : "+v"(v)); }
 
 // A row is its whole 16-byte groups, counted from its first element wherever that lies, and the fewer than PER elements
-// behind them, one per lane.  (Counting from the first 16-byte boundary instead was no faster: 93.0 against 89.5 us for the
-// policy loss of 2,250 rows of 50,257 BF16, and a sum's order would depend on the address.)
+// behind them, one per lane.  (Counted from the first 16-byte boundary, a sum's order would depend on the address.)
 
 // Loads N groups per lane, STEP apart; what lies behind the last group comes as -inf.  The loads are unconditional
 // (lanes without a group read the last one again): a load under a condition makes the compiler wait for it before it
 // issues the next, which took the policy loss of 8,000 rows of 32,000 FP16 from 136 to 246 us.  ONCE: past the
 // caches, for rows that start on a 16-byte boundary (statistics of 4,096 x 151,936 FP16: 187 against 199 us); groups of
-// other rows share cache lines, which would be fetched twice (2,250 rows of 50,257 BF16: 89.5 against 110 us).
+// other rows share cache lines, which would be fetched twice.
 template <typename T, int N, int STEP, bool ONCE>
 __device__ __forceinline__ void load_groups(u32x4 (&held)[N], const char* row, int first, int groups) {
     if (groups == 0) {                        // fewer elements than a group: nothing may be read
@@ -259,10 +257,32 @@ __device__ __forceinline__ void load_groups(u32x4 (&held)[N], const char* row, i
         for (int n = 0; n < N; n++) held[n] = u32x4{T::kLeast, T::kLeast, T::kLeast, T::kLeast};
         return;
     }
+    if constexpr (ONCE || T::SIZE == 4) {
 #pragma unroll
-    for (int n = 0; n < N; n++) {
-        const int g = first + n * STEP < groups ? first + n * STEP : groups - 1;
-        held[n] = ONCE ? load16_once(row + (int64_t)g * 16) : load16(row + (int64_t)g * 16);
+        for (int n = 0; n < N; n++) {
+            const int g = first + n * STEP < groups ? first + n * STEP : groups - 1;
+            held[n] = ONCE ? load16_once(row + (int64_t)g * 16) : load16(row + (int64_t)g * 16);
+        }
+    } else {
+        // Rows of an odd vocabulary start in the middle of a word, and a 16-byte load from there is slow (2,250 rows of 50,257
+        // BF16: 113 against 95 us).  So the words that hold the group are loaded, four and the one with its last element
+        // (the fourth again if the row starts with a word), and shifted into place.
+        const uint32_t off = (uint32_t)(uintptr_t)row & 2;
+        const char* words = row - off;
+        uint32_t tail[N];
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            const int g = first + n * STEP < groups ? first + n * STEP : groups - 1;
+            const char* at = words + (int64_t)g * 16;
+            held[n] = load16(at);
+            tail[n] = *(const RLX_GLOBAL uint32_t*)(const RLX_GLOBAL char*)(at + 12 + 2 * off);
+        }
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            const u32x4 w = held[n];
+            held[n] = u32x4{__builtin_amdgcn_alignbyte(w[1], w[0], off), __builtin_amdgcn_alignbyte(w[2], w[1], off),
+                            __builtin_amdgcn_alignbyte(w[3], w[2], off), __builtin_amdgcn_alignbyte(tail[n], w[3], off)};
+        }
     }
 #pragma unroll
     for (int n = 0; n < N; n++)
