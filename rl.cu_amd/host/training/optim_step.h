@@ -6,7 +6,9 @@
 #pragma once
 #include <chrono>
 #include <functional>
+#include <vector>
 
+#include "kernels/losses.h"
 #include "logger.h"
 #include "lr_scheduler.h"
 #include "optimizer.h"
@@ -74,12 +76,50 @@ public:
         return accum_loss / (float)grad_accum_steps;
     }
 
+    // GRPOTrainer::grpo_training_step (GRPO_trainer.h:452-517) around the optimizer: clear the gradient pools; for each
+    // of n_micro micro-batches forward(k) gives its logits and the arguments of the policy loss, which is divided by n_micro
+    // and whose gradient is written over the logits; backward(k, dlogits) adds its gradients into the pools; then
+    // apply().  Returns the loss; statistics() holds those of each micro-batch, the pre-clip norm is last_grad_norm().
+    struct PolicyBatch {
+        rlx_logits logits;             // overwritten with their gradient
+        const int* targets;            // device [rows]
+        float temperature = 1.0f;
+        rlx_policy_args args;          // norm is set here
+        float* logp;                   // device [rows], written
+        float* entropy = nullptr;      // device [rows] or null, written
+    };
+    float policy_step(GradPools* grads, int n_micro, const std::function<PolicyBatch(int)>& forward,
+                      const std::function<void(int, const rlx_logits&)>& backward, size_t embed_elems = 0,
+                      hipStream_t stream = 0) {
+        if (n_micro < 1) RLX_CHECK(RLX_ERR_INVALID_ARG);
+        grad_pools_zero(grads, stream);
+        const int64_t stats_bytes = (int64_t)(n_micro * sizeof(rlx_policy_stats));
+        rlx_policy_stats* d_stats = (rlx_policy_stats*)stats_memory_.reserve(stats_bytes);
+        for (int k = 0; k < n_micro; k++) {
+            PolicyBatch b = forward(k);
+            b.args.norm = 1.0f / (float)n_micro;
+            launch_policy_loss_logits(b.logits, b.targets, b.temperature, b.args, b.logp, b.entropy, b.logits, d_stats + k,
+                                      loss_memory_, stream);
+            backward(k, b.logits);
+        }
+        apply(grads, embed_elems, stream);
+        statistics_.resize((size_t)n_micro);
+        HIP_CHECK(hipMemcpyAsync(statistics_.data(), d_stats, (size_t)stats_bytes, hipMemcpyDeviceToHost, stream));
+        HIP_CHECK(hipStreamSynchronize(stream));
+        double loss = 0.0;
+        for (const rlx_policy_stats& s : statistics_) loss += (double)s.loss;
+        return (float)loss;
+    }
+
+    const std::vector<rlx_policy_stats>& statistics() const { return statistics_; }
     float last_grad_norm() const { return last_grad_norm_; }
 
 private:
     AdamWOptimizer* optimizer_;
     OptimStepConfig config_;
     float last_grad_norm_ = 0.0f;
+    LossWorkspace loss_memory_, stats_memory_;
+    std::vector<rlx_policy_stats> statistics_;
 };
 
 // The optimizer end of Trainer::train (include/training/trainer.h:183-225): per step set the scheduled

@@ -696,3 +696,14 @@ def test_policy_step(losses, L, host, O, T, fused):
     assert big.any() and np.allclose(moved[big], -1e-2 * np.sign(grad[big]), rtol=2e-2)
     with pytest.raises(ValueError):
         host.policy_step(opt, forward, backward, 0, 1.0)
+
+
+def test_cpp_host_losses(torch_gpu):
+    """tests/cpp/test_losses_host.cpp: the C++ wrappers and OptimStep::policy_step against loops in double."""
+    import os
+    import subprocess
+    folder = os.path.join(os.path.dirname(os.path.abspath(__file__)), "cpp")
+    subprocess.run(["make", "-C", folder, "-s", "test_losses_host.bin"], check=True)
+    res = subprocess.run([os.path.join(folder, "test_losses_host.bin")], capture_output=True, text=True, timeout=100)
+    assert res.returncode == 0, res.stdout + res.stderr
+    assert res.stdout.count("[PASS]") == 5 and "[FAIL]" not in res.stdout
