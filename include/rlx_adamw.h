@@ -27,7 +27,8 @@ typedef enum {
     RLX_ERR_BAD_HYPER = 3,        /* bias correction of 0, or a non-finite hyper-parameter */
     RLX_ERR_HIP = 4,              /* a HIP runtime call failed; see rlx_last_hip_error() */
     RLX_ERR_NO_DEVICE = 5,
-    RLX_ERR_TOO_LARGE = 6,        /* more chunks than one plan can address, or than rlx_grad_norm_static holds */
+    RLX_ERR_TOO_LARGE = 6,        /* more chunks than one plan can address, or than rlx_grad_norm_static holds; more
+                                     rows, tokens or sequences than a loss operator takes */
     RLX_ERR_NO_MEMORY = 7,        /* host allocation failed */
     RLX_ERR_WRONG_DEVICE = 8      /* the plan was made with another device current */
 } rlx_status;
@@ -276,6 +277,7 @@ int rlx_plan_schedule_overrun(rlx_plan* plan, int64_t* overrun, void* stream);
  *    (two streams, two recorded graphs) need a workspace each; calls on one stream may share one.
  *  - Softmax statistics and sums are FP32 per lane, sums over tokens FP64; a result is rounded
  *    once, to its own type.
+ *  - Outputs do not overlap inputs or each other, except for dx, which may be x.
  *  - A row (token) that is masked out, or whose target is negative, is IGNORED: its logits, log
  *    probabilities and so on are not used whatever they hold (NaN included), its outputs are 0 and its
  *    row of gradients is 0.  A target >= vocab makes the row's outputs NaN; nothing outside the row is read.
@@ -315,7 +317,8 @@ int rlx_token_logprob(const rlx_logits* x, const void* targets, int index_type, 
  * Gradient of the logits from those of logp and entropy (dentropy and entropy both NULL, or neither), with the lse
  * and entropy that rlx_token_logprob gave for the same logits and temperature:
  *     dx[r][j] = (dlogp[r] ([j = target] - p[r][j]) - dentropy[r] p[r][j] (log p[r][j] + entropy[r])) / temperature,
- * p = exp(z - lse).  A row whose two gradients are 0 gets zeros without being read.  dx has x's rows, vocab and dtype;
+ * p = exp(z - lse) (so the lse has to tell: that of a row of the type's lowest value only does not hold log vocab).  A row
+ * whose two gradients are 0 gets zeros without being read.  dx has x's rows, vocab and dtype;
  * it may be x itself (same data and strides) but may not overlap it otherwise.
  * Replaces the backward half of the log-softmax gather (src/model/qwen3.cu:170).
  */

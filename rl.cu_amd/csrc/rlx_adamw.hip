@@ -1798,7 +1798,7 @@ const char* rlx_status_string(int status) {
     case RLX_ERR_BAD_HYPER: return "bias correction is zero or a hyper-parameter is not finite";
     case RLX_ERR_HIP: return "HIP runtime error";
     case RLX_ERR_NO_DEVICE: return "no HIP device";
-    case RLX_ERR_TOO_LARGE: return "too many chunks: more than one plan can address, or more than the 262,144 partials that the static scratch of rlx_grad_norm_static holds";
+    case RLX_ERR_TOO_LARGE: return "too many chunks: more than one plan can address, or more than the 262,144 partials that the static scratch of rlx_grad_norm_static holds, or more rows, tokens or sequences than a loss operator takes";
     case RLX_ERR_NO_MEMORY: return "out of host memory";
     case RLX_ERR_WRONG_DEVICE: return "the plan belongs to another device than the current one";
     default: return "unknown status";

@@ -3,6 +3,8 @@
 // include/rlx_adamw.h.
 //
 // The work is streams of logits over HBM with one exponential per element; there is nothing for the matrix cores.
+// Measured rates below are bytes that have to move (each read once, each written once) over the time on the GPU, inputs
+// changing from call to call so that nothing is left in the caches.
 //
 // Softmax statistics.  With k = log2(e) / temperature a row's softmax is 2^(z k) / sum 2^(z k).  A lane keeps
 //     ref = an integer, sum = sum 2^(z k - ref), dot = sum 2^(z k - ref) (z k - ref),
@@ -33,8 +35,8 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.693147180559945309417f;
-constexpr float kLn2Hi = 0.693145751953125f;              // 15 bits: an integer below 2^9 times this is exact
-constexpr float kLn2Lo = 1.42860682030941723212e-6f;
+constexpr float kLn2Hi = 45426.0f / 65536.0f;             // ln 2 cut to 15 bits: an integer below 2^9 times this is exact
+constexpr float kLn2Lo = (float)(0.693147180559945309417 - 45426.0 / 65536.0);
 constexpr float kRefMost = 536870912.0f;                  // 2^29
 constexpr float kLeastD = -1e30f;                         // keeps 0 * (-inf) out of sums of p log p
 
@@ -264,9 +266,10 @@ __device__ __forceinline__ void load_groups(u32x4 (&held)[N], const char* row, i
             held[n] = ONCE ? load16_once(row + (int64_t)g * 16) : load16(row + (int64_t)g * 16);
         }
     } else {
-        // Rows of an odd vocabulary start in the middle of a word, and a 16-byte load from there is slow (2,250 rows of 50,257
-        // BF16: 113 against 95 us).  So the words that hold the group are loaded, four and the one with its last element
-        // (the fourth again if the row starts with a word), and shifted into place.
+        // Rows of an odd vocabulary start in the middle of a word, and a 16-byte load from there is slow (policy loss of 2,250
+        // rows of 50,257 BF16: 113 against 95 us).  So the words that hold the group are loaded, four and the one with its
+        // last element (the fourth again if the row starts with a word), and shifted into place.  No word is read that
+        // holds none of the group's bytes; its other half may be another row's, and is dropped.
         const uint32_t off = (uint32_t)(uintptr_t)row & 2;
         const char* words = row - off;
         uint32_t tail[N];
@@ -505,6 +508,9 @@ __device__ __forceinline__ void put_values(const RowOutputs& o, uint32_t r, cons
 // Statistics of one chunk of a row (BLOCK * NG groups) per workgroup: consecutive workgroups read consecutive memory, so
 // that the addresses in flight stay a narrow window, and a few rows still fill the chip.  A row of one chunk is
 // finished here, with `o`; the chunks of longer rows are added up by the joining launch.
+// Bound by HBM reads: 4,096 rows of 151,936 FP16 take 180 us in 32 KiB chunks (6.9 TB/s; the vector units are busy for 115
+// of them), 190 in 16 KiB, 333 in 4 KiB, 206 with a workgroup walking its row.  Rows of up to 32 KiB have one chunk (8,192
+// rows of 5,001 FP16: 37 us against 47 in chunks of a fixed size).
 template <typename T, int BLOCK, int NG, bool DOT, bool ONCE>
 __global__ __launch_bounds__(BLOCK) void chunk_statistics_kernel(Logits x, const void* __restrict__ targets, int wide,
                                                                  const uint8_t* __restrict__ mask, float k, float inv_t,
@@ -573,8 +579,10 @@ __global__ __launch_bounds__(kJoinBlock) void token_logprob_join_kernel(Logits x
     if (threadIdx.x == 0) put_values(o, r, v);
 }
 
-// dx from the saved lse (and entropy), one chunk per workgroup.  p = exp(z - lse) is formed as 2^((z/T - lse) log2 e), the
-// difference first, so that the rounding is of the size of log p.
+// dx from the saved lse (and entropy), 4 KiB of a row per workgroup.  Bound by HBM, reads and writes: 4,096 rows of 151,936
+// BF16, a quarter of them ignored, 335 us = 6.5 TB/s (8 KiB per workgroup 357, 16 KiB 372, a workgroup per row 437); rows
+// that do not start on 16 bytes do better with half the lanes and two groups each (50,257 BF16: 143 against 156 us).
+// p = exp(z - lse) is formed as 2^((z/T - lse) log2 e), the difference first, so that the rounding is of the size of log p.
 template <typename T, int BLOCK, int NG, bool DOT, bool ONCE>
 __global__ __launch_bounds__(BLOCK) void token_logprob_backward_kernel(
     Logits x, Logits dx, const void* __restrict__ targets, int wide, float inv_t, const float* __restrict__ lse,
@@ -945,6 +953,8 @@ constexpr int kTokensPerBlock = 4 * kTokenBlock;
 // Policy loss over log-probabilities (of at least four tokens): a workgroup takes kTokensPerBlock tokens, a lane four in a
 // row; the quads of the lanes at the end of the arrays move back into them.  The sequences of a workgroup's first
 // and last token are searched once; only where they differ does a lane search between them.
+// 1.6 M tokens with every input (46 MB): 15.4 us, of which the arithmetic is 8 (193 vector instructions a token) and
+// the memory 9; all wavefronts are resident at once, so the two overlap little.  A token per lane took 37.
 __global__ __launch_bounds__(kTokenBlock) void policy_loss_kernel(Policy a, const float* __restrict__ logp,
                                                                   const int32_t* __restrict__ seq_counts,
                                                                   float* __restrict__ dlogp, float* __restrict__ dentropy,
@@ -1142,7 +1152,13 @@ __device__ __forceinline__ RowTerms row_terms(const Policy& a, const Row& row, f
 
 // Policy loss from logits: one workgroup per row, the row held in registers between its statistics and its gradient
 // (NG 16-byte groups per lane; a vocabulary beyond BLOCK * NG groups has its rest read a second time, from the
-// last-level cache mostly).
+// last-level cache mostly).  A row of 151,936 halves is 304 KB: it fits the 512 KB of registers of a compute unit, not its
+// 160 KB of LDS.  Every logit is read once and every gradient written once (FETCH_SIZE 1.54 GB, WRITE_SIZE 1.94 GB at 6,360
+// rows of 151,936 FP16, a fifth of them masked), which takes 663 us = 5.2 TB/s; reading the rows twice took 990, and
+// statistics and gradient as launches of their own, the second read from the last-level cache where it fits, 15 % more.
+// Bound by the memory system on this pattern of one long row per compute unit: without any arithmetic the same accesses
+// take 640 us, and workgroups that stay and load the next row while they write the present one gained nothing (272
+// against 274 us at 90,000 FP16).
 template <typename T, int BLOCK, int NG, bool DOT, bool ONCE>
 __global__ __launch_bounds__(BLOCK) void policy_loss_row_kernel(
     Logits x, Logits dx, const void* __restrict__ targets, int wide, float k, float inv_t, Policy a,
@@ -1434,7 +1450,8 @@ __device__ __forceinline__ void clear_outside(const Preference& a, float* dlogp,
 constexpr int kPairBlock = 512;
 
 // One workgroup per pair: both sums, the pair's loss, and the gradient of its
-// tokens.  Each lane has its first kPairQuads quads of both sequences on the way at once (that covers 4,096 tokens a
+// tokens (1,024 sequences, 3.1 M tokens, 40 MB: 12 us, latencies of two phases and 8 us of memory; 19 with a token per
+// lane).  Each lane has its first kPairQuads quads of both sequences on the way at once (that covers 4,096 tokens a
 // sequence) and keeps which of their tokens count for the gradient; the rest of longer sequences goes in a loop.
 constexpr int kPairQuads = 2;
 

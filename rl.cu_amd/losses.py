@@ -8,7 +8,7 @@ formulas and what is done with masked, empty and out-of-range input.
 
 Arguments are device tensors of one GPU; work goes to that GPU's current stream and nothing is waited for.  Every call
 takes its scratch memory and its outputs from torch's allocator, so calls on several streams and calls recorded
-into graphs never share any.  Per-token tensors are contiguous; logits may be any view whose last dimension is
+into graphs never share any.  Gradients are explicit: nothing here takes part in torch's autograd.  Per-token tensors are contiguous; logits may be any view whose last dimension is
 contiguous and whose other dimensions step through memory in at most two strides (logits[:, :-1] of a padded batch).
 """
 import ctypes as C
@@ -224,8 +224,8 @@ def policy_loss(logp, advantages, old_logp=None, ref_logp=None, entropy=None, ma
                 clip_low=0.2, clip_high=0.2, kl_coef=0.0, entropy_coef=0.0, reduction="sequence", norm=1.0,
                 grad_scale=1.0):
     """Clipped policy loss with a KL term over log-probabilities, its statistics and its gradients.
-    Tokens are packed ([tokens] with cu_seqlens) or padded ([sequences, length]).  advantages: [sequences], or
-    one per token in logp's shape.  entropy is needed if entropy_coef is not 0; dentropy is its gradient then (else
+    Tokens are packed ([tokens] with cu_seqlens, without them one sequence) or padded ([sequences, length]).  advantages:
+    [sequences] (as many as sequences means one each), or one per token in logp's shape.  entropy is needed if entropy_coef is not 0; dentropy is its gradient then (else
     None)."""
     device, shape = _on_gpu("logp", logp), logp.shape
     if entropy_coef != 0.0 and entropy is None:

@@ -44,10 +44,10 @@ def check(got, want, bound, what):
     assert np.array_equal(np.isnan(got), np.isnan(want)), what + ": NaN in other places"
     fine = np.isfinite(want)
     assert np.array_equal(got[~fine & ~np.isnan(want)], want[~fine & ~np.isnan(want)]), what + ": infinities"
-    bound = np.broadcast_to(bound, want.shape)
-    off = np.abs(got - want)[fine]
-    assert (off <= bound[fine]).all(), "%s: off by %.3g where %.3g is allowed" % (
-        what, off[np.argmax(off - bound[fine])], bound[fine][np.argmax(off - bound[fine])])
+    bound = np.broadcast_to(bound, want.shape)[fine]
+    off = np.abs(got[fine] - want[fine])
+    assert (off <= bound).all(), "%s: off by %.3g where %.3g is allowed" % (
+        what, off[np.argmax(off - bound)], bound[np.argmax(off - bound)])
 
 
 def check_forward(losses, torch, x, xh, t, th, temperature, what, entropy=True):
@@ -637,6 +637,34 @@ def test_other_streams_and_recorded_graphs(losses, T, rows, vocab):
             assert all(T.equal(a, b) for a, b in zip(outs[k], eager[k])), "replay %d of graph %d" % (turn, k)
 
 
+def test_calls_at_once_on_two_streams(losses, T):
+    """The same chain on two streams at the same time, large enough to overlap, each with other inputs: the bits of either
+    one alone."""
+    rows, vocab = 900, 9001
+    inputs = [make_logits(T, rows, vocab, "float16", seed) for seed in (1, 2)]
+    adv = T.tensor([0.5, -0.5, 1.0]).cuda()
+
+    def chain(x, t):
+        f = losses.token_logprobs(x, t, with_entropy=True)
+        q = losses.policy_loss_logits(x.view(3, rows // 3, vocab), t.view(3, -1), adv, reduction="token")
+        few = losses.policy_loss_logits(x[:40].reshape(4, -1), t[:4], adv[:1])
+        p = losses.policy_loss(f.logp.view(3, -1), adv, entropy=f.entropy.view(3, -1), entropy_coef=0.1)
+        w = losses.preference_loss(f.logp.view(4, -1))
+        return [f.logp, f.lse, f.entropy, q.stats, q.dlogits, few.stats, few.dlogits, p.stats, p.dlogp, w.stats, w.dlogp]
+
+    want = [[o.clone() for o in chain(x, t)] for x, _, t, _ in inputs]
+    streams = [T.cuda.Stream(), T.cuda.Stream()]
+    T.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for s, (x, _, t, _) in zip(streams, inputs):
+            with T.cuda.stream(s):
+                got.append(chain(x, t))
+        T.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert all(T.equal(u, v) for u, v in zip(a, b))
+
+
 # --- the operators in the framework's own step ----------------------------------------------------------------------------
 
 @pytest.mark.parametrize("fused", [False, True])
@@ -696,6 +724,20 @@ def test_policy_step(losses, L, host, O, T, fused):
     assert big.any() and np.allclose(moved[big], -1e-2 * np.sign(grad[big]), rtol=2e-2)
     with pytest.raises(ValueError):
         host.policy_step(opt, forward, backward, 0, 1.0)
+    with pytest.raises(ValueError):
+        host.policy_step(opt, forward, backward, 1, 1.0, norm=0.5)
+    # the same step on a stream of its own
+    st2 = host.ParamStore(specs, "cuda:0")
+    st2.param(0).copy_(w0.reshape(-1))
+    opt2 = host.AdamWOptimizer(st2, lr=1e-2)
+    side = T.cuda.Stream()
+    side.wait_stream(T.cuda.current_stream())
+    loss2, norm2, _ = host.policy_step(
+        opt2, lambda k: dict(forward(k), logits=acts[k] @ st2.param(0).view(vocab, hidden).t()),
+        lambda k, d: st2.grad(0).view(vocab, hidden).add_(d.t() @ acts[k]), n_micro, 0.01, fused_clip=fused,
+        stream=side.cuda_stream, mask=mask, cu_seqlens=cu, kl_coef=0.1)
+    T.cuda.synchronize()
+    assert (loss2, norm2) == (loss, norm) and T.equal(st2.param(0), st.param(0))
 
 
 def test_cpp_host_losses(torch_gpu):
