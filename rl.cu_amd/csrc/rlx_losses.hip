@@ -948,13 +948,75 @@ __device__ __forceinline__ Terms terms_of(const LaneTerms& v) {
     return {(double)v.policy, (double)v.kl, (double)v.entropy, (double)v.clipped, (double)v.ratio, v.count};
 }
 
+// --- the workgroup of a launch that finishes last ------------------------------------------------------------------------
+// Every workgroup publishes its terms with device-scope stores, waits until they have arrived and takes a ticket; the one
+// that draws the last ticket adds all terms up, in their order, with device-scope loads.  Tickets decide who adds, never in
+// which order.  The launch in front clears the counter.  For launches of up to kFewRows workgroups that take part.
+
+__device__ __forceinline__ void publish8(void* p, double x) {
+    __hip_atomic_store((uint64_t*)p, __builtin_bit_cast(uint64_t, x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+__device__ __forceinline__ double published8(const void* p) {
+    return __builtin_bit_cast(double, __hip_atomic_load((const uint64_t*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
+
+// Publishes terms[block] and says, to every lane, whether this workgroup is the last of `blocks`.
+__device__ __forceinline__ bool last_with(const Terms& t, Terms* terms, uint32_t block, uint32_t blocks, uint32_t* ticket,
+                                          int* shared) {
+    if (threadIdx.x < 64) {
+        if (threadIdx.x == 0) {
+            publish8(&terms[block].policy, t.policy);
+            publish8(&terms[block].kl, t.kl);
+            publish8(&terms[block].entropy, t.entropy);
+            publish8(&terms[block].clipped, t.clipped);
+            publish8(&terms[block].ratio, t.ratio);
+            publish8(&terms[block].count, __builtin_bit_cast(double, t.count));
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // they have arrived before the ticket is taken
+        if (threadIdx.x == 0) {
+            *shared = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == blocks;
+        }
+    }
+    __syncthreads();
+    const bool last = *shared != 0;
+    if (last) __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+    return last;
+}
+
+// The sum of all published terms, by the last workgroup.
+template <int BLOCK>
+__device__ __forceinline__ Terms sum_published(const Terms* terms, uint32_t blocks, double* shared, int64_t* shared_n) {
+    Terms v = {0.0, 0.0, 0.0, 0.0, 0.0, 0};
+    for (uint32_t i = threadIdx.x; i < blocks; i += BLOCK) {
+        v.policy += published8(&terms[i].policy);
+        v.kl += published8(&terms[i].kl);
+        v.entropy += published8(&terms[i].entropy);
+        v.clipped += published8(&terms[i].clipped);
+        v.ratio += published8(&terms[i].ratio);
+        v.count += __builtin_bit_cast(int64_t, published8(&terms[i].count));
+    }
+    return sum_terms<BLOCK>(v, shared, shared_n);
+}
+
+__device__ void write_stats(const Terms& v, float kl_coef, float entropy_coef, rlx_policy_stats* stats) {
+    double loss = v.policy;
+    if (kl_coef != 0.0f) loss += (double)kl_coef * v.kl;
+    if (entropy_coef != 0.0f) loss -= (double)entropy_coef * v.entropy;
+    const double m = v.count > 0 ? (double)v.count : 1.0;
+    *stats = {(float)loss, (float)v.policy, (float)v.kl, (float)v.entropy, (float)(v.clipped / m), (float)(v.ratio / m),
+              v.count};
+}
+
 constexpr int kTokensPerBlock = 4 * kTokenBlock;
 
 // Policy loss over log-probabilities (of at least four tokens): a workgroup takes kTokensPerBlock tokens, a lane four in a
 // row; the quads of the lanes at the end of the arrays move back into them.  The sequences of a workgroup's first
 // and last token are searched once; only where they differ does a lane search between them.
 // 1.6 M tokens with every input (46 MB): 15.4 us, of which the arithmetic is 8 (193 vector instructions a token) and
-// the memory 9; all wavefronts are resident at once, so the two overlap little.  A token per lane took 37.
+// the memory 9; all wavefronts are resident at once, so the two overlap little.  A token per lane took 37.  (The partial
+// terms are added by a launch of its own, 4 us: with tickets, as few rows do it, 1,562 workgroups took 14 us longer.)
 __global__ __launch_bounds__(kTokenBlock) void policy_loss_kernel(Policy a, const float* __restrict__ logp,
                                                                   const int32_t* __restrict__ seq_counts,
                                                                   float* __restrict__ dlogp, float* __restrict__ dentropy,
@@ -1015,15 +1077,6 @@ __global__ __launch_bounds__(kTokenBlock) void policy_loss_kernel(Policy a, cons
     }
     const Terms sum = sum_terms<kTokenBlock>(terms_of(v), shared, shared_n);
     if (threadIdx.x == 0) partials[blockIdx.x] = sum;
-}
-
-__device__ void write_stats(const Terms& v, float kl_coef, float entropy_coef, rlx_policy_stats* stats) {
-    double loss = v.policy;
-    if (kl_coef != 0.0f) loss += (double)kl_coef * v.kl;
-    if (entropy_coef != 0.0f) loss -= (double)entropy_coef * v.entropy;
-    const double m = v.count > 0 ? (double)v.count : 1.0;
-    *stats = {(float)loss, (float)v.policy, (float)v.kl, (float)v.entropy, (float)(v.clipped / m), (float)(v.ratio / m),
-              v.count};
 }
 
 // The whole of a small batch in one launch of one workgroup: counts in LDS (integers, so that the order of their
@@ -1234,15 +1287,6 @@ __global__ __launch_bounds__(BLOCK) void policy_loss_row_kernel(
 
 constexpr int kFewGroups = 2;                // 16-byte groups per lane of such a chunk (8 KiB)
 
-// Loads from and stores to memory that other workgroups of the same launch share.
-__device__ __forceinline__ void publish8(void* p, double x) {
-    __hip_atomic_store((uint64_t*)p, __builtin_bit_cast(uint64_t, x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-
-__device__ __forceinline__ double published8(const void* p) {
-    return __builtin_bit_cast(double, __hip_atomic_load((const uint64_t*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-}
-
 // How many rows of begin .. end - 1 count, by one wavefront.
 __device__ __forceinline__ int64_t count_rows(const Batch& b, const void* targets, int wide, int64_t begin, int64_t end) {
     int64_t n = 0;
@@ -1255,7 +1299,7 @@ __device__ __forceinline__ int64_t count_rows(const Batch& b, const void* target
 
 // The launch behind chunk_statistics_kernel<256, kFewGroups>: every workgroup joins its row's chunks, works out the row's
 // loss for itself and writes its chunk of the gradient; the first chunk's workgroup also writes the row's values.
-// The last of those to finish (the launch in front has cleared the ticket) adds up the rows, in their order.
+// The last of those to finish adds up the rows, in their order.
 // The logits of the targets come from the first launch: here another workgroup may have overwritten them.
 template <typename T, bool DOT>
 __global__ __launch_bounds__(kChunkBlock) void policy_loss_few_kernel(
@@ -1329,35 +1373,12 @@ __global__ __launch_bounds__(kChunkBlock) void policy_loss_few_kernel(
         }
     }
     if (c != 0) return;
-    if (tid < 64) {
-        if (tid == 0) {
-            logp[r] = o.values.logp;
-            if (entropy) entropy[r] = o.values.entropy;
-            publish8(&terms[r].policy, o.terms.policy);
-            publish8(&terms[r].kl, o.terms.kl);
-            publish8(&terms[r].entropy, o.terms.entropy);
-            publish8(&terms[r].clipped, o.terms.clipped);
-            publish8(&terms[r].ratio, o.terms.ratio);
-            publish8(&terms[r].count, __builtin_bit_cast(double, o.terms.count));
-        }
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // they have arrived before the ticket is taken
-        if (tid == 0)
-            last_shared = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == gridDim.y;
+    if (tid == 0) {
+        logp[r] = o.values.logp;
+        if (entropy) entropy[r] = o.values.entropy;
     }
-    __syncthreads();
-    if (!last_shared) return;
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
-    Terms v = {0.0, 0.0, 0.0, 0.0, 0.0, 0};
-    for (uint32_t i = tid; i < gridDim.y; i += kChunkBlock) {
-        v.policy += published8(&terms[i].policy);
-        v.kl += published8(&terms[i].kl);
-        v.entropy += published8(&terms[i].entropy);
-        v.clipped += published8(&terms[i].clipped);
-        v.ratio += published8(&terms[i].ratio);
-        v.count += __builtin_bit_cast(int64_t, published8(&terms[i].count));
-    }
-    v = sum_terms<kChunkBlock>(v, sums, sums_n);
+    if (!last_with(o.terms, terms, r, gridDim.y, ticket, &last_shared)) return;
+    const Terms v = sum_published<kChunkBlock>(terms, gridDim.y, sums, sums_n);
     if (tid == 0) write_stats(v, a.kl_coef, a.entropy_coef, stats);
 }
 
@@ -1955,15 +1976,12 @@ int rlx_policy_loss(const float* logp, int64_t tokens, const rlx_policy_args* ar
         RLX_HIP(hipGetLastError());
         return RLX_OK;
     }
+    const int64_t blocks = token_blocks(tokens);
     int32_t* seq_counts = (int32_t*)workspace;
     Terms* partials = (Terms*)((char*)workspace + counts_bytes(a.batch.n_seqs));
-    if (tokens && a.reduction != RLX_LOSS_SUM) RLX_HIP(launch_counts(a, nullptr, 0, seq_counts, nullptr, s));
-    const int64_t blocks = token_blocks(tokens);
-    if (blocks) {
-        policy_loss_kernel<<<dim3((unsigned)blocks), dim3(kTokenBlock), 0, s>>>(a, logp, seq_counts, dlogp, dentropy,
-                                                                                partials);
-        RLX_HIP(hipGetLastError());
-    }
+    if (a.reduction != RLX_LOSS_SUM) RLX_HIP(launch_counts(a, nullptr, 0, seq_counts, nullptr, s));
+    policy_loss_kernel<<<dim3((unsigned)blocks), dim3(kTokenBlock), 0, s>>>(a, logp, seq_counts, dlogp, dentropy, partials);
+    RLX_HIP(hipGetLastError());
     policy_stats_kernel<<<dim3(1), dim3(kStatsBlock), 0, s>>>(partials, blocks, a.kl_coef, a.entropy_coef, stats);
     RLX_HIP(hipGetLastError());
     return RLX_OK;

@@ -214,10 +214,19 @@ def _policy_args(shape, device, advantages, old_logp, ref_logp, entropy, mask, c
                         kl_coef, entropy_coef, norm, grad_scale, _REDUCTIONS[reduction], 0 if per_sequence else 1)
 
 
-def _policy_stats(device):
-    """An rlx_policy_stats on the device and its parts."""
-    buf = torch.empty(4, dtype=torch.int64, device=device)
-    return buf, buf.view(torch.float32)[:6], buf[3]
+_SHARED = 1 << 20
+
+
+def _policy_memory(nbytes, device, where):
+    """(tensor, address of an rlx_policy_stats, its parts, address of scratch memory).  The statistics, which live on, and
+    up to 1 MiB of scratch memory share an allocation."""
+    if nbytes < 0:
+        raise B.RlxError(B.ERR_INVALID_ARG, where)
+    words = 4 + ((nbytes + 7) >> 3 if nbytes <= _SHARED else 0)
+    buf = torch.empty(words, dtype=torch.int64, device=device)
+    at = buf.data_ptr()
+    scratch, scratch_ptr = (buf, at + 32) if nbytes <= _SHARED else _workspace(nbytes, device, where)
+    return scratch, at, buf.view(torch.float32)[:6], buf[3], scratch_ptr
 
 
 def policy_loss(logp, advantages, old_logp=None, ref_logp=None, entropy=None, mask=None, cu_seqlens=None,
@@ -225,8 +234,8 @@ def policy_loss(logp, advantages, old_logp=None, ref_logp=None, entropy=None, ma
                 grad_scale=1.0):
     """Clipped policy loss with a KL term over log-probabilities, its statistics and its gradients.
     Tokens are packed ([tokens] with cu_seqlens, without them one sequence) or padded ([sequences, length]).  advantages:
-    [sequences] (as many as sequences means one each), or one per token in logp's shape.  entropy is needed if entropy_coef is not 0; dentropy is its gradient then (else
-    None)."""
+    [sequences] (as many as sequences means one each), or one per token in logp's shape.  entropy is needed if
+    entropy_coef is not 0; dentropy is its gradient then (else None)."""
     device, shape = _on_gpu("logp", logp), logp.shape
     if entropy_coef != 0.0 and entropy is None:
         raise ValueError("entropy_coef needs entropy")
@@ -237,11 +246,10 @@ def policy_loss(logp, advantages, old_logp=None, ref_logp=None, entropy=None, ma
     lib = B.load()
     with _on(device):
         dlogp, dentropy = _floats(logp), _floats(logp) if entropy_coef != 0.0 else None
-        buf, stats, count = _policy_stats(device)
         nbytes = lib.rlx_policy_loss_workspace(tokens, args.n_seqs)
-        ws, ws_ptr = _workspace(nbytes, device, "rlx_policy_loss")
+        scratch, stats_ptr, stats, count, ws_ptr = _policy_memory(nbytes, device, "rlx_policy_loss")
         B.check(lib.rlx_policy_loss(logp_p, tokens, C.byref(args), dlogp.data_ptr(), _address(dentropy),
-                                    buf.data_ptr(), ws_ptr, nbytes, _raw_stream(device.index)), "rlx_policy_loss")
+                                    stats_ptr, ws_ptr, nbytes, _raw_stream(device.index)), "rlx_policy_loss")
     return PolicyLoss(stats, count, dlogp, dentropy)
 
 
@@ -260,11 +268,10 @@ def policy_loss_logits(logits, targets, advantages, old_logp=None, ref_logp=None
     with _on(device):
         logp, entropy = _floats(targets), _floats(targets) if with_entropy else None
         out, dx = _gradient(logits, x, out)
-        buf, stats, count = _policy_stats(device)
         nbytes = lib.rlx_policy_loss_logits_workspace(C.byref(x), args.n_seqs)
-        ws, ws_ptr = _workspace(nbytes, device, "rlx_policy_loss_logits")
+        scratch, stats_ptr, stats, count, ws_ptr = _policy_memory(nbytes, device, "rlx_policy_loss_logits")
         B.check(lib.rlx_policy_loss_logits(C.byref(x), target_ptr, index_type, temperature, C.byref(args),
-                                           logp.data_ptr(), _address(entropy), C.byref(dx), buf.data_ptr(),
+                                           logp.data_ptr(), _address(entropy), C.byref(dx), stats_ptr,
                                            ws_ptr, nbytes, _raw_stream(device.index)), "rlx_policy_loss_logits")
     return PolicyLossLogits(stats, count, logp, entropy, out)
 
