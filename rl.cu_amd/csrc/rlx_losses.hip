@@ -14,6 +14,10 @@
 // References are kept within +-2^29, so that logits of -inf and of a type's lowest value simply contribute 0.  Rows
 // whose own values lie out there (every logit the lowest value, +inf, NaN) come out with a sum of 0, infinity or NaN;
 // such rows, and only they, are computed again with the row's maximum subtracted first.
+//
+// The target's own term is kept apart from the sums over the others (`rest`): where the target has most of the
+// probability, log p = -log(1 + rest / own) and 1 - p = rest / sum keep their relative precision, which a sum that has
+// swallowed both no longer holds (it left log p = -0.0007 off by 2e-4 of itself).
 
 #include <hip/hip_runtime.h>
 
@@ -61,9 +65,18 @@ __device__ __forceinline__ uint32_t max_f16x2(uint32_t a, uint32_t b) {       //
     return r;
 }
 
+// Element `at` of eight 16-bit ones becomes the half of `least`.
+__device__ __forceinline__ void drop_half(u32x4& v, int at, uint32_t least) {
+    const uint32_t keep = at & 1 ? 0x0000ffffu : 0xffff0000u;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (i == at >> 1) v[i] = (v[i] & keep) | (least & ~keep);
+}
+
 struct F16 {
     static constexpr int PER = 8, SIZE = 2;
     static constexpr uint32_t kLeast = 0xfc00fc00u;                             // -inf, twice
+    static __device__ __forceinline__ void drop(u32x4& v, int at) { drop_half(v, at, kLeast); }
     typedef uint32_t Top;                                                       // two running maxima
     static __device__ __forceinline__ Top no_top() { return kLeast; }
     static __device__ __forceinline__ void add_top(Top& t, u32x4 v) {
@@ -100,6 +113,7 @@ struct F16 {
 struct BF16 {
     static constexpr int PER = 8, SIZE = 2;
     static constexpr uint32_t kLeast = 0xff80ff80u;
+    static __device__ __forceinline__ void drop(u32x4& v, int at) { drop_half(v, at, kLeast); }
     typedef float Top;
     static __device__ __forceinline__ Top no_top() { return -INFINITY; }
     static __device__ __forceinline__ void add_top(Top& t, u32x4 v) {
@@ -137,6 +151,11 @@ struct BF16 {
 struct F32 {
     static constexpr int PER = 4, SIZE = 4;
     static constexpr uint32_t kLeast = 0xff800000u;
+    static __device__ __forceinline__ void drop(u32x4& v, int at) {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (i == at) v[i] = kLeast;
+    }
     typedef float Top;
     static __device__ __forceinline__ Top no_top() { return -INFINITY; }
     static __device__ __forceinline__ void add_top(Top& t, u32x4 v) {
@@ -292,6 +311,15 @@ __device__ __forceinline__ void load_groups(u32x4 (&held)[N], const char* row, i
         if (first + n * STEP >= groups) held[n] = u32x4{T::kLeast, T::kLeast, T::kLeast, T::kLeast};
 }
 
+// Takes the target out of the groups that the lanes of a workgroup hold (first group of lane 0: `from`).
+template <typename T, int N, int STEP>
+__device__ __forceinline__ void drop_target(u32x4 (&held)[N], int from, int target) {
+    const int group = target / T::PER - from;                   // the same in all lanes
+#pragma unroll
+    for (int n = 0; n < N; n++)
+        if (group >= n * STEP && group < (n + 1) * STEP && (int)threadIdx.x == group - n * STEP) T::drop(held[n], target % T::PER);
+}
+
 // --- statistics of a row ---------------------------------------------------------------------------------------------
 
 struct Stat {
@@ -337,10 +365,24 @@ __device__ __forceinline__ Stat join_block(Stat s, Stat* shared) {
     return s;
 }
 
-// What the row's softmax is computed from: 2^((z - shift) k - ref) / sum.
+// What the row's softmax is computed from: 2^((z - shift) k - ref) / (rest + hot), hot being the target's term and rest and
+// dot the sums over the others.
 struct Row {
-    float shift, ref, sum, dot;
+    float shift, ref, rest, dot, hot;
+    __device__ __forceinline__ float sum() const { return rest + hot; }
 };
+
+// A row from the statistics of all logits but the target's, and that one.
+__device__ __forceinline__ Row row_of(const Stat& s, float zt, float k) {
+    Row r;
+    r.shift = 0.0f;
+    r.ref = fmaxf(s.ref, reference_of(zt, k));
+    const float d = s.ref - r.ref, f = exp2_of(d);              // a power of two: exact
+    r.rest = s.sum * f;
+    r.dot = f * (s.dot + d * s.sum);
+    r.hot = exp2_of(__builtin_fmaf(zt, k, -r.ref));
+    return r;
+}
 
 template <int BLOCK>
 __device__ __forceinline__ float max_block(float v, float* shared) {
@@ -356,7 +398,7 @@ __device__ __forceinline__ float max_block(float v, float* shared) {
 
 // The rare rows: maximum first, then the sums with it subtracted, one element at a time.
 template <typename T, int BLOCK>
-__device__ __attribute__((noinline)) Row row_by_maximum(const char* row, int vocab, float k, Stat* shared) {
+__device__ __attribute__((noinline)) Row row_by_maximum(const char* row, int vocab, int target, float k, Stat* shared) {
     float top = -INFINITY;
     for (int j = threadIdx.x; j < vocab; j += BLOCK) top = fmaxf(top, T::one(row, j));
     __syncthreads();                                  // `shared` held the row's first result
@@ -364,12 +406,13 @@ __device__ __attribute__((noinline)) Row row_by_maximum(const char* row, int voc
     __syncthreads();
     Stat s = {0.0f, 0.0f, 0.0f};
     for (int j = threadIdx.x; j < vocab; j += BLOCK) {
+        if (j == target) continue;
         const float d = (T::one(row, j) - top) * k, e = exp2_of(d);
         s.sum += e;
         s.dot = __builtin_fmaf(e, fmaxf(d, kLeastD), s.dot);
     }
     s = join_block<true, BLOCK>(s, shared);
-    return {top, 0.0f, s.sum, s.dot};
+    return {top, 0.0f, s.sum, s.dot, exp2_of((T::one(row, target) - top) * k)};
 }
 
 __device__ __forceinline__ bool ordinary(float sum) { return sum > 0.0f && sum < INFINITY; }
@@ -382,14 +425,16 @@ struct RowValues {
 // reference, so that what is rounded is of the size of the result.
 __device__ __forceinline__ RowValues row_values(const Row& row, float zt, float k, float inv_t) {
     int e;
-    const float mant = frexpf(row.sum, &e);
+    const float sum = row.sum(), mant = frexpf(sum, &e);
     const float ref = row.ref + (float)e, lm = log2f(mant);
     RowValues v;
     v.log2_sum = (float)e + lm;
     v.lse = __builtin_fmaf(ref, kLn2Hi, __builtin_fmaf(ref, kLn2Lo, kLn2 * lm));
     if (row.shift != 0.0f) v.lse = row.shift * inv_t + v.lse;
-    v.logp = (__builtin_fmaf(zt - row.shift, k, -ref) - lm) * kLn2;
-    v.entropy = (v.log2_sum - row.dot / row.sum) * kLn2;
+    v.logp = row.hot > row.rest ? 0.0f - log1pf(row.rest / row.hot) : (__builtin_fmaf(zt - row.shift, k, -ref) - lm) * kLn2;
+    // - p log p of the target, and of the others: log2 p = d - log2 sum
+    const float own = row.hot > 0.0f ? row.hot * v.logp : 0.0f;
+    v.entropy = (0.0f - (own + (row.dot - row.rest * v.log2_sum) * kLn2)) / sum;
     return v;
 }
 
@@ -422,21 +467,22 @@ __device__ __forceinline__ Stat held_statistics(u32x4 (&held)[N], float loose, f
     return s;
 }
 
-// The gradient of a row: -p (b0 + b1 d) with d = (z - shift) k - ref, plus `hot` at the target.
+// The gradient of a row: 2^d (b0 + b1 d) with d = (z - shift) k - ref, and `hot` at the target.
 struct RowGrad {
     float shift, ref, b0, b1, hot;
 };
 
 // g: gradient of logp; c: gradient of the entropy (both with 1/temperature in them).
 __device__ __forceinline__ RowGrad row_gradient(const Row& row, const RowValues& v, float g, float c) {
-    const float inv = 1.0f / row.sum;
+    const float inv = 1.0f / row.sum();
     RowGrad q;
     q.shift = row.shift;
     q.ref = row.ref;
     // log p = ln2 (d - log2 sum), so p (g + c (log p + H)) = p (g + c (H - ln2 log2 sum) + c ln2 d)
     q.b0 = -inv * (g + c * (v.entropy - kLn2 * v.log2_sum));
     q.b1 = -inv * (c * kLn2);
-    q.hot = g;
+    q.hot = g * (row.rest * inv);                              // g (1 - p)
+    if (row.hot > 0.0f) q.hot -= c * (row.hot * inv) * (v.logp + v.entropy);
     return q;
 }
 
@@ -468,7 +514,7 @@ __device__ void fill_row(char* out, int vocab, float value) {
     if (j < vocab) T::put(out, j, value);
 }
 
-// The gradient of one group, `hot` added if the target is in it (at < 0 or >= PER: it is not).
+// The gradient of one group, with the target's own if it is in it (at < 0 or >= PER: it is not).
 template <typename T, bool DOT>
 __device__ __forceinline__ u32x4 grad_group(const RowGrad& q, u32x4 v, float k, int at) {
     float z[T::PER];
@@ -478,7 +524,7 @@ __device__ __forceinline__ u32x4 grad_group(const RowGrad& q, u32x4 v, float k, 
     if ((unsigned)at < (unsigned)T::PER) {
 #pragma unroll
         for (int i = 0; i < T::PER; i++)
-            if (i == at) z[i] += q.hot;
+            if (i == at) z[i] = q.hot;
     }
     return T::pack(z);
 }
@@ -489,7 +535,7 @@ __device__ __attribute__((noinline)) void rare_gradient(RowGrad q, const char* r
                                                         float k, int target) {
     for (int j = from + threadIdx.x; j < to; j += BLOCK) {
         const float d = grad_by_maximum<DOT>(q, T::one(row, j), k);
-        T::put(out, j, j == target ? d + q.hot : d);
+        T::put(out, j, j == target ? q.hot : d);
     }
 }
 
@@ -531,14 +577,15 @@ __global__ __launch_bounds__(BLOCK) void chunk_statistics_kernel(Logits x, const
     const int groups = x.vocab / T::PER, at = (int)c * BLOCK * NG + tid, j = groups * T::PER + tid;
     u32x4 held[NG];
     load_groups<T, NG, BLOCK, ONCE>(held, row, at, groups);
-    const float loose = c == 0 && j < x.vocab ? T::one(row, j) : -INFINITY;
+    drop_target<T, NG, BLOCK>(held, (int)c * BLOCK * NG, (int)t);
+    const float loose = c == 0 && j < x.vocab && j != (int)t ? T::one(row, j) : -INFINITY;
     const bool finish = o.logp != nullptr;
     const float zt = finish || (target_logits && c == 0) ? T::one(row, t) : 0.0f;
     Stat s = held_statistics<T, NG, DOT>(held, loose, k);
     s = join_block<DOT, BLOCK>(s, shared);
     if (finish) {
-        Row rv = {0.0f, s.ref, s.sum, s.dot};
-        if (!ordinary(s.sum)) rv = row_by_maximum<T, BLOCK>(row, x.vocab, k, shared);
+        Row rv = row_of(s, zt, k);
+        if (!ordinary(rv.sum())) rv = row_by_maximum<T, BLOCK>(row, x.vocab, (int)t, k, shared);
         if (tid == 0) put_values(o, r, row_values(rv, zt, k, inv_t));
     } else if (tid == 0) {
         partials[(int64_t)r * gridDim.x + c] = s;
@@ -572,8 +619,8 @@ __global__ __launch_bounds__(kJoinBlock) void token_logprob_join_kernel(Logits x
         const char* row = x.data + row_at(x, r) * T::SIZE;
         const float zt = T::one(row, t);
         const Stat s = join_chunks<DOT>(partials + (int64_t)r * chunks, chunks);
-        Row rv = {0.0f, s.ref, s.sum, s.dot};
-        if (!ordinary(s.sum)) rv = row_by_maximum<T, kJoinBlock>(row, x.vocab, k, shared);
+        Row rv = row_of(s, zt, k);
+        if (!ordinary(rv.sum())) rv = row_by_maximum<T, kJoinBlock>(row, x.vocab, (int)t, k, shared);
         v = row_values(rv, zt, k, inv_t);
     }
     if (threadIdx.x == 0) put_values(o, r, v);
@@ -616,6 +663,12 @@ __global__ __launch_bounds__(BLOCK) void token_logprob_backward_kernel(
         if constexpr (DOT) return -p * __builtin_fmaf(cs, fmaxf(lp, kLeastD) + h, gs);
         else return -p * gs;
     };
+    auto grad_hot = [&](float z) {                          // 1 - p of a likely target without the difference
+        const float lp = __builtin_fmaf(z, inv_t, -l);
+        float d = -gs * expm1f(lp);
+        if constexpr (DOT) d -= exp2_of(lp * kLog2e) * cs * (fmaxf(lp, kLeastD) + h);
+        return d;
+    };
     u32x4 held[NG];
     load_groups<T, NG, BLOCK, ONCE>(held, row, at, groups);
     const float loose = has_loose ? T::one(row, j) : 0.0f;
@@ -623,19 +676,24 @@ __global__ __launch_bounds__(BLOCK) void token_logprob_backward_kernel(
     for (int n = 0; n < NG; n++) {
         float z[PER];
         T::unpack(held[n], z);
-#pragma unroll
-        for (int e = 0; e < PER; e++) z[e] = grad(z[e]);
         const int in = target - (at + n * BLOCK) * PER;
+        float hot = 0.0f;
         if ((unsigned)in < (unsigned)PER) {
 #pragma unroll
             for (int e = 0; e < PER; e++)
-                if (e == in) z[e] += gs;
+                if (e == in) hot = grad_hot(z[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < PER; e++) z[e] = grad(z[e]);
+        if ((unsigned)in < (unsigned)PER) {
+#pragma unroll
+            for (int e = 0; e < PER; e++)
+                if (e == in) z[e] = hot;
         }
         if (at + n * BLOCK < groups) store16_once(out + (int64_t)(at + n * BLOCK) * 16, T::pack(z));
     }
     if (has_loose) {
-        const float d = grad(loose);
-        T::put(out, j, j == target ? d + gs : d);
+        T::put(out, j, j == target ? grad_hot(loose) : grad(loose));
     }
 }
 
@@ -1240,18 +1298,20 @@ __global__ __launch_bounds__(BLOCK) void policy_loss_row_kernel(
     const int groups = x.vocab / T::PER, j = groups * T::PER + tid, target = (int)t;
     u32x4 held[NG];
     load_groups<T, NG, BLOCK, ONCE>(held, row, tid, groups);
-    const float loose = j < x.vocab ? T::one(row, j) : -INFINITY;
+    drop_target<T, NG, BLOCK>(held, 0, target);
+    const float loose = j < x.vocab && j != target ? T::one(row, j) : -INFINITY;
     const float zt = T::one(row, t), advantage = a.advantages[a.per_token ? (int64_t)r : s];
     const float old = a.old_logp ? a.old_logp[r] : 0.0f, ref = a.ref_logp ? a.ref_logp[r] : 0.0f;
 
     Stat st = held_statistics<T, NG, true>(held, loose, k);
     for (int g = NG * BLOCK + tid; g < groups; g += BLOCK) {
         u32x4 more[1] = {load16(row + (int64_t)g * 16)};
+        if (g == target / T::PER) T::drop(more[0], target % T::PER);
         st = joined<true>(st, held_statistics<T, 1, true>(more, -INFINITY, k));
     }
     st = join_block<true, BLOCK>(st, shared);
-    Row rv = {0.0f, st.ref, st.sum, st.dot};
-    if (!ordinary(st.sum)) rv = row_by_maximum<T, BLOCK>(row, x.vocab, k, shared_rare);
+    Row rv = row_of(st, zt, k);
+    if (!ordinary(rv.sum())) rv = row_by_maximum<T, BLOCK>(row, x.vocab, target, k, shared_rare);
     // the row's few scalars by one wavefront: every wavefront doing the same would hold up the compute unit as long
     if (tid < 64) {
         const RowTerms o = row_terms<DOT>(a, rv, zt, old, ref, advantage, count_for(a, seq_counts, s), k, inv_t);
@@ -1279,7 +1339,7 @@ __global__ __launch_bounds__(BLOCK) void policy_loss_row_kernel(
         store16_once(out + (int64_t)g * 16, grad_group<T, DOT>(q, load16(row + (int64_t)g * 16), k, target - g * T::PER));
     if (j < x.vocab) {
         const float d = grad_of<DOT>(q, loose, k);
-        T::put(out, j, j == target ? d + q.hot : d);
+        T::put(out, j, j == target ? q.hot : d);
     }
 }
 
@@ -1349,12 +1409,12 @@ __global__ __launch_bounds__(kChunkBlock) void policy_loss_few_kernel(
         }
         const float advantage = a.advantages[a.per_token ? (int64_t)r : s];
         const float old = a.old_logp ? a.old_logp[r] : 0.0f, ref = a.ref_logp ? a.ref_logp[r] : 0.0f;
-        const Stat st = join_chunks<true>(partials + (int64_t)r * gridDim.x, (int)gridDim.x);
-        const bool rare = !ordinary(st.sum);
+        const float zt = target_logits[r];
+        Row rv = row_of(join_chunks<true>(partials + (int64_t)r * gridDim.x, (int)gridDim.x), zt, k);
+        const bool rare = !ordinary(rv.sum());
         if (rare && c != 0) return;                          // the first chunk's workgroup does a rare row by itself
-        Row rv = {0.0f, st.ref, st.sum, st.dot};
-        if (rare) rv = row_by_maximum<T, kChunkBlock>(row, x.vocab, k, shared);
-        o = row_terms<DOT>(a, rv, target_logits[r], old, ref, advantage, m, k, inv_t);
+        if (rare) rv = row_by_maximum<T, kChunkBlock>(row, x.vocab, (int)t, k, shared);
+        o = row_terms<DOT>(a, rv, zt, old, ref, advantage, m, k, inv_t);
         const int target = (int)t;
         if (rare) {
             __syncthreads();                                 // every lane has read what is overwritten now
@@ -1368,7 +1428,7 @@ __global__ __launch_bounds__(kChunkBlock) void policy_loss_few_kernel(
             }
             if (has_loose) {
                 const float d = grad_of<DOT>(o.grad, loose, k);
-                T::put(out, j, j == target ? d + o.grad.hot : d);
+                T::put(out, j, j == target ? o.grad.hot : d);
             }
         }
     }

@@ -80,6 +80,44 @@ def test_forward(losses, T, name, rows, vocab):
         assert T.equal(a, b)                        # both index types, and the same bits on every run
 
 
+@pytest.mark.parametrize("rows,vocab", [(1, 1), (3, 7), (6, 513), (300, 1003), (4, 50257), (120, 50257), (2, 151936), (99, 200001)])
+@pytest.mark.parametrize("name", TYPES)
+def test_certain_targets(losses, T, name, rows, vocab):
+    """A target with nearly all of the probability: log p, 1 - p and the entropy hold relative to themselves.
+
+    With R = sum over the others of exp(z_i - z_t): log p = -log1p(R), and 1 - p = R / (1 + R) moves by R's relative error
+    times 1 - p at most.  R is a sum of positive terms like the one that slack() counts, whose exponents are log(V) + |log R|
+    on the mean over the terms; the quotient, log1p (2 ulp) and the result add 6u.
+    """
+    x, _, t, th = make_logits(T, rows, vocab, name, rows * 7 + vocab, lift=False)
+    rng = np.random.default_rng(rows)
+    th = np.resize([0, vocab - 1, vocab // 2, vocab - vocab % 8 - 1, vocab * 5 // 7], rows).clip(0, vocab - 1)
+    t = T.tensor(th).cuda()
+    pick = T.arange(rows).cuda()
+    lift = T.tensor(rng.uniform(1.0, 30.0, rows)).cuda()
+    x[pick, t] = (x.double().logsumexp(1) + lift).to(x.dtype)
+    xh = x.cpu().double().numpy()
+    z = xh - xh[np.arange(rows), th][:, None]
+    z[np.arange(rows), th] = -np.inf
+    with np.errstate(all="ignore"):
+        e = np.exp(z)
+        R = e.sum(1)
+        logp, miss = -np.log1p(R), R / (1 + R)
+        ent = ((e * np.where(e > 0, -z, 0.0)).sum(1) + R * np.log1p(R) + np.log1p(R)) / (1 + R)
+        far = np.where(R > 0, np.abs(np.log(R)), 0.0)
+    assert (miss < 0.4).all()
+    rel = LO.slack(vocab, LO.finite_max(xh), np.log(vocab) + far)
+    r = losses.token_logprobs(x, t, with_entropy=True)
+    check(r.logp, logp, rel * miss + 6 * U * np.abs(logp) + 1e-37, "logp")
+    # every -p log p moves by its p's error and by the log's, which is of R's relative size for the target and rel for others
+    check(r.entropy, ent, 2 * rel * (ent + miss) + 1e-37, "entropy")
+    adv = rng.normal(size=rows).astype(np.float32)
+    f = losses.policy_loss_logits(x, t, T.tensor(adv).cuda(), cu_seqlens=T.arange(rows + 1, dtype=T.int32).cuda(), reduction="sum")
+    check(f.logp, logp, rel * miss + 6 * U * np.abs(logp) + 1e-37, "fused logp")
+    want = -adv.astype(np.float64) * miss
+    check(f.dlogits[pick, t].double(), want, np.abs(want) * (LO.EPS[name] * 1.01 + rel + 8 * U) + LO.TINY[name], "fused gradient")
+
+
 @pytest.mark.parametrize("rows,vocab", SHAPES)
 @pytest.mark.parametrize("name", TYPES)
 def test_backward(losses, T, name, rows, vocab):
