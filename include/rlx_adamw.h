@@ -340,7 +340,7 @@ enum {
  *                       + kl_coef (exp(d) - d - 1) - entropy_coef entropy),
  *     dlogp[t] = grad_scale w_t (-A rho [not clipped] + kl_coef (1 - exp(d))),
  *     dentropy[t] = -grad_scale w_t entropy_coef.
- * "Clipped" is logp - old_logp > log(1 + clip_high) for A >= 0, < log(1 - clip_low) for A < 0, decided in FP64.
+ * "Clipped" is logp - old_logp > log(1 + clip_high) for A >= 0, < log(1 - clip_low) for A < 0, decided as if in 48 bits.
  * old_logp NULL: rho is 1 (logp is its own old value).  ref_logp NULL: no KL term.
  * Sequence s is the tokens [cu_seqlens[s], cu_seqlens[s + 1]) of the packed arrays; cu_seqlens NULL: n_seqs
  * sequences of tokens / n_seqs tokens each (a padded batch).  Sequences may be empty.  Tokens in
@@ -401,7 +401,7 @@ typedef struct rlx_preference_args {
     const float*    ref_logp;       /* device [tokens] or NULL */
     const uint8_t*  mask;           /* device [tokens] or NULL */
     const int32_t*  cu_seqlens;     /* device [2 n_pairs + 1] or NULL */
-    int64_t         n_pairs;        /* < 2^30 */
+    int64_t         n_pairs;        /* <= 2^22 */
     float           beta, label_smoothing /* 0 .. 1 */, margin, grad_scale;
     int32_t         average;
     int32_t         reserved;       /* 0 */

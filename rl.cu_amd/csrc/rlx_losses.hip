@@ -1689,6 +1689,7 @@ __global__ __launch_bounds__(kStatsBlock) void preference_stats_kernel(const Pai
 
 constexpr int64_t kMaxRows = 0x7fffffff;
 constexpr int64_t kMaxVocab = 1 << 30;
+constexpr int64_t kMaxPairs = 1 << 22;               // a workgroup of 512 lanes each: below the 2^32 lanes of one launch
 constexpr uint32_t kRowsPerLaunch = 1u << 21;        // times up to 1,024 lanes: below the 2^32 lanes of one launch
 
 size_t elem_size(int dtype) { return dtype == RLX_DTYPE_F32 ? 4 : 2; }
@@ -2119,7 +2120,7 @@ int rlx_policy_loss_logits(const rlx_logits* x, const void* targets, int index_t
 }
 
 int64_t rlx_preference_loss_workspace(int64_t tokens, int64_t n_pairs) {
-    if (tokens < 0 || n_pairs < 0 || tokens > kMaxRows || n_pairs > kMaxRows / 2) return -1;
+    if (tokens < 0 || n_pairs < 0 || tokens > kMaxRows || n_pairs > kMaxPairs) return -1;
     return small_pairs(tokens, n_pairs) ? 0 : n_pairs * (int64_t)sizeof(PairTerms);
 }
 
@@ -2127,7 +2128,7 @@ int rlx_preference_loss(const float* logp, int64_t tokens, const rlx_preference_
                         float* rewards, rlx_preference_stats* stats, void* workspace, int64_t workspace_bytes,
                         void* stream) {
     if (!args || !stats || args->reserved != 0 || args->n_pairs < 0) return RLX_ERR_INVALID_ARG;
-    if (args->n_pairs > kMaxRows / 2) return RLX_ERR_TOO_LARGE;
+    if (args->n_pairs > kMaxPairs) return RLX_ERR_TOO_LARGE;
     Preference a;
     a.ref_logp = args->ref_logp;
     a.batch = {args->mask, args->cu_seqlens, tokens, 2 * args->n_pairs};

@@ -171,6 +171,8 @@ def test_preference_arguments_are_checked(B):
                dict(ref_logp=P + 1), dict(cu_seqlens=P + 1)):
         assert call(**kw) == B.ERR_MISALIGNED, kw
     assert call(n_pairs=1 << 30) == B.ERR_TOO_LARGE
+    assert call(n_pairs=(1 << 22) + 1, nbytes=1 << 40) == B.ERR_TOO_LARGE      # more than one launch holds
+    assert B.load().rlx_preference_loss_workspace(0, (1 << 22) + 1) == -1
     assert lib.rlx_preference_loss(P, 8, None, P, P, P, P, 1 << 40, None) == bad
     assert lib.rlx_preference_loss_workspace(-1, 1) == -1 and lib.rlx_preference_loss_workspace(100000, 4) > 8
 
