@@ -555,8 +555,7 @@ __device__ __forceinline__ void put_values(const RowOutputs& o, uint32_t r, cons
 // that the addresses in flight stay a narrow window, and a few rows still fill the chip.  A row of one chunk is
 // finished here, with `o`; the chunks of longer rows are added up by the joining launch.
 // Bound by HBM reads: 4,096 rows of 151,936 FP16 take 180 us in 32 KiB chunks (6.9 TB/s; the vector units are busy for 115
-// of them), 190 in 16 KiB, 333 in 4 KiB, 206 with a workgroup walking its row.  Rows of up to 32 KiB have one chunk (8,192
-// rows of 5,001 FP16: 37 us against 47 in chunks of a fixed size).
+// of them), 190 in 16 KiB, 333 in 4 KiB, 206 with a workgroup walking its row.
 template <typename T, int BLOCK, int NG, bool DOT, bool ONCE>
 __global__ __launch_bounds__(BLOCK) void chunk_statistics_kernel(Logits x, const void* __restrict__ targets, int wide,
                                                                  const uint8_t* __restrict__ mask, float k, float inv_t,
@@ -1760,14 +1759,23 @@ struct Cut {
     int block, per_lane, chunks;
 };
 
+// Rows up to 4,096 groups (32,768 halves) go whole to a workgroup, which writes their results in the same launch; longer
+// ones in 32 KiB chunks that a second launch joins, or in 8 KiB ones where those would not fill the chip.  Recorded and
+// replayed, whole / in chunks: 32,000 FP16, 1 row 4.2 / 4.8 us, 256 rows 6.6 / 8.8, 8,192 rows 79 / 89; 16,384 FP32 256 rows
+// 6.1 / 8.3; 50,257 FP16 1 row 5.7 / 4.8, 8,192 rows 153 / 147.  In between, for 97 to 256 rows, a launch less weighs more
+// than what the few lanes of a workgroup cost: 129 rows of 50,257 FP16 7.8 / 9.1 us, of 90,000 9.7 / 10.0; 64 rows 7.5 / 7.3
+// and 9.2 / 7.7; beyond 12,288 groups chunks do better for any number of rows (129 rows of 151,936 13.9 / 12.3).
 Cut cut_of(const rlx_logits& x) {
     const int groups = row_groups(x);
-    Cut c = {64, 8, 1};
-    if (groups <= 64 * 8) return c;
-    c.block = 128;
-    if (groups <= 128 * 8) return c;
-    c.block = 256;
-    c.chunks = (groups + 256 * 8 - 1) / (256 * 8);
+    if (groups <= 64 * 8) return {64, 8, 1};
+    if (groups <= 128 * 8) return {128, 8, 1};
+    if (groups <= 256 * 8) return {256, 8, 1};
+    if (groups <= 512 * 8) return {512, 8, 1};
+    if (x.rows > 96 && x.rows <= 256) {
+        if (groups <= 512 * 14) return {512, 14, 1};
+        if (groups <= 1024 * 12) return {1024, 12, 1};
+    }
+    Cut c = {256, 8, (groups + 256 * 8 - 1) / (256 * 8)};
     if (x.rows * c.chunks < 512) {
         c.per_lane = 2;
         c.chunks = (groups + 256 * 2 - 1) / (256 * 2);
@@ -1911,6 +1919,9 @@ template <typename Fn>
 void for_cut(const Cut& c, Fn f) {
     if (c.block == 64) f(Int<64>{}, Int<8>{});
     else if (c.block == 128) f(Int<128>{}, Int<8>{});
+    else if (c.block == 512 && c.per_lane == 8) f(Int<512>{}, Int<8>{});
+    else if (c.block == 512) f(Int<512>{}, Int<14>{});
+    else if (c.block == 1024) f(Int<1024>{}, Int<12>{});
     else if (c.per_lane == 8) f(Int<256>{}, Int<8>{});
     else f(Int<256>{}, Int<2>{});
 }

@@ -66,9 +66,11 @@ def check_forward(losses, torch, x, xh, t, th, temperature, what, entropy=True):
 
 SHAPES = [(1, 1), (1, 2), (3, 7), (2, 8), (4, 9), (70, 33), (3, 513), (2, 4095), (5, 4099), (300, 1000), (2, 32003),
           (9, 50257), (1, 151936), (17, 151936), (2, 200001)]
+# statistics of whole rows by one large workgroup
+WIDE = [(11, 20003), (3, 32768), (97, 32777), (129, 50257), (99, 70001)]
 
 
-@pytest.mark.parametrize("rows,vocab", SHAPES)
+@pytest.mark.parametrize("rows,vocab", SHAPES + WIDE)
 @pytest.mark.parametrize("name", TYPES)
 def test_forward(losses, T, name, rows, vocab):
     x, xh, t, th = make_logits(T, rows, vocab, name, rows * 31 + vocab)
