@@ -396,21 +396,35 @@ __device__ __forceinline__ float max_block(float v, float* shared) {
     return v;
 }
 
+// Calls f(index, element) for all elements of a row, six loads of a lane on the way at once (one: a batch of NaN takes twice as long;
+// eight: the row kernels' registers spill around the call).
+template <typename T, int BLOCK, typename Fn>
+__device__ __forceinline__ void for_elements(const char* row, int vocab, Fn f) {
+    int j = threadIdx.x;
+    for (; j < vocab - 5 * BLOCK; j += 6 * BLOCK) {
+        float z[6];
+#pragma unroll
+        for (int i = 0; i < 6; i++) z[i] = T::one(row, j + i * BLOCK);
+#pragma unroll
+        for (int i = 0; i < 6; i++) f(j + i * BLOCK, z[i]);
+    }
+    for (; j < vocab; j += BLOCK) f(j, T::one(row, j));
+}
+
 // The rare rows: maximum first, then the sums with it subtracted, one element at a time.
 template <typename T, int BLOCK>
 __device__ __attribute__((noinline)) Row row_by_maximum(const char* row, int vocab, int target, float k, Stat* shared) {
     float top = -INFINITY;
-    for (int j = threadIdx.x; j < vocab; j += BLOCK) top = fmaxf(top, T::one(row, j));
+    for_elements<T, BLOCK>(row, vocab, [&](int, float z) { top = fmaxf(top, z); });
     __syncthreads();                                  // `shared` held the row's first result
     top = max_block<BLOCK>(top, (float*)shared);
     __syncthreads();
     Stat s = {0.0f, 0.0f, 0.0f};
-    for (int j = threadIdx.x; j < vocab; j += BLOCK) {
-        if (j == target) continue;
-        const float d = (T::one(row, j) - top) * k, e = exp2_of(d);
-        s.sum += e;
-        s.dot = __builtin_fmaf(e, fmaxf(d, kLeastD), s.dot);
-    }
+    for_elements<T, BLOCK>(row, vocab, [&](int j, float z) {
+        const float d = (z - top) * k, e = exp2_of(d);
+        s.sum += j == target ? 0.0f : e;
+        s.dot = j == target ? s.dot : __builtin_fmaf(e, fmaxf(d, kLeastD), s.dot);
+    });
     s = join_block<true, BLOCK>(s, shared);
     return {top, 0.0f, s.sum, s.dot, exp2_of((T::one(row, target) - top) * k)};
 }
@@ -601,28 +615,42 @@ __device__ __forceinline__ Stat join_chunks(const Stat* __restrict__ partials, i
     return join_wave<DOT, 64>(s);
 }
 
-constexpr int kChunkBlock = 256, kJoinBlock = 256;
+constexpr int kChunkBlock = 256, kJoinBlock = 256, kJoinRows = kJoinBlock / 64;
 
+// A row per wavefront (a workgroup per row took 3 to 5 us longer for 4,096 and 8,192 rows); the rare rows of a workgroup are
+// done again by all of it, one after the other.
 template <typename T, bool DOT>
 __global__ __launch_bounds__(kJoinBlock) void token_logprob_join_kernel(Logits x, const void* __restrict__ targets, int wide,
                                                                         float k, float inv_t,
                                                                         const Stat* __restrict__ partials, int chunks,
-                                                                        RowOutputs o, uint32_t first) {
+                                                                        RowOutputs o, uint32_t first, uint32_t rows) {
     __shared__ Stat shared[kJoinBlock / 64];
-    const uint32_t r = first + blockIdx.x;
-    const int64_t t = target_at(targets, wide, r);
-    RowValues v;
-    if (t < 0 || t >= x.vocab) {
-        v.logp = v.lse = v.entropy = t < 0 ? 0.0f : NAN;
-    } else {
-        const char* row = x.data + row_at(x, r) * T::SIZE;
-        const float zt = T::one(row, t);
-        const Stat s = join_chunks<DOT>(partials + (int64_t)r * chunks, chunks);
-        Row rv = row_of(s, zt, k);
-        if (!ordinary(rv.sum())) rv = row_by_maximum<T, kJoinBlock>(row, x.vocab, (int)t, k, shared);
-        v = row_values(rv, zt, k, inv_t);
+    __shared__ int again[kJoinRows];
+    const uint32_t wave = threadIdx.x >> 6, in_launch = blockIdx.x * kJoinRows + wave, r = first + in_launch;
+    const bool head = (threadIdx.x & 63) == 0;
+    bool rare = false;
+    if (in_launch < rows) {
+        const int64_t t = target_at(targets, wide, r);
+        if (t < 0 || t >= x.vocab) {
+            const float v = t < 0 ? 0.0f : NAN;
+            if (head) put_values(o, r, {v, v, v, v});
+        } else {
+            const float zt = T::one(x.data + row_at(x, r) * T::SIZE, t);
+            const Row rv = row_of(join_chunks<DOT>(partials + (int64_t)r * chunks, chunks), zt, k);
+            rare = !ordinary(rv.sum());
+            if (head && !rare) put_values(o, r, row_values(rv, zt, k, inv_t));
+        }
     }
-    if (threadIdx.x == 0) put_values(o, r, v);
+    if (head) again[wave] = rare ? 1 : 0;
+    __syncthreads();
+    for (uint32_t w = 0; w < kJoinRows; w++) {
+        if (!again[w]) continue;
+        const uint32_t rr = first + blockIdx.x * kJoinRows + w;
+        const char* row = x.data + row_at(x, rr) * T::SIZE;
+        const int64_t t = target_at(targets, wide, rr);
+        const Row rv = row_by_maximum<T, kJoinBlock>(row, x.vocab, (int)t, k, shared);
+        if (threadIdx.x == 0) put_values(o, rr, row_values(rv, T::one(row, t), k, inv_t));
+    }
 }
 
 // dx from the saved lse (and entropy), 4 KiB of a row per workgroup.  Bound by HBM, reads and writes: 4,096 rows of 151,936
@@ -1981,12 +2009,13 @@ int rlx_token_logprob(const rlx_logits* x, const void* targets, int index_type, 
         });
         if (st != RLX_OK || cut.chunks == 1) return;
         st = for_row_launches(v.rows, kRowsPerLaunch, [&](uint32_t first, uint32_t here) {
+            const dim3 grid((here + kJoinRows - 1) / kJoinRows), block(kJoinBlock);
             if (entropy)
-                token_logprob_join_kernel<T, true><<<dim3(here), dim3(kJoinBlock), 0, s>>>(v, targets, wide, k, inv_t,
-                                                                                           partials, cut.chunks, o, first);
+                token_logprob_join_kernel<T, true><<<grid, block, 0, s>>>(v, targets, wide, k, inv_t, partials, cut.chunks, o, first,
+                                                                          here);
             else
-                token_logprob_join_kernel<T, false><<<dim3(here), dim3(kJoinBlock), 0, s>>>(v, targets, wide, k, inv_t,
-                                                                                            partials, cut.chunks, o, first);
+                token_logprob_join_kernel<T, false><<<grid, block, 0, s>>>(v, targets, wide, k, inv_t, partials, cut.chunks, o, first,
+                                                                           here);
         });
     });
     return st;
