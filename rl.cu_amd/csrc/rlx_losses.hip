@@ -617,7 +617,7 @@ __device__ __forceinline__ Stat join_chunks(const Stat* __restrict__ partials, i
 
 constexpr int kChunkBlock = 256, kJoinBlock = 256, kJoinRows = kJoinBlock / 64;
 
-// A row per wavefront (a workgroup per row took 3 to 5 us longer for 4,096 and 8,192 rows); the rare rows of a workgroup are
+// A row per wavefront (a workgroup per row took 2 to 4 us longer for 4,096 and 8,192 rows); the rare rows of a workgroup are
 // done again by all of it, one after the other.
 template <typename T, bool DOT>
 __global__ __launch_bounds__(kJoinBlock) void token_logprob_join_kernel(Logits x, const void* __restrict__ targets, int wide,
@@ -1293,7 +1293,7 @@ __device__ __forceinline__ RowTerms row_terms(const Policy& a, const Row& row, f
 // last-level cache mostly).  A row of 151,936 halves is 304 KB: it fits the 512 KB of registers of a compute unit, not its
 // 160 KB of LDS.  Every logit is read once and every gradient written once (FETCH_SIZE 1.54 GB, WRITE_SIZE 1.94 GB at 6,360
 // rows of 151,936 FP16, a fifth of them masked), which takes 663 us = 5.2 TB/s; reading the rows twice took 990, and
-// statistics and gradient as launches of their own, the second read from the last-level cache where it fits, 15 % more.
+// statistics and gradient as launches of their own 22 % more (4,096 unmasked rows: 479 and 586 us).
 // Bound by the memory system on this pattern of one long row per compute unit: without any arithmetic the same accesses
 // take 640 us, and workgroups that stay and load the next row while they write the present one gained nothing (272
 // against 274 us at 90,000 FP16).
