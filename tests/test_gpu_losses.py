@@ -206,11 +206,9 @@ def test_starts_of_rows(losses, T, name):
         assert (room == 7.0).all()
 
 
-@pytest.mark.parametrize("name", TYPES)
-@pytest.mark.parametrize("rows", [1, 40, 700])
-def test_masked_and_broken_rows(losses, T, name, rows):
+def broken_rows(T, name, rows, vocab):
+    """Rows with masked, lowest, infinite and NaN logits, ignored and bad targets; the kind of each, logits and targets (host)."""
     dt = getattr(T, name)
-    vocab = 3001
     lowest = T.finfo(dt).min
     x = (T.randn(rows, vocab, generator=T.Generator().manual_seed(rows)) * 2).to(dt)
     t = T.randint(0, 1000, (rows,), generator=T.Generator().manual_seed(3))
@@ -242,6 +240,13 @@ def test_masked_and_broken_rows(losses, T, name, rows):
             x[i, t[i]] = 1.5
         elif k == 10:
             x[i] = 3.25
+    return kinds, kind, x, t
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("rows,vocab", [(1, 3001), (40, 3001), (700, 3001), (1, 50001), (43, 50001), (130, 50001)])
+def test_masked_and_broken_rows(losses, T, name, rows, vocab):
+    kinds, kind, x, t = broken_rows(T, name, rows, vocab)
     xh, th = x.double().numpy(), t.numpy()
     x, t = x.cuda(), t.cuda()
     r = losses.token_logprobs(x, t, with_entropy=True)
@@ -262,6 +267,37 @@ def test_masked_and_broken_rows(losses, T, name, rows):
         elif k != 2:                                  # lse of an all-lowest row holds no log V
             d, size = LO.rows_grad(xh[i:i + 1], th[i:i + 1], 1.0, host(r.lse)[i:i + 1], np.ones(1))
             assert (np.abs(got[i] - d[0]) <= LO.grad_bound(name, d, size, U * 800)[0]).all(), kinds[k]
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("rows,vocab", [(40, 3001), (1, 50001), (43, 50001), (130, 50001), (13, 160003), (100, 160003)])
+@pytest.mark.parametrize("over", [False, True])
+def test_masked_and_broken_rows_in_the_loss(losses, T, name, rows, vocab, over):
+    """The loss straight from such logits, a sequence per row: with old_logp absent and the plain sum, dlogits = -A (1[j = t] - p)."""
+    kinds, kind, x, t = broken_rows(T, name, rows, vocab)
+    xh, th = x.double().numpy(), t.numpy()
+    x, t = x.cuda(), t.cuda()
+    adv = np.random.default_rng(rows).normal(size=rows).astype(np.float32)
+    cu = T.arange(rows + 1, dtype=T.int32).cuda()
+    r = losses.policy_loss_logits(x, t, T.tensor(adv).cuda(), cu_seqlens=cu, reduction="sum", with_entropy=True,
+                                  out=x if over else None)
+    logp, _, ent = LO.rows(xh, th, 1.0)
+    z, nz = LO.finite_max(xh), lambda a: np.nan_to_num(a, nan=0.0, neginf=0.0)
+    check(r.logp, logp, LO.slack(vocab, z, nz(logp)), "logp")
+    check(r.entropy, ent, 2 * LO.slack(vocab, z, np.log(vocab) + nz(ent)), "entropy")
+    got = host(r.dlogits)
+    for i, k in enumerate(kind):
+        if k in (6, 11):
+            assert (got[i] == 0).all()
+        elif k in (3, 4, 5, 7):
+            assert np.isnan(got[i]).all(), kinds[k]
+        else:
+            # of logits less their maximum: beside a lowest value of 1e38 even 64 bits hold no log V
+            off = xh[i:i + 1] - xh[i].max()
+            own = np.log(np.exp(off).sum(1))
+            d, size = LO.rows_grad(off, th[i:i + 1], 1.0, own, -adv[i:i + 1])
+            rel = LO.slack(vocab, z[i], np.log(vocab) + np.abs(nz(off - own)).clip(0, 200))
+            assert (np.abs(got[i] - d[0]) <= LO.grad_bound(name, d, size, rel)[0]).all(), kinds[k]
 
 
 @pytest.mark.parametrize("name,size,temperature", [("float16", 60000.0, 1.0), ("float16", 100.0, 1e-3),
