@@ -7,31 +7,33 @@
 
 #include <cstdio>
 #include <cstdlib>
+#include <vector>
 
 #include "kernels/adamw.h"
 #include "rlx_adamw.h"
 
 // Scratch memory of the loss operators, grown when a call needs more.  One per stream: calls on one stream may share it,
-// calls that can overlap may not.  Growing waits for the device, so a call that is to be recorded into a graph
-// has to be made once before (or reserve() called).
+// calls that can overlap may not.  What was handed out before stays allocated as long as the object, because a recorded graph
+// may still use it (sizes at least double, so that is less than the last block once more).  A call that is to be
+// recorded has to be made once before, or reserve() called: nothing can be allocated while a stream is recorded.
+// A copy starts without memory, and an assignment keeps what it has: there is nothing in it to copy.
 class LossWorkspace {
 public:
     LossWorkspace() = default;
-    LossWorkspace(const LossWorkspace&) = delete;
-    LossWorkspace& operator=(const LossWorkspace&) = delete;
-    ~LossWorkspace() { if (data_) (void)hipFree(data_); }
+    LossWorkspace(const LossWorkspace&) {}
+    LossWorkspace& operator=(const LossWorkspace&) { return *this; }
+    ~LossWorkspace() { for (void* p : blocks_) (void)hipFree(p); }
 
     void* reserve(int64_t bytes) {
         if (bytes < 0) RLX_CHECK(RLX_ERR_INVALID_ARG);
         if (bytes > bytes_) {
-            check(hipDeviceSynchronize());
-            if (data_) check(hipFree(data_));
-            data_ = nullptr;
-            bytes_ = 0;
-            check(hipMalloc(&data_, (size_t)bytes));
-            bytes_ = bytes;
+            const int64_t size = bytes > 2 * bytes_ ? bytes : 2 * bytes_;
+            void* p = nullptr;
+            check(hipMalloc(&p, (size_t)size));
+            blocks_.push_back(p);
+            bytes_ = size;
         }
-        return data_;
+        return blocks_.empty() ? nullptr : blocks_.back();
     }
     int64_t bytes() const { return bytes_; }
 
@@ -41,8 +43,8 @@ private:
         fprintf(stderr, "loss workspace: %s\n", hipGetErrorString(e));
         exit(1);
     }
-    void* data_ = nullptr;
-    int64_t bytes_ = 0;
+    std::vector<void*> blocks_;             // the last one is in use
+    int64_t bytes_ = 0;                     // its size
 };
 
 // Rows of contiguous logits, or of logits whose rows lie row_stride elements apart.

@@ -5,12 +5,14 @@
 //   3. policy loss from logits, the gradient over the logits    4. preference loss
 //   5. OptimStep::policy_step: the logits are the parameters themselves (one row of weights per token), so the
 //      gradient in the pool, the norm and the update can be checked end to end (the update against the C oracle, bit for bit)
+//   6. a recorded call replayed after its LossWorkspace has grown
 // Bounds: FP32 arithmetic on values of size 1 to 10 over 101 logits: 1e-5 is more than ten times what its roundings add up to
 // (each of at most 6e-8 of the value, fewer than ten of them on the way to a result, plus sums of 101 positive terms).
 #include <cmath>
 #include <cstdint>
 #include <cstdio>
 #include <cstring>
+#include <type_traits>
 #include <vector>
 
 #include "training/optim_step.h"
@@ -255,6 +257,45 @@ static void test_policy_step() {
     grad_pools_free(&grads);
 }
 
+static_assert(std::is_copy_constructible<OptimStep>::value && std::is_copy_assignable<OptimStep>::value,
+              "steps are held by value");
+
+// Rows of equal logits, long enough to need scratch memory: every log-probability is -log(vocabulary).
+static void test_workspace_grows() {
+    const char* name = "a recorded call replayed after its workspace has grown";
+    const int rows = 3, vocab = 20000;
+    Dev<float> x((size_t)rows * vocab), logp(rows), lse(rows);
+    Dev<int> t(rows);
+    const rlx_logits view = logit_rows(x.p, RLX_DTYPE_F32, rows, vocab);
+    const int64_t need = rlx_token_logprob_workspace(&view);
+    LossWorkspace ws;
+    hipStream_t s;
+    hipGraph_t graph;
+    hipGraphExec_t exec;
+    HIP_CHECK(hipStreamCreate(&s));
+    launch_token_logprob(view, t.p, 1.0f, logp.p, lse.p, nullptr, ws, s);
+    HIP_CHECK(hipStreamSynchronize(s));
+    HIP_CHECK(hipStreamBeginCapture(s, hipStreamCaptureModeThreadLocal));
+    launch_token_logprob(view, t.p, 1.0f, logp.p, lse.p, nullptr, ws, s);
+    HIP_CHECK(hipStreamEndCapture(s, &graph));
+    HIP_CHECK(hipGraphInstantiate(&exec, graph, nullptr, nullptr, 0));
+    const void* before = ws.reserve(need);
+    const bool moved = ws.reserve(need + 1) != before && ws.bytes() >= 2 * need && ws.reserve(need) != before;
+    LossWorkspace copy(ws);
+    double worst = need > 0 && moved && copy.bytes() == 0 ? 0.0 : 1.0;
+    for (int i = 0; i < 3; i++) {
+        HIP_CHECK(hipMemcpy(logp.p, std::vector<float>(rows, 7.0f).data(), rows * sizeof(float), hipMemcpyHostToDevice));
+        HIP_CHECK(hipGraphLaunch(exec, s));
+        HIP_CHECK(hipStreamSynchronize(s));
+        for (float v : logp.get()) worst = fmax(worst, fabs(v + log((double)vocab)));
+    }
+    // 20,000 equal terms of 1 and a logarithm near 10: sums that are exact, and two roundings of 6e-7
+    if (worst < 1e-5) PASS(name); else FAIL(name, "off by %g (%lld bytes)", worst, (long long)need);
+    (void)hipGraphExecDestroy(exec);
+    (void)hipGraphDestroy(graph);
+    (void)hipStreamDestroy(s);
+}
+
 int main() {
     int ndev = 0;
     if (hipGetDeviceCount(&ndev) != hipSuccess || ndev == 0) {
@@ -266,6 +307,7 @@ int main() {
     test_policy_logits();
     test_preference();
     test_policy_step();
+    test_workspace_grows();
     printf("=== %s (%d failures) ===\n", g_fails ? "FAILED" : "ALL PASSED", g_fails);
     return g_fails;
 }

@@ -824,4 +824,4 @@ def test_cpp_host_losses(torch_gpu):
     subprocess.run(["make", "-C", folder, "-s", "test_losses_host.bin"], check=True)
     res = subprocess.run([os.path.join(folder, "test_losses_host.bin")], capture_output=True, text=True, timeout=100)
     assert res.returncode == 0, res.stdout + res.stderr
-    assert res.stdout.count("[PASS]") == 5 and "[FAIL]" not in res.stdout
+    assert res.stdout.count("[PASS]") == 6 and "[FAIL]" not in res.stdout
