@@ -59,11 +59,27 @@ def hipcc_path():
 
 def build_library(verbose=False):
     """Compiles the library every time it is called; returns the path of the .so."""
-    cmd = [hipcc_path()] + HIPCC_FLAGS + ["-I", os.path.join(ROOT, "include"), "-o", OUT + ".tmp"] + SOURCES
-    res = subprocess.run(cmd, capture_output=True, text=True)
+    hipcc, objects, jobs = hipcc_path(), [], []
+    compile_flags = [f for f in HIPCC_FLAGS if f != "-shared"] + ["-I", os.path.join(ROOT, "include"), "-c"]
+    try:
+        for src in SOURCES:                       # side by side: the loss kernels alone take a minute and a half
+            objects.append("%s.%d.%s.o" % (OUT, os.getpid(), os.path.basename(src)))
+            jobs.append(subprocess.Popen([hipcc] + compile_flags + ["-o", objects[-1], src], stdout=subprocess.DEVNULL,
+                                         stderr=subprocess.PIPE, text=True))
+        stderr = [j.communicate()[1] for j in jobs]
+        failed = any(j.returncode != 0 for j in jobs)
+        if not failed:
+            res = subprocess.run([hipcc, "--offload-arch=gfx950", "-shared", "-o", OUT + ".tmp"] + objects,
+                                 capture_output=True, text=True)
+            stderr.append(res.stderr)
+            failed = res.returncode != 0
+    finally:
+        for path in objects:
+            if os.path.exists(path):
+                os.remove(path)
     noise = "packed-fp32-ops"
-    err = "\n".join(l for l in res.stderr.splitlines() if noise not in l)
-    if res.returncode != 0:
+    err = "\n".join(l for l in "".join(stderr).splitlines() if noise not in l)
+    if failed:
         raise RuntimeError("hipcc failed:\n" + err)
     if verbose and err.strip():
         print(err)

@@ -1790,7 +1790,7 @@ struct Cut {
 // Rows up to 4,096 groups (32,768 halves) go whole to a workgroup, which writes their results in the same launch; longer
 // ones in 32 KiB chunks that a second launch joins, or in 8 KiB ones where those would not fill the chip.  Recorded and
 // replayed, whole / in chunks: 32,000 FP16, 1 row 4.2 / 4.8 us, 256 rows 6.6 / 8.8, 8,192 rows 79 / 89; 16,384 FP32 256 rows
-// 6.1 / 8.3; 50,257 FP16 1 row 5.7 / 4.8, 8,192 rows 153 / 147.  In between, for 97 to 256 rows, a launch less weighs more
+// 6.1 / 8.3; 50,257 FP16 1 row 5.7 / 4.8, 8,192 rows 153 / 147.  (512 x 6 beside 512 x 8: 16,384 rows of 17,000 97 / 106.)  In between, for 97 to 256 rows, a launch less weighs more
 // than what the few lanes of a workgroup cost: 129 rows of 50,257 FP16 7.8 / 9.1 us, of 90,000 9.7 / 10.0; 64 rows 7.5 / 7.3
 // and 9.2 / 7.7; beyond 12,288 groups chunks do better for any number of rows (129 rows of 151,936 13.9 / 12.3).
 Cut cut_of(const rlx_logits& x) {
@@ -1798,6 +1798,7 @@ Cut cut_of(const rlx_logits& x) {
     if (groups <= 64 * 8) return {64, 8, 1};
     if (groups <= 128 * 8) return {128, 8, 1};
     if (groups <= 256 * 8) return {256, 8, 1};
+    if (groups <= 512 * 6) return {512, 6, 1};
     if (groups <= 512 * 8) return {512, 8, 1};
     if (x.rows > 96 && x.rows <= 256) {
         if (groups <= 512 * 14) return {512, 14, 1};
@@ -1947,6 +1948,7 @@ template <typename Fn>
 void for_cut(const Cut& c, Fn f) {
     if (c.block == 64) f(Int<64>{}, Int<8>{});
     else if (c.block == 128) f(Int<128>{}, Int<8>{});
+    else if (c.block == 512 && c.per_lane == 6) f(Int<512>{}, Int<6>{});
     else if (c.block == 512 && c.per_lane == 8) f(Int<512>{}, Int<8>{});
     else if (c.block == 512) f(Int<512>{}, Int<14>{});
     else if (c.block == 1024) f(Int<1024>{}, Int<12>{});
@@ -1954,16 +1956,26 @@ void for_cut(const Cut& c, Fn f) {
     else f(Int<256>{}, Int<2>{});
 }
 
-// Calls f(lanes, 16-byte groups per lane) for the shape that holds a row of `groups` groups in registers.
+// Calls f(lanes, 16-byte groups per lane) for the shape that holds a row of `groups` groups in registers.  Groups that a shape
+// has and the row has not are loaded all the same (the last one again), so the steps are small: with 512 x 8, 512 x 14, 1,024 x
+// 12 and 1,024 x 19 alone 17,000 FP16 took 255 us for 300 M logits, not 233, 36,000 239 and 225, 64,000 265 and 221, 100,000
+// 277 and 252, 128,256 243 and 233.  Two workgroups of 512 lanes do better on a compute unit than one of 1,024 (64,000 as
+// 1,024 x 8: 230), as long as they have the registers (98,304 as 512 x 24: 246, as 1,024 x 12 236).
 template <typename Fn>
 void for_row_shape(int groups, Fn f) {
     if (groups <= 64 * 4) f(Int<64>{}, Int<4>{});
     else if (groups <= 64 * 8) f(Int<64>{}, Int<8>{});
     else if (groups <= 128 * 8) f(Int<128>{}, Int<8>{});
     else if (groups <= 256 * 8) f(Int<256>{}, Int<8>{});
+    else if (groups <= 512 * 6) f(Int<512>{}, Int<6>{});
     else if (groups <= 512 * 8) f(Int<512>{}, Int<8>{});
+    else if (groups <= 512 * 10) f(Int<512>{}, Int<10>{});
     else if (groups <= 512 * 14) f(Int<512>{}, Int<14>{});
+    else if (groups <= 512 * 16) f(Int<512>{}, Int<16>{});
+    else if (groups <= 1024 * 10) f(Int<1024>{}, Int<10>{});
     else if (groups <= 1024 * 12) f(Int<1024>{}, Int<12>{});
+    else if (groups <= 1024 * 14) f(Int<1024>{}, Int<14>{});
+    else if (groups <= 1024 * 16) f(Int<1024>{}, Int<16>{});
     else f(Int<1024>{}, Int<19>{});
 }
 

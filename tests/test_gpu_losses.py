@@ -550,6 +550,40 @@ def test_policy_loss_logits_equals_the_separate_operators(losses, T):
     assert (r.dlogits[~mask] == 0).all()
 
 
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("vocab", [24000, 24575, 33001, 50257, 64007, 65536, 80001, 98304, 110001, 128256, 151936, 155657])
+def test_every_shape_of_a_row(losses, T, name, vocab):
+    """Rows of each size that is held in registers, masked and partly banned, against the separate operators in FP32.
+
+    Both have the same logits; what differs is the type that the gradient is rounded to (half a step relative to itself) and
+    the two computations' own errors, each within slack(); values below the type's smallest step are off by half of one.
+    """
+    rows = 97
+    g = T.Generator(device="cuda").manual_seed(vocab)
+    x = (T.randn(rows, vocab, generator=g, device="cuda") * 2.5).to(getattr(T, name))
+    x[:, vocab // 3:vocab // 3 + 40] = -math.inf
+    t = T.randint(0, vocab // 3, (rows,), generator=g, device="cuda")
+    t[5], t[6], t[7] = vocab - 1, 0, -1
+    adv = T.randn(rows, generator=g, device="cuda")
+    cu = T.arange(rows + 1, dtype=T.int32, device="cuda")
+    x32 = x.float()
+    f = losses.token_logprobs(x32, t, with_entropy=True)
+    for ec in (0.0, 0.5):
+        r = losses.policy_loss_logits(x, t, adv, cu_seqlens=cu, reduction="sum", entropy_coef=ec, with_entropy=True)
+        dh = T.full_like(adv, -ec) if ec else None
+        d = losses.token_logprobs_backward(x32, t, f.lse, -adv, entropy=f.entropy if ec else None, dentropy=dh)
+        lp = (x32 - f.lse[:, None]).abs().nan_to_num(posinf=0.0)
+        zmax = 16.0                                     # of 1.6e7 normal values times 2.5
+        rel = 2 * U * (4 * zmax + 6 * lp + vocab / 256 + 40 + 8)
+        p = T.exp(x32 - f.lse[:, None]) * (t >= 0)[:, None]
+        size = adv.abs()[:, None] * p + ec * p * (lp + f.entropy[:, None] + 1)
+        size[T.arange(rows).cuda()[t >= 0], t[t >= 0]] += adv.abs()[t >= 0]
+        bound = d.abs() * (LO.EPS[name] * 1.01) + size * rel + LO.TINY[name]
+        assert x32.isfinite().logical_not().sum() == rows * 40 and x32.nan_to_num(neginf=0.0).abs().max() <= zmax
+        assert bool(((r.dlogits.float() - d).abs() <= bound).all()), "entropy_coef %g" % ec
+        assert T.allclose(r.logp, f.logp, rtol=1e-5, atol=2e-5) and T.allclose(r.entropy, f.entropy, rtol=2e-5, atol=2e-5)
+
+
 def test_gradient_of_the_logits_against_differences(losses, T):
     """Differences of the loss itself (in 64 bits) in some of the logits."""
     rows, vocab = 6, 37
