@@ -275,8 +275,9 @@ int rlx_plan_schedule_overrun(rlx_plan* plan, int64_t* overrun, void* stream);
  *  - Scratch memory is the caller's: `workspace` (device, 16-byte aligned, contents arbitrary) of
  *    at least the bytes that the operator's _workspace function returns.  Two calls that may overlap
  *    (two streams, two recorded graphs) need a workspace each; calls on one stream may share one.
- *  - Softmax statistics and sums are FP32 per lane, sums over tokens FP64; a result is rounded
- *    once, to its own type.
+ *  - Softmax statistics and the gradient of the logits are computed in FP32 (the latter rounded to the
+ *    logits' type at the end).  What a loss makes of log-probabilities, its weights and its sums over
+ *    tokens are FP64, rounded to FP32 once.
  *  - Outputs do not overlap inputs or each other, except for dx, which may be x.
  *  - A row (token) that is masked out, or whose target is negative, is IGNORED: its logits, log
  *    probabilities and so on are not used whatever they hold (NaN included), its outputs are 0 and its
@@ -340,7 +341,7 @@ enum {
  *                       + kl_coef (exp(d) - d - 1) - entropy_coef entropy),
  *     dlogp[t] = grad_scale w_t (-A rho [not clipped] + kl_coef (1 - exp(d))),
  *     dentropy[t] = -grad_scale w_t entropy_coef.
- * "Clipped" is logp - old_logp > log(1 + clip_high) for A >= 0, < log(1 - clip_low) for A < 0, decided as if in 48 bits.
+ * "Clipped" is logp - old_logp > log(1 + clip_high) for A >= 0, < log(1 - clip_low) for A < 0, decided in FP64.
  * old_logp NULL: rho is 1 (logp is its own old value).  ref_logp NULL: no KL term.
  * Sequence s is the tokens [cu_seqlens[s], cu_seqlens[s + 1]) of the packed arrays; cu_seqlens NULL: n_seqs
  * sequences of tokens / n_seqs tokens each (a padded batch).  Sequences may be empty.  Tokens in

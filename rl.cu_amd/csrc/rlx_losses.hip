@@ -772,9 +772,9 @@ __device__ __forceinline__ int64_t wave_offsets_up_to(const RLX_GLOBAL int32_t* 
 struct Policy {             // rlx_policy_args as the kernels take it
     const float *old_logp, *ref_logp, *advantages, *entropy;
     Batch batch;
-    float log_high[2], log_low[2]; // borders of the clip, each as a sum of two
+    double log_high, log_low;      // borders of the clip
+    double high, low;              // 1 + clip_high, 1 - clip_low
     double norm;
-    float high, low;               // 1 + clip_high, 1 - clip_low
     float kl_coef, entropy_coef, grad_scale;
     int reduction, per_token;
 };
@@ -786,56 +786,54 @@ struct Terms {
     int64_t count;
 };
 
-// exp(d) - 1 and exp(d) - 1 - d.  Near 0 the second is a Taylor series (the direct form would lose everything to
-// cancellation): the first term left out is below 2^-25 of the sum for |d| < 1/2.
-__device__ __forceinline__ void kl_of(float d, float& em1, float& kl) {
-    if (fabsf(d) < 0.5f) {
-        float p = 1.0f / 3628800.0f;
-        p = __builtin_fmaf(p, d, 1.0f / 362880.0f);
-        p = __builtin_fmaf(p, d, 1.0f / 40320.0f);
-        p = __builtin_fmaf(p, d, 1.0f / 5040.0f);
-        p = __builtin_fmaf(p, d, 1.0f / 720.0f);
-        p = __builtin_fmaf(p, d, 1.0f / 120.0f);
-        p = __builtin_fmaf(p, d, 1.0f / 24.0f);
-        p = __builtin_fmaf(p, d, 1.0f / 6.0f);
-        p = __builtin_fmaf(p, d, 0.5f);
-        kl = p * d * d;
-        em1 = d + kl;
-    } else {
-        em1 = expf(d) - 1.0f;
-        kl = em1 == INFINITY ? em1 : em1 - d;
-    }
+// exp(x), exp(x) - 1 and exp(x) - 1 - x in FP64, within 2^-41, 2^-39 and 2^-37 of themselves.  x = n ln 2 + r with
+// |r| <= ln 2 / 2, and exp(r) = 1 + r + r^2 q(r) with q the Taylor series up to r^10 (the first term left out is below 2^-42).
+// For n = 0 the last two are r + r^2 q and r^2 q as they stand, where differences of exp(x) would lose everything.
+// The factors of the series are scalar operands: left to itself the compiler puts each into a pair of vector registers, and
+// policy_loss_kernel has 82 of them, not 68.
+struct Exp {
+    double e, less1, less_x;
+};
+
+__device__ __forceinline__ Exp exp_of(double x) {
+    const double top = x > 2000.0 ? 2000.0 : x, in = top < -2000.0 ? -2000.0 : top;      // NaN stays
+    const double n = __builtin_rint(in * 1.4426950408889634), r = __builtin_fma(n, -0.6931471805599453, in);
+    double q = 1.0 / 3628800.0;
+    for (const double c : {1.0 / 362880.0, 1.0 / 40320.0, 1.0 / 5040.0, 1.0 / 720.0, 1.0 / 120.0, 1.0 / 24.0, 1.0 / 6.0, 0.5})
+        asm("v_fma_f64 %0, %1, %2, %3" : "=v"(q) : "v"(q), "v"(r), "s"(c));
+    q *= r * r;
+    const double rq = r + q;
+    Exp o;
+    o.e = __builtin_amdgcn_ldexp(1.0 + rq, (int)n);
+    const double far = o.e - 1.0;
+    o.less1 = n == 0.0 ? rq : far;
+    o.less_x = n == 0.0 ? q : far == (double)INFINITY ? far : far - x;
+    return o;
 }
 
+// What follows from the log-probabilities is computed in FP64 and rounded once, as a gradient or as a sum.  (Differences of
+// FP32 values are exact there, so the side of the clip's border is, too.)  With weights, products and exponentials in FP32,
+// up to a quarter of the gradients were off by more than that, by up to three roundings; it took 16.8 us for 1.6 M tokens, and
+// 19.0 this way.
 struct TokenLoss {
-    float policy, kl, ratio, slope;      // slope: gradient of the token's loss by its log-probability
+    double policy, kl, ratio, slope;     // slope: gradient of the token's loss by its log-probability
     bool clipped;
 };
 
 // old and ref are used only where the batch has them.
 __device__ __forceinline__ TokenLoss token_loss(const Policy& a, float logp, float old, float ref, float advantage) {
     TokenLoss o;
-    // The side of the border is decided as if in 48 bits: lr + rest is the inputs' difference exactly, and near the border
-    // its difference from the border's upper part is exact too.  (1.6 M tokens: 15.6 us, and 16.0 with this and the weighted
-    // terms in FP64.)
-    float lr = 0.0f, rest = 0.0f;
-    if (a.old_logp) {
-        lr = logp - old;
-        const float back = lr - logp;
-        rest = (logp - (lr - back)) - (old + back);
-        if (!(fabsf(rest) < INFINITY)) rest = 0.0f;          // of infinities
-    }
-    o.clipped = advantage >= 0.0f ? (lr - a.log_high[0]) + (rest - a.log_high[1]) > 0.0f
-                                  : (lr - a.log_low[0]) + (rest - a.log_low[1]) < 0.0f;
-    o.ratio = expf(lr);
+    const double lr = a.old_logp ? (double)logp - (double)old : 0.0, adv = (double)advantage;
+    o.clipped = advantage >= 0.0f ? lr > a.log_high : lr < a.log_low;
+    o.ratio = exp_of(lr).e;
     // min(rho A, clip(rho) A) without the product of an infinite rho and A = 0
-    o.policy = -(advantage * (o.clipped ? (advantage >= 0.0f ? a.high : a.low) : o.ratio));
-    o.slope = o.clipped ? 0.0f : -(advantage * o.ratio);
-    o.kl = 0.0f;
+    o.policy = -(adv * (o.clipped ? (advantage >= 0.0f ? a.high : a.low) : o.ratio));
+    o.slope = o.clipped ? 0.0 : -(adv * o.ratio);
+    o.kl = 0.0;
     if (a.ref_logp) {
-        float em1;
-        kl_of(ref - logp, em1, o.kl);
-        if (a.kl_coef != 0.0f) o.slope -= a.kl_coef * em1;
+        const Exp x = exp_of((double)ref - (double)logp);
+        o.kl = x.less_x;
+        if (a.kl_coef != 0.0f) o.slope -= (double)a.kl_coef * x.less1;
     }
     return o;
 }
@@ -1002,18 +1000,19 @@ __device__ __forceinline__ uint32_t tokens_within(int64_t at, int64_t from, int6
 
 // What a lane adds up over its few tokens.
 struct LaneTerms {
-    float policy, kl, entropy, ratio;      // the first three weighted
+    double policy, kl, entropy, ratio;     // the first three weighted
     int clipped, count;
 };
 
 // A token's weight as it is used: in the loss, in the gradients of logp and of the entropy.
 struct Weight {
-    float loss, logp, entropy;
+    double loss, logp;
+    float entropy;
 };
 
 __device__ __forceinline__ Weight weights(const Policy& a, int64_t count) {
     const double w = weight_of(a, count), g = w * (double)a.grad_scale;
-    return {(float)w, (float)g, (float)(g * -(double)a.entropy_coef)};
+    return {w, g, (float)(g * -(double)a.entropy_coef)};
 }
 
 // One token's share of the loss; returns its gradient.
@@ -1022,15 +1021,15 @@ __device__ __forceinline__ float add_token(const Policy& a, const Weight& w, flo
     const TokenLoss o = token_loss(a, logp, old, ref, advantage);
     v.policy += w.loss * o.policy;
     v.kl += w.loss * o.kl;
-    v.entropy += w.loss * entropy;
+    v.entropy += w.loss * (double)entropy;
     v.ratio += o.ratio;
     v.clipped += o.clipped ? 1 : 0;
     v.count++;
-    return w.logp * o.slope;
+    return (float)(w.logp * o.slope);
 }
 
 __device__ __forceinline__ Terms terms_of(const LaneTerms& v) {
-    return {(double)v.policy, (double)v.kl, (double)v.entropy, (double)v.clipped, (double)v.ratio, v.count};
+    return {v.policy, v.kl, v.entropy, (double)v.clipped, v.ratio, v.count};
 }
 
 // --- the workgroup of a launch that finishes last ------------------------------------------------------------------------
@@ -1099,9 +1098,9 @@ constexpr int kTokensPerBlock = 4 * kTokenBlock;
 // Policy loss over log-probabilities (of at least four tokens): a workgroup takes kTokensPerBlock tokens, a lane four in a
 // row; the quads of the lanes at the end of the arrays move back into them.  The sequences of a workgroup's first
 // and last token are searched once; only where they differ does a lane search between them.
-// 1.6 M tokens with every input (46 MB): 15.4 us, of which the arithmetic is 8 (193 vector instructions a token) and
-// the memory 9; all wavefronts are resident at once, so the two overlap little.  A token per lane took 37.  (The partial
-// terms are added by a launch of its own, 4 us: with tickets, as few rows do it, 1,562 workgroups took 14 us longer.)
+// 1.6 M tokens with every input (46 MB): 19 us; the memory alone takes 9, and as all wavefronts are resident at once (72
+// registers or fewer), it overlaps little with the arithmetic.  A token per lane took 37.  (The partial terms are added by a
+// launch of its own, 4 us: with tickets, as few rows do it, 1,562 workgroups took 14 us longer.)
 __global__ __launch_bounds__(kTokenBlock) void policy_loss_kernel(Policy a, const float* __restrict__ logp,
                                                                   const int32_t* __restrict__ seq_counts,
                                                                   float* __restrict__ dlogp, float* __restrict__ dentropy,
@@ -1115,29 +1114,28 @@ __global__ __launch_bounds__(kTokenBlock) void policy_loss_kernel(Policy a, cons
     Tokens4 x = load_tokens(a, logp, t0);
     x.in &= tokens_within(t0, own, tokens);
     // offsets up to a token: its sequence is one less (0: in front of the first, n_seqs + 1: behind the last)
-    int64_t lo, hi, len = 1;
+    uint32_t lo, hi, len = 1;
     if (cu) {
-        lo = wave_offsets_up_to(cu, 0, n_seqs + 1, begin);
-        hi = wave_offsets_up_to(cu, lo, n_seqs + 1, end - 1);
+        lo = (uint32_t)wave_offsets_up_to(cu, 0, n_seqs + 1, begin);
+        hi = (uint32_t)wave_offsets_up_to(cu, lo, n_seqs + 1, end - 1);
     } else {
-        len = tokens / n_seqs;
-        lo = begin / len + 1;
-        hi = (end - 1) / len + 1;
+        len = (uint32_t)(tokens / n_seqs);
+        lo = (uint32_t)begin / len + 1;
+        hi = (uint32_t)(end - 1) / len + 1;
     }
     const int64_t total = a.reduction == RLX_LOSS_TOKEN_MEAN ? count_for(a, seq_counts, 0) : 1;
-    int64_t at = lo, weighed = -1;
-    if (lo != hi) at = cu ? offsets_up_to(cu, lo, hi, t0) : t0 / len + 1;
-    Weight w = {0.0f, 0.0f, 0.0f};
+    uint32_t at = lo, weighed = 0;
+    if (lo != hi) at = cu ? (uint32_t)offsets_up_to(cu, lo, hi, t0) : (uint32_t)t0 / len + 1;
+    Weight w = {0.0, 0.0, 0.0f};
     float advantage = 0.0f;
-    LaneTerms v = {0.0f, 0.0f, 0.0f, 0.0f, 0, 0};
+    LaneTerms v = {0.0, 0.0, 0.0, 0.0, 0, 0};
     f32x4_any g = {0.0f, 0.0f, 0.0f, 0.0f}, dh = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const int64_t t = t0 + i;
         if (cu) {
-            while (at < hi && cu[at] <= t) at++;
+            while (at < hi && cu[at] <= t0 + i) at++;
         } else if (lo != hi) {
-            at = t / len + 1;
+            at = ((uint32_t)t0 + i) / len + 1;
         }
         if ((x.in >> (8 * i) & 0x80u) && at >= 1 && at <= n_seqs) {
             if (weighed != at) {
@@ -1227,7 +1225,7 @@ __global__ __launch_bounds__(BLOCK) void policy_loss_small_kernel(Policy a, cons
         for (int s = tid; s < slots; s += BLOCK) total += many ? (in_seq[s] > 0 ? 1 : 0) : in_seq[s];
         total = sum_block<BLOCK>(total, shared_m);
     }
-    LaneTerms v = {0.0f, 0.0f, 0.0f, 0.0f, 0, 0};
+    LaneTerms v = {0.0, 0.0, 0.0, 0.0, 0, 0};
 #pragma unroll
     for (int i = 0; i < kSmallPerLane; i++) {
         const int t = tid + i * BLOCK;
@@ -1281,10 +1279,9 @@ __device__ __forceinline__ RowTerms row_terms(const Policy& a, const Row& row, f
     const double w = weight_of(a, m);
     o.values = row_values(row, zt, k, inv_t);
     const TokenLoss l = token_loss(a, o.values.logp, old, ref, advantage);
-    const float ws = (float)w * (inv_t * a.grad_scale);
-    o.grad = row_gradient(row, o.values, ws * l.slope, DOT ? -(ws * a.entropy_coef) : 0.0f);
-    o.terms = {w * (double)l.policy, w * (double)l.kl, w * (double)o.values.entropy, l.clipped ? 1.0 : 0.0,
-               (double)l.ratio, 1};
+    const double ws = w * (double)a.grad_scale * (double)inv_t;
+    o.grad = row_gradient(row, o.values, (float)(ws * l.slope), DOT ? (float)-(ws * (double)a.entropy_coef) : 0.0f);
+    o.terms = {w * l.policy, w * l.kl, w * (double)o.values.entropy, l.clipped ? 1.0 : 0.0, l.ratio, 1};
     return o;
 }
 
@@ -1881,13 +1878,10 @@ int make_policy(const rlx_policy_args* p, int64_t tokens, Policy& a) {
     if (p->clip_low < 0.0f || p->clip_low > 1.0f || p->clip_high < 0.0f) return RLX_ERR_BAD_HYPER;
     if (tokens > 0 && !p->advantages) return RLX_ERR_INVALID_ARG;
     if (!floats_aligned({p->old_logp, p->ref_logp, p->advantages, p->entropy})) return RLX_ERR_MISALIGNED;
-    const double high = std::log1p((double)p->clip_high), low = std::log1p(-(double)p->clip_low);
-    a.log_high[0] = (float)high;
-    a.log_high[1] = (float)(high - (double)a.log_high[0]);
-    a.log_low[0] = (float)low;                              // -inf for clip_low = 1: nothing is below it
-    a.log_low[1] = std::isfinite(low) ? (float)(low - (double)a.log_low[0]) : 0.0f;
-    a.high = (float)(1.0 + (double)p->clip_high);
-    a.low = (float)(1.0 - (double)p->clip_low);
+    a.log_high = std::log1p((double)p->clip_high);
+    a.log_low = std::log1p(-(double)p->clip_low);           // -inf for clip_low = 1: nothing is below it
+    a.high = 1.0 + (double)p->clip_high;
+    a.low = 1.0 - (double)p->clip_low;
     a.norm = (double)p->norm;
     a.kl_coef = p->kl_coef;
     a.entropy_coef = p->entropy_coef;

@@ -1,0 +1,110 @@
+"""What the loss operators promise beyond ordinary rows and sizes, on the GPU: one rounding of what is computed in 64 bits,
+gradients of near-certain targets and of rows whose log-sum-exp tells nothing, results that hold no scratch memory, and
+gradients over the logits that autograd and the allocator know of."""
+import importlib
+import math
+import weakref
+
+import numpy as np
+import pytest
+
+import loss_oracle as LO
+
+pytestmark = pytest.mark.gpu
+
+U = LO.U
+TYPES = ["float16", "bfloat16", "float32"]
+
+
+@pytest.fixture(scope="module")
+def T(torch_gpu):
+    return torch_gpu
+
+
+@pytest.fixture(scope="module")
+def losses(pkg, torch_gpu):
+    return importlib.import_module(pkg.__name__ + ".losses")
+
+
+def host64(t):
+    return t.detach().cpu().double().numpy()
+
+
+def within(got, want, bound, what):
+    got, want = host64(got), np.asarray(want, np.float64)
+    assert got.shape == want.shape, what
+    bound = np.broadcast_to(bound, want.shape)
+    off = np.abs(got - want)
+    bad = ~(off <= bound)
+    assert not bad.any(), "%s: %d of %d off, worst by %.3g of %.3g where %.3g is allowed" % (
+        what, bad.sum(), bad.size, off[np.argmax(off - bound)], want.reshape(-1)[np.argmax(off - bound)],
+        bound.reshape(-1)[np.argmax(off - bound)])
+
+
+# --- one rounding of what is computed in 64 bits ---------------------------------------------------------------------------
+
+# Errors of one token's terms in FP64: 2^-53 for each difference, product and quotient, and for the exponential, e^d - 1 and
+# e^d - d - 1 below 2^-40, 2^-38 and 2^-36 of themselves (a series up to r^10 with |r| <= ln 2 / 2).  Sums add at most a few
+# thousand times 2^-53.  2^-34 of the terms' sizes covers it, a thousandth of an FP32 rounding.
+REL64 = 2.0 ** -34
+FLUSHED = 2.0 ** -126
+
+
+def once(want, size):
+    """Bound of a value that is computed in 64 bits and rounded to FP32 at the end."""
+    return np.abs(want) * U * (1.0 + 1e-6) + size * REL64 + FLUSHED
+
+
+def cancelling(rng, tokens, n_seqs, per_token):
+    """Log-probabilities, old and reference ones, and advantages of either sign whose loss is far below its terms."""
+    lp = -rng.exponential(1.0, tokens)
+    old, ref = lp - rng.normal(0, 0.15, tokens), lp + rng.normal(0, 0.4, tokens)
+    n = tokens if per_token else n_seqs
+    adv = rng.normal(0, 1, n) + np.where(np.arange(n) % 2, 3.0, -3.0)
+    return [a.astype(np.float32) for a in (lp, old, ref, rng.random(tokens) * 3, adv)]
+
+
+@pytest.mark.parametrize("reduction", ["sequence", "token", "sum"])
+@pytest.mark.parametrize("cu", [[0, 5], [1, 8, 10, 13], [0, 300, 307, 900, 2000], [0, 7, 1200, 4001, 4003, 30000],
+                                list(range(0, 700 * 13 + 1, 13))], ids=lambda c: "%d-%d" % (len(c) - 1, c[-1]))
+def test_policy_loss_is_rounded_once(losses, T, cu, reduction):
+    tokens, n_seqs = cu[-1] + 2, len(cu) - 1
+    seq = LO.sequences(tokens, cu)
+    cu_t = T.tensor(np.array(cu, np.int32)).cuda()
+    for variant in range(3):
+        rng = np.random.default_rng(tokens + variant)
+        per_token = variant != 1 or n_seqs == 1
+        lp, old, ref, ent, adv = cancelling(rng, tokens, n_seqs, per_token)
+        mask = rng.random(tokens) < 0.8
+        kw = dict(clip_low=0.2, clip_high=0.3, kl_coef=0.07 if variant else 0.0, entropy_coef=0.013 if variant == 2 else 0.0,
+                  reduction=reduction, norm=0.3, grad_scale=3.0)
+        put = lambda a: T.tensor(a).cuda()  # noqa: E731
+        r = losses.policy_loss(put(lp), put(adv), old_logp=put(old), ref_logp=put(ref), entropy=put(ent),
+                               mask=put(mask), cu_seqlens=cu_t, **kw)
+        stats, n, dlogp, dent, size, terms, _ = LO.policy(lp, adv, seq, n_seqs, mask, old=old, ref=ref, entropy=ent, **kw)
+        assert int(r.tokens) == n
+        within(r.dlogp, dlogp, once(dlogp, size), "dlogp, variant %d" % variant)
+        if kw["entropy_coef"]:
+            within(r.dentropy, dent, once(dent, np.abs(dent)), "dentropy")
+        within(r.stats, stats, once(stats, terms), "statistics, variant %d" % variant)
+
+
+@pytest.mark.parametrize("rows", [14, 130])
+def test_statistics_of_the_loss_from_logits_are_rounded_once(losses, T, rows):
+    """Given the log-probabilities and entropies that the call returns (FP32), its statistics are sums in 64 bits."""
+    vocab = 20001
+    gen = T.Generator().manual_seed(rows)
+    x = (T.randn(rows, vocab, generator=gen) * 2).cuda()
+    t = T.randint(0, vocab, (rows,), generator=gen).cuda()
+    cu = [0, 3, rows - 4, rows]
+    rng = np.random.default_rng(rows)
+    for reduction in ("sequence", "token", "sum"):
+        lp = losses.token_logprobs(x, t).logp
+        _, noise, shift, _, adv = cancelling(rng, rows, 3, True)
+        old, ref = lp + T.tensor(noise).cuda() * 0.1, lp + T.tensor(shift).cuda() * 0.1
+        kw = dict(kl_coef=0.07, entropy_coef=0.013, reduction=reduction, norm=0.3)
+        r = losses.policy_loss_logits(x, t, T.tensor(adv).cuda(), old_logp=old, ref_logp=ref, with_entropy=True,
+                                      cu_seqlens=T.tensor(cu, dtype=T.int32).cuda(), **kw)
+        stats, n, _, _, _, terms, _ = LO.policy(r.logp.cpu().numpy(), adv, LO.sequences(rows, cu), 3, np.ones(rows, bool),
+                                                old=old.cpu().numpy(), ref=ref.cpu().numpy(), entropy=r.entropy.cpu().numpy(), **kw)
+        within(r.stats, stats, once(stats, terms), reduction)
