@@ -321,11 +321,18 @@ int rlx_token_logprob(const rlx_logits* x, const void* targets, int index_type, 
  * p = exp(z - lse) (so the lse has to tell: that of a row of the type's lowest value only does not hold log vocab).  A row
  * whose two gradients are 0 gets zeros without being read.  dx has x's rows, vocab and dtype;
  * it may be x itself (same data and strides) but may not overlap it otherwise.
+ * An lse of FP32 leaves a probability off by up to 2^-24 |lse| of itself, and so the target's 1 - p by up to
+ * 2^-24 |lse| / (1 - p) of itself: nothing of it is left where 1 - p is below that.  The second form takes
+ * rlx_token_logprob's logp too (NULL: as the first form), from which the target's own gradient keeps the
+ * precision of 1 - p, as in rlx_policy_loss_logits.
  * Replaces the backward half of the log-softmax gather (src/model/qwen3.cu:170).
  */
 int rlx_token_logprob_backward(const rlx_logits* x, const void* targets, int index_type, float temperature,
                                const float* lse, const float* entropy, const float* dlogp, const float* dentropy,
                                const rlx_logits* dx, void* stream);
+int rlx_token_logprob_backward_logp(const rlx_logits* x, const void* targets, int index_type, float temperature,
+                                    const float* lse, const float* entropy, const float* logp, const float* dlogp,
+                                    const float* dentropy, const rlx_logits* dx, void* stream);
 
 /* Weights w of the tokens in a loss (m = tokens that count: not masked, target not negative): */
 enum {

@@ -93,6 +93,8 @@ SIGNATURES = {
     "rlx_token_logprob": ([C.POINTER(Logits), _VP, _INT, _F, _VP, _VP, _VP, _VP, _I64, _VP], _INT),
     "rlx_token_logprob_backward": ([C.POINTER(Logits), _VP, _INT, _F, _VP, _VP, _VP, _VP, C.POINTER(Logits), _VP],
                                    _INT),
+    "rlx_token_logprob_backward_logp": ([C.POINTER(Logits), _VP, _INT, _F, _VP, _VP, _VP, _VP, _VP, C.POINTER(Logits),
+                                         _VP], _INT),
     "rlx_policy_loss_workspace": ([_I64, _I64], _I64),
     "rlx_policy_loss": ([_VP, _I64, C.POINTER(PolicyArgs), _VP, _VP, _VP, _VP, _I64, _VP], _INT),
     "rlx_policy_loss_logits_workspace": ([C.POINTER(Logits), _I64], _I64),
@@ -107,7 +109,7 @@ SIGNATURES = {
 _lib = None
 
 
-ABI_VERSION = 110        # rlx_version() of the library this binding was written against
+ABI_VERSION = 111        # rlx_version() of the library this binding was written against
 
 
 def load():

@@ -656,11 +656,14 @@ __global__ __launch_bounds__(kJoinBlock) void token_logprob_join_kernel(Logits x
 // dx from the saved lse (and entropy), 4 KiB of a row per workgroup.  Bound by HBM, reads and writes: 4,096 rows of 151,936
 // BF16, a quarter of them ignored, 335 us = 6.5 TB/s (8 KiB per workgroup 357, 16 KiB 372, a workgroup per row 437); rows
 // that do not start on 16 bytes do better with half the lanes and two groups each (50,257 BF16: 143 against 156 us).
-// p = exp(z - lse) is formed as 2^((z/T - lse) log2 e), the difference first, so that the rounding is of the size of log p.
+// p = exp(z - lse) is formed as 2^((z/T - lse) log2 e), the difference first; what it inherits is the rounding of lse, up to
+// u |lse| of p (u = 2^-24) and, at a target, u |lse| / (1 - p) of 1 - p.  Where log p of the target is given, its own gradient
+// comes from that and keeps the precision of 1 - p.
 template <typename T, int BLOCK, int NG, bool DOT, bool ONCE>
 __global__ __launch_bounds__(BLOCK) void token_logprob_backward_kernel(
     Logits x, Logits dx, const void* __restrict__ targets, int wide, float inv_t, const float* __restrict__ lse,
-    const float* __restrict__ entropy, const float* __restrict__ dlogp, const float* __restrict__ dentropy, uint32_t first) {
+    const float* __restrict__ entropy, const float* __restrict__ logp, const float* __restrict__ dlogp,
+    const float* __restrict__ dentropy, uint32_t first) {
     constexpr int PER = T::PER;
     const uint32_t r = first + blockIdx.y;
     const int tid = threadIdx.x;
@@ -690,8 +693,8 @@ __global__ __launch_bounds__(BLOCK) void token_logprob_backward_kernel(
         if constexpr (DOT) return -p * __builtin_fmaf(cs, fmaxf(lp, kLeastD) + h, gs);
         else return -p * gs;
     };
-    auto grad_hot = [&](float z) {                          // 1 - p of a likely target without the difference
-        const float lp = __builtin_fmaf(z, inv_t, -l);
+    auto grad_hot = [&](float z) {                          // the target's: 1 - p = -expm1(log p)
+        const float lp = logp ? logp[r] : __builtin_fmaf(z, inv_t, -l);
         float d = -gs * expm1f(lp);
         if constexpr (DOT) d -= exp2_of(lp * kLog2e) * cs * (fmaxf(lp, kLeastD) + h);
         return d;
@@ -2027,9 +2030,9 @@ int rlx_token_logprob(const rlx_logits* x, const void* targets, int index_type, 
     return st;
 }
 
-int rlx_token_logprob_backward(const rlx_logits* x, const void* targets, int index_type, float temperature,
-                               const float* lse, const float* entropy, const float* dlogp, const float* dentropy,
-                               const rlx_logits* dx, void* stream) {
+int rlx_token_logprob_backward_logp(const rlx_logits* x, const void* targets, int index_type, float temperature,
+                                    const float* lse, const float* entropy, const float* logp, const float* dlogp,
+                                    const float* dentropy, const rlx_logits* dx, void* stream) {
     int st = check_logits(x);
     if (st != RLX_OK) return st;
     if ((st = check_gradient(x, dx)) != RLX_OK) return st;
@@ -2037,7 +2040,7 @@ int rlx_token_logprob_backward(const rlx_logits* x, const void* targets, int ind
     if (x->rows == 0) return RLX_OK;
     if ((st = check_targets(targets, index_type)) != RLX_OK) return st;
     if (!lse || !dlogp || !entropy != !dentropy) return RLX_ERR_INVALID_ARG;
-    if (!floats_aligned({lse, entropy, dlogp, dentropy})) return RLX_ERR_MISALIGNED;
+    if (!floats_aligned({lse, entropy, logp, dlogp, dentropy})) return RLX_ERR_MISALIGNED;
     const Logits v = view(*x), dv = view(*dx);
     const float inv_t = 1.0f / temperature;
     const int wide = index_type == RLX_INDEX_I64, groups = row_groups(*x);
@@ -2049,11 +2052,17 @@ int rlx_token_logprob_backward(const rlx_logits* x, const void* targets, int ind
                 constexpr bool ONCE = decltype(once)::value;
                 token_logprob_backward_kernel<T, ONCE ? 256 : 128, ONCE ? 1 : 2, decltype(dot)::value, ONCE>
                     <<<dim3(chunks, here), dim3(ONCE ? 256 : 128), 0, (hipStream_t)stream>>>(
-                        v, dv, targets, wide, inv_t, lse, entropy, dlogp, dentropy, first);
+                        v, dv, targets, wide, inv_t, lse, entropy, logp, dlogp, dentropy, first);
             });
         });
     });
     return st;
+}
+
+int rlx_token_logprob_backward(const rlx_logits* x, const void* targets, int index_type, float temperature,
+                               const float* lse, const float* entropy, const float* dlogp, const float* dentropy,
+                               const rlx_logits* dx, void* stream) {
+    return rlx_token_logprob_backward_logp(x, targets, index_type, temperature, lse, entropy, nullptr, dlogp, dentropy, dx, stream);
 }
 
 int64_t rlx_policy_loss_workspace(int64_t tokens, int64_t n_seqs) {

@@ -63,9 +63,9 @@ inline void launch_token_logprob(const rlx_logits& x, const int* targets, float 
 
 inline void launch_token_logprob_backward(const rlx_logits& x, const int* targets, float temperature, const float* lse,
                                           const float* entropy, const float* dlogp, const float* dentropy,
-                                          const rlx_logits& dx, hipStream_t stream = 0) {
-    RLX_CHECK(rlx_token_logprob_backward(&x, targets, RLX_INDEX_I32, temperature, lse, entropy, dlogp, dentropy, &dx,
-                                         (void*)stream));
+                                          const rlx_logits& dx, hipStream_t stream = 0, const float* logp = nullptr) {
+    RLX_CHECK(rlx_token_logprob_backward_logp(&x, targets, RLX_INDEX_I32, temperature, lse, entropy, logp, dlogp, dentropy,
+                                              &dx, (void*)stream));
 }
 
 inline void launch_policy_loss(const float* logp, int64_t tokens, const rlx_policy_args& args, float* dlogp,

@@ -179,9 +179,11 @@ def token_logprobs(logits, targets, temperature=1.0, with_entropy=False):
     return TokenLogprobs(logp, lse, entropy)
 
 
-def token_logprobs_backward(logits, targets, lse, dlogp, temperature=1.0, entropy=None, dentropy=None, out=None):
+def token_logprobs_backward(logits, targets, lse, dlogp, temperature=1.0, entropy=None, dentropy=None, out=None,
+                            logp=None):
     """Gradient of the logits from the gradients of token_logprobs' logp and (with its entropy) entropy.
-    out=logits writes it over the logits."""
+    out=logits writes it over the logits.  With token_logprobs' logp the gradients of likely targets keep the relative
+    precision of 1 - p; an lse alone leaves them off by up to 2^-24 |lse| / (1 - p) of themselves."""
     x = _logits("logits", logits)
     device, shape = logits.device, logits.shape[:-1]
     target_ptr, index_type = _targets(targets, device, shape)
@@ -190,13 +192,14 @@ def token_logprobs_backward(logits, targets, lse, dlogp, temperature=1.0, entrop
     f32 = torch.float32
     lse_p, dlogp_p = _ptr("lse", lse, device, f32, shape), _ptr("dlogp", dlogp, device, f32, shape)
     ent_p, dent_p = _ptr("entropy", entropy, device, f32, shape), _ptr("dentropy", dentropy, device, f32, shape)
+    logp_p = _ptr("logp", logp, device, f32, shape)
     if lse_p is None or dlogp_p is None:
         raise ValueError("lse and dlogp are needed")
     with _on(device):
         out, dx = _gradient(logits, x, out)
-        B.check(B.load().rlx_token_logprob_backward(C.byref(x), target_ptr, index_type, temperature, lse_p, ent_p,
-                                                    dlogp_p, dent_p, C.byref(dx), _raw_stream(device.index)),
-                "rlx_token_logprob_backward")
+        B.check(B.load().rlx_token_logprob_backward_logp(C.byref(x), target_ptr, index_type, temperature, lse_p, ent_p,
+                                                         logp_p, dlogp_p, dent_p, C.byref(dx),
+                                                         _raw_stream(device.index)), "rlx_token_logprob_backward")
     return out
 
 

@@ -108,3 +108,69 @@ def test_statistics_of_the_loss_from_logits_are_rounded_once(losses, T, rows):
         stats, n, _, _, _, terms, _ = LO.policy(r.logp.cpu().numpy(), adv, LO.sequences(rows, cu), 3, np.ones(rows, bool),
                                                 old=old.cpu().numpy(), ref=ref.cpu().numpy(), entropy=r.entropy.cpu().numpy(), **kw)
         within(r.stats, stats, once(stats, terms), reduction)
+
+
+# --- gradients of near-certain targets ---------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("rows,vocab", [(1, 1), (3, 7), (6, 513), (300, 1003), (120, 50257), (2, 151936)])
+@pytest.mark.parametrize("temperature", [1.0, 0.7])
+@pytest.mark.parametrize("name", TYPES)
+def test_certain_targets_in_the_backward(losses, T, name, temperature, rows, vocab):
+    """Given the forward's log p, a target's own gradient g (1 - p) - c p (log p + H) holds relative to 1 - p.
+
+    With R = sum over the others of exp(z_i - z_t): log p = -log1p(R) with an error of rel R / (1 + R) + 6u|log p| (rel: that of
+    R, a sum like the one that slack() counts, with exponents of log(V) + |log R| on the mean), so 1 - p = -expm1(log p) moves by
+    rel + 6u of itself, and expm1 (2 ulp), the temperature and two products add 8u.  The entropy is given with an error of
+    2 rel (H + 1 - p), which the formula takes over, and each sum and product of that term rounds by u.
+    """
+    rng = np.random.default_rng(rows)
+    gen = T.Generator().manual_seed(rows * 7 + vocab)
+    x = (T.randn(rows, vocab, generator=gen) * 2.5).to(getattr(T, name)).cuda()
+    th = np.resize([0, vocab - 1, vocab // 2, vocab - vocab % 8 - 1, vocab * 5 // 7], rows).clip(0, vocab - 1)
+    t, pick = T.tensor(th).cuda(), T.arange(rows).cuda()
+    lift = T.tensor(rng.uniform(1.0, 20.0, rows)).cuda()
+    x[pick, t] = (((x.double() / temperature).logsumexp(1) + lift) * temperature).to(x.dtype)
+    xh = host64(x) / float(np.float32(temperature))
+    z = xh - xh[np.arange(rows), th][:, None]
+    z[np.arange(rows), th] = -np.inf
+    with np.errstate(all="ignore"):
+        e = np.exp(z)
+        R = e.sum(1)
+        logp, miss = -np.log1p(R), R / (1 + R)
+        ent = ((e * np.where(e > 0, -z, 0.0)).sum(1) + R * np.log1p(R) + np.log1p(R)) / (1 + R)
+        far = np.where(R > 0, np.abs(np.log(R)), 0.0)
+    assert (miss < 0.4).all()
+    rel = LO.slack(vocab, LO.finite_max(xh), np.log(vocab) + far)
+    g, c = (rng.normal(size=rows).astype(np.float32) for _ in range(2))
+    f = losses.token_logprobs(x, t, temperature=temperature, with_entropy=True)
+    put = lambda a: T.tensor(a).cuda()  # noqa: E731
+    bound = np.abs(g) * miss * (rel + 14 * U)
+    got = losses.token_logprobs_backward(x, t, f.lse, put(g), temperature=temperature, logp=f.logp)
+    want = g * miss / temperature
+    within(got[pick, t], want, np.abs(want) * LO.EPS[name] * 1.01 + bound / temperature + LO.TINY[name], "gradient")
+    both = losses.token_logprobs_backward(x, t, f.lse, put(g), temperature=temperature, entropy=f.entropy, dentropy=put(c),
+                                          logp=f.logp)
+    want = (g * miss - c * (1 - miss) * (logp + ent)) / temperature
+    bound = bound + np.abs(c) * (2 * rel * (ent + miss) + rel * miss + 16 * U * (np.abs(logp) + ent))
+    within(both[pick, t], want, np.abs(want) * LO.EPS[name] * 1.01 + bound / temperature + LO.TINY[name], "with the entropy's")
+    # the other logits' gradients do not ask for log p
+    for a, kw in ((got, {}), (both, dict(entropy=f.entropy, dentropy=put(c)))):
+        b = losses.token_logprobs_backward(x, t, f.lse, put(g), temperature=temperature, **kw)
+        a[pick, t], b[pick, t] = 0.0, 0.0
+        assert T.equal(a, b)
+    with pytest.raises(ValueError):
+        losses.token_logprobs_backward(x, t, f.lse, put(g), temperature=temperature, logp=f.logp.double())
+
+
+def test_targets_without_probability_in_the_backward(losses, T):
+    """log p given: targets at -inf and at a type's lowest value (p = 0), ignored and bad ones."""
+    for name in TYPES:
+        x = (T.randn(5, 2003, generator=T.Generator().manual_seed(4)) * 2).to(getattr(T, name)).cuda()
+        x[0, 5], x[1, 6] = -math.inf, T.finfo(x.dtype).min
+        t = T.tensor([5, 6, -1, 2003, 0]).cuda()
+        f = losses.token_logprobs(x, t, with_entropy=True)
+        g, c = T.full((5,), 0.5).cuda(), T.full((5,), 0.25).cuda()
+        for kw in ({}, dict(entropy=f.entropy, dentropy=c)):
+            d = losses.token_logprobs_backward(x, t, f.lse, g, logp=f.logp, **kw).float()
+            assert d[0, 5] == 0.5 and d[1, 6] == 0.5 and (d[2] == 0).all() and d[3].isnan().all() and d[4].isfinite().all()
+            assert T.equal(d[:2], losses.token_logprobs_backward(x, t, f.lse, g, **kw).float()[:2])

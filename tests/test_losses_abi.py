@@ -246,3 +246,18 @@ def test_oracle_preference_gradient_against_differences(average):
         step[i] = 1e-6
         diff = (LO.preference(lp + step, seq, 2, counts, **kw)[0][0] - LO.preference(lp - step, seq, 2, counts, **kw)[0][0])
         assert abs(diff / 2e-6 - dlogp[i]) < 1e-8
+
+
+def test_backward_with_log_probabilities_is_checked(B):
+    """The form that also takes logp refuses what the other one does, and a misaligned logp."""
+    x, dx = logits(B), logits(B, data=Q)
+
+    def call(logp=P, targets=P, index=0, temp=1.0, lse=P, ent=None, dlogp=P, dent=None, x=x, dx=dx):
+        return B.load().rlx_token_logprob_backward_logp(C.byref(x), targets, index, temp, lse, ent, logp, dlogp, dent,
+                                                        C.byref(dx), None)
+
+    assert call(x=logits(B, rows=0, data=None), dx=logits(B, rows=0, data=None)) == B.OK
+    for kw in (dict(lse=None), dict(dlogp=None), dict(ent=P), dict(dent=P), dict(targets=None), dict(index=2),
+               dict(dx=logits(B, data=P + 200))):
+        assert call(**kw) == B.ERR_INVALID_ARG, kw
+    assert call(logp=P + 2) == B.ERR_MISALIGNED and call(temp=0.0) == B.ERR_BAD_HYPER
