@@ -318,8 +318,9 @@ int rlx_token_logprob(const rlx_logits* x, const void* targets, int index_type, 
  * Gradient of the logits from those of logp and entropy (dentropy and entropy both NULL, or neither), with the lse
  * and entropy that rlx_token_logprob gave for the same logits and temperature:
  *     dx[r][j] = (dlogp[r] ([j = target] - p[r][j]) - dentropy[r] p[r][j] (log p[r][j] + entropy[r])) / temperature,
- * p = exp(z - lse) (so the lse has to tell: that of a row of the type's lowest value only does not hold log vocab).  A row
- * whose two gradients are 0 gets zeros without being read.  dx has x's rows, vocab and dtype;
+ * p = exp(z - lse).  A row whose two gradients are 0 gets zeros without being read.  A row whose lse is 2^14 or more in
+ * size, infinite ones included (nothing but the type's lowest value, say), gets its p, log p and entropy from its logits again,
+ * at four times the cost and more: such an lse holds too little of log vocab.  dx has x's rows, vocab and dtype;
  * it may be x itself (same data and strides) but may not overlap it otherwise.
  * An lse of FP32 leaves a probability off by up to 2^-24 |lse| of itself, and so the target's 1 - p by up to
  * 2^-24 |lse| / (1 - p) of itself: nothing of it is left where 1 - p is below that.  The second form takes

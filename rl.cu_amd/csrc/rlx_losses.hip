@@ -42,6 +42,7 @@ constexpr float kLn2 = 0.693147180559945309417f;
 constexpr float kLn2Hi = 45426.0f / 65536.0f;             // ln 2 cut to 15 bits: an integer below 2^9 times this is exact
 constexpr float kLn2Lo = (float)(0.693147180559945309417 - 45426.0 / 65536.0);
 constexpr float kRefMost = 536870912.0f;                  // 2^29
+constexpr float kMostLse = 16384.0f;                      // beyond, an lse is too coarse to take logits from
 constexpr float kLeastD = -1e30f;                         // keeps 0 * (-inf) out of sums of p log p
 
 struct Logits {             // rlx_logits as the kernels take it
@@ -658,13 +659,15 @@ __global__ __launch_bounds__(kJoinBlock) void token_logprob_join_kernel(Logits x
 // that do not start on 16 bytes do better with half the lanes and two groups each (50,257 BF16: 143 against 156 us).
 // p = exp(z - lse) is formed as 2^((z/T - lse) log2 e), the difference first; what it inherits is the rounding of lse, up to
 // u |lse| of p (u = 2^-24) and, at a target, u |lse| / (1 - p) of 1 - p.  Where log p of the target is given, its own gradient
-// comes from that and keeps the precision of 1 - p.
+// comes from that and keeps the precision of 1 - p.  Rows whose lse is so large that even log V drowns in its rounding (nothing but
+// the type's lowest value), or that overflowed, are worked out again from their logits.
 template <typename T, int BLOCK, int NG, bool DOT, bool ONCE>
 __global__ __launch_bounds__(BLOCK) void token_logprob_backward_kernel(
-    Logits x, Logits dx, const void* __restrict__ targets, int wide, float inv_t, const float* __restrict__ lse,
+    Logits x, Logits dx, const void* __restrict__ targets, int wide, float k, float inv_t, const float* __restrict__ lse,
     const float* __restrict__ entropy, const float* __restrict__ logp, const float* __restrict__ dlogp,
     const float* __restrict__ dentropy, uint32_t first) {
     constexpr int PER = T::PER;
+    __shared__ Stat shared[BLOCK / 64];
     const uint32_t r = first + blockIdx.y;
     const int tid = threadIdx.x;
     const int64_t t = target_at(targets, wide, r);
@@ -688,6 +691,14 @@ __global__ __launch_bounds__(BLOCK) void token_logprob_backward_kernel(
     }
     const float gs = g * inv_t, cs = c * inv_t;
     const int target = (int)t;
+    if (fabsf(l) >= kMostLse) {
+        if (blockIdx.x != 0) return;                        // the first workgroup does the row by itself: dx may be x
+        const Row rv = row_by_maximum<T, BLOCK>(row, x.vocab, target, k, shared);
+        const RowValues v = row_values(rv, T::one(row, t), k, inv_t);
+        __syncthreads();                                    // every lane has read what is overwritten now
+        rare_gradient<T, BLOCK, DOT>(row_gradient(rv, v, gs, cs), row, out, 0, x.vocab, k, target);
+        return;
+    }
     auto grad = [&](float z) {
         const float lp = __builtin_fmaf(z, inv_t, -l), p = exp2_of(lp * kLog2e);
         if constexpr (DOT) return -p * __builtin_fmaf(cs, fmaxf(lp, kLeastD) + h, gs);
@@ -2042,7 +2053,7 @@ int rlx_token_logprob_backward_logp(const rlx_logits* x, const void* targets, in
     if (!lse || !dlogp || !entropy != !dentropy) return RLX_ERR_INVALID_ARG;
     if (!floats_aligned({lse, entropy, logp, dlogp, dentropy})) return RLX_ERR_MISALIGNED;
     const Logits v = view(*x), dv = view(*dx);
-    const float inv_t = 1.0f / temperature;
+    const float inv_t = 1.0f / temperature, k = kLog2e / temperature;
     const int wide = index_type == RLX_INDEX_I64, groups = row_groups(*x);
     const unsigned chunks = groups ? (groups + 255) / 256 : 1;          // 4 KiB of a row per workgroup
     for_type(x->dtype, [&](auto type) {
@@ -2052,7 +2063,7 @@ int rlx_token_logprob_backward_logp(const rlx_logits* x, const void* targets, in
                 constexpr bool ONCE = decltype(once)::value;
                 token_logprob_backward_kernel<T, ONCE ? 256 : 128, ONCE ? 1 : 2, decltype(dot)::value, ONCE>
                     <<<dim3(chunks, here), dim3(ONCE ? 256 : 128), 0, (hipStream_t)stream>>>(
-                        v, dv, targets, wide, inv_t, lse, entropy, logp, dlogp, dentropy, first);
+                        v, dv, targets, wide, k, inv_t, lse, entropy, logp, dlogp, dentropy, first);
             });
         });
     });

@@ -36,9 +36,9 @@ def within(got, want, bound, what):
     bound = np.broadcast_to(bound, want.shape)
     off = np.abs(got - want)
     bad = ~(off <= bound)
-    assert not bad.any(), "%s: %d of %d off, worst by %.3g of %.3g where %.3g is allowed" % (
-        what, bad.sum(), bad.size, off[np.argmax(off - bound)], want.reshape(-1)[np.argmax(off - bound)],
-        bound.reshape(-1)[np.argmax(off - bound)])
+    at = np.unravel_index(np.argmax(np.where(bad, np.nan_to_num(off - bound, nan=np.inf), -np.inf)), bad.shape) if bad.size else ()
+    assert not bad.any(), "%s: %d of %d off, worst at %s by %.3g of %.3g where %.3g is allowed" % (
+        what, bad.sum(), bad.size, at, off[at], want[at], bound[at])
 
 
 # --- one rounding of what is computed in 64 bits ---------------------------------------------------------------------------
@@ -174,3 +174,79 @@ def test_targets_without_probability_in_the_backward(losses, T):
             d = losses.token_logprobs_backward(x, t, f.lse, g, logp=f.logp, **kw).float()
             assert d[0, 5] == 0.5 and d[1, 6] == 0.5 and (d[2] == 0).all() and d[3].isnan().all() and d[4].isfinite().all()
             assert T.equal(d[:2], losses.token_logprobs_backward(x, t, f.lse, g, **kw).float()[:2])
+
+
+# --- rows whose log-sum-exp tells nothing ------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("over", [False, True])
+@pytest.mark.parametrize("temperature", [1.0, 0.7, 2.0])
+@pytest.mark.parametrize("vocab", [5, 3001, 50001])
+@pytest.mark.parametrize("name", TYPES)
+def test_backward_of_rows_of_huge_logits(losses, T, name, vocab, temperature, over):
+    """Rows whose log-sum-exp is so large that its rounding hides log V (or that overflow once divided by the temperature): the
+    gradient is that of the logits less their maximum.  p is off by the rounding of (z - max) k (2u|lp|, and 2u of the
+    factor), the sum and the quotient: slack() of the logits that have a share, which lie within 200 of the maximum."""
+    lowest = T.finfo(getattr(T, name)).min
+    rng = np.random.default_rng(vocab)
+    x = T.randn(9, vocab, generator=T.Generator().manual_seed(vocab)) * 2
+    t = T.tensor([0, 1, 2, vocab - 1, 3, 4, 2, 1, 0])
+    x[0] = lowest
+    x[1] = lowest
+    x[1, 1] = -math.inf                                 # the target among those that have no share
+    x[2] = 60000.0 + 32.0 * T.tensor(rng.integers(-2, 3, vocab)).float()
+    x[3] = -60000.0 - 32.0 * T.tensor(rng.integers(0, 3, vocab)).float()
+    x[4] = lowest
+    x[4, vocab // 2:] = -math.inf
+    x[5, 0] = 50000.0                                   # one logit far above the others
+    x[6] = lowest                                       # ignored
+    x[7] = lowest                                       # gradients of 0
+    t[6] = -1
+    x = x.to(getattr(T, name))
+    xh, th = host64(x) / float(np.float32(temperature)), t.numpy()
+    x, t = x.cuda(), t.cuda()
+    g, c = rng.normal(size=9).astype(np.float32), rng.normal(size=9).astype(np.float32)
+    g[7] = c[7] = 0.0
+    f = losses.token_logprobs(x, t, temperature=temperature, with_entropy=True)
+    top = xh.max(1, keepdims=True)
+    off = xh - top
+    own = np.log(np.exp(off).sum(1))
+    lq = off - own[:, None]
+    ent = -(np.exp(lq) * np.where(np.exp(lq) > 0, lq, 0.0)).sum(1)
+    zeros = np.array([6, 7])
+    for kw, with_c in (({}, False), (dict(entropy=f.entropy, dentropy=T.tensor(c).cuda()), True)):
+        into = x.clone() if over else None
+        for more in (dict(logp=f.logp), {}):
+            got = losses.token_logprobs_backward(into if over else x, t, f.lse, T.tensor(g).cuda(), temperature=temperature,
+                                                 out=into, **more, **kw)
+            # of logits already divided: the temperature is 1 for the oracle, and divides its result
+            d, size = LO.rows_grad(off, th, 1.0, own, g, ent, c if with_c else None)
+            d, size = d / temperature, size / temperature
+            rel = LO.slack(vocab, 200.0, np.abs(np.nan_to_num(lq, neginf=0.0)).clip(0, 200))
+            # a p below 2^-126 comes out as 0: off by that p, times g and times c (log p + H)
+            flushed = np.abs(g)[:, None] + np.abs(c)[:, None] * (np.abs(np.nan_to_num(lq, neginf=0.0)) + ent[:, None] + 1)
+            bound = LO.grad_bound(name, d, size, rel) + 2.0 ** -126 * flushed / temperature
+            d[zeros], bound[zeros] = 0.0, 0.0
+            want_rows = [0, 1, 2, 3, 4, 5, 6, 7]
+            within(got[want_rows], d[want_rows], bound[want_rows], "%s %r" % (name, sorted(kw)))
+            if over:
+                into = x.clone()
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("rows,vocab", [(1, 3001), (40, 3001), (43, 50001)])
+def test_backward_of_rows_without_an_answer(losses, T, name, rows, vocab):
+    """Rows of -inf only, with a NaN, with +inf, with a bad target: NaN all over; their neighbours keep theirs."""
+    import test_gpu_losses as other
+    _, kind, x, t = other.broken_rows(T, name, rows, vocab)
+    x, t = x.cuda(), t.cuda()
+    f = losses.token_logprobs(x, t, with_entropy=True)
+    one = T.ones(rows).cuda()
+    for kw in ({}, dict(logp=f.logp), dict(entropy=f.entropy, dentropy=one)):
+        got = losses.token_logprobs_backward(x, t, f.lse, one, **kw)
+        for i, k in enumerate(kind):
+            if k in (3, 4, 5, 7):
+                assert got[i].isnan().all(), (i, k)
+            elif k in (6, 11):
+                assert (got[i] == 0).all(), (i, k)
+            else:
+                assert got[i].isfinite().all(), (i, k)
