@@ -410,7 +410,9 @@ def policy_step(optimizer, forward, backward, n_micro, max_grad_norm, fused_clip
     advantages, old_logp, ref_logp, mask, cu_seqlens; whatever is the same for all goes into loss_args), the clipped
     policy loss divided by n_micro, and backward(k, dlogits), which adds its gradients into the pools; then clear the
     gradients of the tensor views in `freeze`, clip, step.  The gradient of the logits is written over the logits, so
-    they are read and written once and no second buffer is held.  Nothing is read by the host before the clip.
+    they are read and written once and no second buffer is held; a model whose last operation keeps its result for its
+    backward pass gives `out` too (a tensor for the gradient, or None for a new one), without which torch raises in that pass.
+    Nothing is read by the host before the clip.
     Returns (loss, pre-clip norm, statistics per micro-batch)."""
     import numpy as np
     import torch
@@ -430,7 +432,8 @@ def policy_step(optimizer, forward, backward, n_micro, max_grad_norm, fused_clip
     results = []
     for k in range(n_micro):
         batch = dict(forward(k))
-        r = losses.policy_loss_logits(out=batch["logits"], norm=norm, **batch, **loss_args)
+        out = batch.pop("out", batch["logits"])
+        r = losses.policy_loss_logits(out=out, norm=norm, **batch, **loss_args)
         backward(k, r.dlogits)
         results.append(r._replace(dlogits=None))
     for t in (freeze or ()):

@@ -8,8 +8,11 @@ formulas and what is done with masked, empty and out-of-range input.
 
 Arguments are device tensors of one GPU; work goes to that GPU's current stream and nothing is waited for.  Every call
 takes its scratch memory and its outputs from torch's allocator, so calls on several streams and calls recorded
-into graphs never share any.  Gradients are explicit: nothing here takes part in torch's autograd.  Per-token tensors are contiguous; logits may be any view whose last dimension is
-contiguous and whose other dimensions step through memory in at most two strides (logits[:, :-1] of a padded batch).
+into graphs never share any.  Gradients are explicit: nothing here takes part in torch's autograd.  It is told of tensors that
+are written over, though: if an operation kept the logits for its own backward pass (a tanh does), out=logits makes
+that pass raise torch's error, and the gradient has to go elsewhere.  Per-token tensors are contiguous; logits may be any
+view whose last dimension is contiguous and whose other dimensions step through memory in at most two strides
+(logits[:, :-1] of a padded batch).
 """
 import ctypes as C
 from collections import namedtuple
@@ -113,6 +116,10 @@ def _targets(targets, device, shape):
             B.INDEX_I64 if targets.dtype == torch.int64 else B.INDEX_I32)
 
 
+# tells autograd that a tensor's values have changed
+_changed = torch.autograd.graph.increment_version
+
+
 def _gradient(logits, x, out):
     """The gradient's tensor (a new one unless given) and its rows; x: those of the logits."""
     if out is logits:
@@ -195,11 +202,14 @@ def token_logprobs_backward(logits, targets, lse, dlogp, temperature=1.0, entrop
     logp_p = _ptr("logp", logp, device, f32, shape)
     if lse_p is None or dlogp_p is None:
         raise ValueError("lse and dlogp are needed")
+    given = out
     with _on(device):
         out, dx = _gradient(logits, x, out)
         B.check(B.load().rlx_token_logprob_backward_logp(C.byref(x), target_ptr, index_type, temperature, lse_p, ent_p,
                                                          logp_p, dlogp_p, dent_p, C.byref(dx),
                                                          _raw_stream(device.index)), "rlx_token_logprob_backward")
+    if given is not None:
+        _changed(given)
     return out
 
 
@@ -267,7 +277,7 @@ def policy_loss_logits(logits, targets, advantages, old_logp=None, ref_logp=None
     target_ptr, index_type = _targets(targets, device, shape)
     args = _policy_args(shape, device, advantages, old_logp, ref_logp, None, mask, cu_seqlens, clip_low, clip_high,
                         kl_coef, entropy_coef, reduction, norm, grad_scale)
-    lib = B.load()
+    lib, given = B.load(), out
     with _on(device):
         logp, entropy = _floats(targets), _floats(targets) if with_entropy else None
         out, dx = _gradient(logits, x, out)
@@ -276,6 +286,8 @@ def policy_loss_logits(logits, targets, advantages, old_logp=None, ref_logp=None
         B.check(lib.rlx_policy_loss_logits(C.byref(x), target_ptr, index_type, temperature, C.byref(args),
                                            logp.data_ptr(), _address(entropy), C.byref(dx), stats_ptr,
                                            ws_ptr, nbytes, _raw_stream(device.index)), "rlx_policy_loss_logits")
+    if given is not None:
+        _changed(given)
     return PolicyLossLogits(stats, count, logp, entropy, out)
 
 

@@ -250,3 +250,97 @@ def test_backward_of_rows_without_an_answer(losses, T, name, rows, vocab):
                 assert (got[i] == 0).all(), (i, k)
             else:
                 assert got[i].isfinite().all(), (i, k)
+
+
+# --- gradients over the logits, and autograd ---------------------------------------------------------------------------------
+
+def gradients_over(losses, T, z, t):
+    """Every call that can write over the logits, as (name, call(out))."""
+    f = losses.token_logprobs(z, t)
+    adv, g = T.ones(1, device="cuda"), T.ones(t.shape, device="cuda")
+    return [("token_logprobs_backward", lambda out: losses.token_logprobs_backward(z, t, f.lse, g, out=out)),
+            ("policy_loss_logits", lambda out: losses.policy_loss_logits(
+                z, t, adv, cu_seqlens=T.tensor([0, t.numel()], dtype=T.int32, device="cuda"), out=out).dlogits)]
+
+
+def test_autograd_learns_that_logits_were_overwritten(losses, T):
+    """A forward pass that keeps its logits for its own backward pass (a tanh) gets torch's error, not wrong gradients; one
+    that does not, or whose gradient goes elsewhere, gets the right ones."""
+    rows, vocab = 6, 301
+    gen = T.Generator().manual_seed(0)
+    h = (T.randn(rows, vocab, generator=gen) * 0.5).cuda()
+    t = T.randint(0, vocab, (rows,), generator=gen).cuda()
+    for which in range(2):
+        w = h.clone().requires_grad_()
+        z = T.tanh(w)
+        what, call = gradients_over(losses, T, z, t)[which]
+        before = z._version
+        call(None)
+        other = T.empty_like(z)
+        v = other._version
+        d = call(other)
+        assert d is other and z._version == before and other._version > v, what
+        z.backward(d)
+        want = (1.0 - T.tanh(h) ** 2) * d
+        assert T.allclose(w.grad, want, rtol=1e-5, atol=1e-7), what
+        w = h.clone().requires_grad_()
+        z = T.tanh(w)
+        what, call = gradients_over(losses, T, z, t)[which]
+        before = z._version
+        d = call(z)
+        assert d is z and z._version > before, what
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            z.backward(d)
+        w = h.clone().requires_grad_()
+        z = w * 2.0                                           # does not need its result
+        d = gradients_over(losses, T, z, t)[which][1](z)
+        z.backward(d.detach().clone())
+        assert T.allclose(w.grad, 2.0 * d.detach(), rtol=1e-6)
+
+
+def step_parts(host, L, T, rows=24, vocab=257, hidden=16, n_micro=3):
+    st = host.ParamStore([L.TensorSpec("lm_head", vocab * hidden, L.DTYPE_F32, L.NO_DECAY, hidden)], "cuda:0")
+    gen = T.Generator().manual_seed(0)
+    st.param(0).copy_((T.randn(vocab, hidden, generator=gen) * 0.3).reshape(-1))
+    acts = [T.randn(rows, hidden, generator=gen).cuda() for _ in range(n_micro)]
+    targets = [T.randint(0, vocab, (rows,), generator=gen).cuda() for _ in range(n_micro)]
+    adv = [T.randn(3, generator=gen).cuda() for _ in range(n_micro)]
+    return st, host.AdamWOptimizer(st, lr=1e-2), acts, targets, adv, T.tensor([0, 7, 15, 24], dtype=T.int32).cuda()
+
+
+@pytest.mark.parametrize("own_buffer", [False, True])
+def test_policy_step_of_logits_that_autograd_keeps(losses, host, L, T, own_buffer):
+    """A model that ends in a tanh: policy_step over its logits raises, with `out` (None, or a buffer) it is right."""
+    vocab, hidden, n_micro = 257, 16, 3
+    st, opt, acts, targets, adv, cu = step_parts(host, L, T)
+    ref_st, ref_opt, *_ = step_parts(host, L, T)
+    buffer = T.empty(24, vocab, device="cuda") if own_buffer else None
+
+    live = {}
+
+    def forward(k, **more):
+        w = st.param(0).view(vocab, hidden).detach().clone().requires_grad_()
+        z = T.tanh(acts[k] @ w.t())
+        live["w"], live["z"] = w, z
+        return dict(logits=z, targets=targets[k], advantages=adv[k], **more)
+
+    def backward(k, dlogits):
+        live["z"].backward(dlogits)
+        st.grad(0).view(vocab, hidden).add_(live["w"].grad)
+
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        host.policy_step(opt, forward, backward, n_micro, 0.01, cu_seqlens=cu)
+    loss, norm, results = host.policy_step(opt, lambda k: forward(k, out=buffer), backward, n_micro, 0.01, cu_seqlens=cu)
+
+    def plain_forward(k):
+        with T.no_grad():
+            z = T.tanh(acts[k] @ ref_st.param(0).view(vocab, hidden).t())
+        live["y"] = z.clone()
+        return dict(logits=z, targets=targets[k], advantages=adv[k])
+
+    def plain_backward(k, d):
+        ref_st.grad(0).view(vocab, hidden).add_(((1.0 - live["y"] ** 2) * d).t() @ acts[k])
+
+    loss2, norm2, _ = host.policy_step(ref_opt, plain_forward, plain_backward, n_micro, 0.01, cu_seqlens=cu)
+    assert loss == loss2 and abs(norm - norm2) <= 1e-5 * norm2 and norm > 0
+    assert len(results) == n_micro and T.allclose(st.param(0), ref_st.param(0), atol=1e-5)
