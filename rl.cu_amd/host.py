@@ -429,13 +429,15 @@ def policy_step(optimizer, forward, backward, n_micro, max_grad_norm, fused_clip
     st = _stream()
     optimizer.store.zero_grads(st)
     norm = float(np.float32(1.0) / np.float32(n_micro))
-    results = []
-    for k in range(n_micro):
+
+    def micro_batch(k):                       # a function, so that its logits are gone when the next ones are made
         batch = dict(forward(k))
         out = batch.pop("out", batch["logits"])
         r = losses.policy_loss_logits(out=out, norm=norm, **batch, **loss_args)
         backward(k, r.dlogits)
-        results.append(r._replace(dlogits=None))
+        return r._replace(dlogits=None)
+
+    results = [micro_batch(k) for k in range(n_micro)]
     for t in (freeze or ()):
         B.clear(t.data_ptr(), t.numel() * t.element_size(), st)
     grad_norm = training_step(optimizer, max_grad_norm, fused_clip=fused_clip)

@@ -344,3 +344,34 @@ def test_policy_step_of_logits_that_autograd_keeps(losses, host, L, T, own_buffe
     loss2, norm2, _ = host.policy_step(ref_opt, plain_forward, plain_backward, n_micro, 0.01, cu_seqlens=cu)
     assert loss == loss2 and abs(norm - norm2) <= 1e-5 * norm2 and norm > 0
     assert len(results) == n_micro and T.allclose(st.param(0), ref_st.param(0), atol=1e-5)
+
+
+# --- memory ------------------------------------------------------------------------------------------------------------------
+
+def test_policy_step_holds_one_buffer_of_logits(losses, host, L, T):
+    """When forward(k + 1) runs, and when the clip does, the logits of every earlier micro-batch are gone."""
+    vocab, hidden, n_micro = 257, 16, 3
+    st, opt, acts, targets, adv, cu = step_parts(host, L, T)
+    made = []
+
+    def gone():
+        return [r() is None for r in made]
+
+    def forward(k):
+        assert gone() == [True] * k
+        z = acts[k] @ st.param(0).view(vocab, hidden).t()
+        made.append(weakref.ref(z))
+        return dict(logits=z, targets=targets[k], advantages=adv[k])
+
+    def backward(k, dlogits):
+        st.grad(0).view(vocab, hidden).add_(dlogits.t() @ acts[k])
+
+    clip = opt.clip_grad_norm_
+
+    def watched(*args, **kw):
+        assert gone() == [True] * n_micro
+        return clip(*args, **kw)
+
+    opt.clip_grad_norm_ = watched
+    host.policy_step(opt, forward, backward, n_micro, 1.0, cu_seqlens=cu)
+    assert gone() == [True] * n_micro
