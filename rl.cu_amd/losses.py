@@ -227,19 +227,12 @@ def _policy_args(shape, device, advantages, old_logp, ref_logp, entropy, mask, c
                         kl_coef, entropy_coef, norm, grad_scale, _REDUCTIONS[reduction], 0 if per_sequence else 1)
 
 
-_SHARED = 1 << 20
-
-
 def _policy_memory(nbytes, device, where):
-    """(tensor, address of an rlx_policy_stats, its parts, address of scratch memory).  The statistics, which live on, and
-    up to 1 MiB of scratch memory share an allocation."""
-    if nbytes < 0:
-        raise B.RlxError(B.ERR_INVALID_ARG, where)
-    words = 4 + ((nbytes + 7) >> 3 if nbytes <= _SHARED else 0)
-    buf = torch.empty(words, dtype=torch.int64, device=device)
-    at = buf.data_ptr()
-    scratch, scratch_ptr = (buf, at + 32) if nbytes <= _SHARED else _workspace(nbytes, device, where)
-    return scratch, at, buf.view(torch.float32)[:6], buf[3], scratch_ptr
+    """(scratch tensor to keep alive, address of an rlx_policy_stats, its parts, address of scratch memory).  The statistics live
+    on, so they have an allocation of their own (1 us more than in one with the scratch memory, which they would hold)."""
+    scratch, scratch_ptr = _workspace(nbytes, device, where)
+    buf = torch.empty(4, dtype=torch.int64, device=device)
+    return scratch, buf.data_ptr(), buf.view(torch.float32)[:6], buf[3], scratch_ptr
 
 
 def policy_loss(logp, advantages, old_logp=None, ref_logp=None, entropy=None, mask=None, cu_seqlens=None,

@@ -375,3 +375,15 @@ def test_policy_step_holds_one_buffer_of_logits(losses, host, L, T):
     opt.clip_grad_norm_ = watched
     host.policy_step(opt, forward, backward, n_micro, 1.0, cu_seqlens=cu)
     assert gone() == [True] * n_micro
+
+
+@pytest.mark.parametrize("rows,vocab", [(9, 50257), (2000, 700)])
+def test_results_hold_no_scratch_memory(losses, T, rows, vocab):
+    """Kept statistics keep 32 bytes, not what the call worked with."""
+    x, t = T.randn(rows, vocab, device="cuda"), T.zeros(rows, dtype=T.int64, device="cuda")
+    adv, cu = T.ones(2, device="cuda"), T.tensor([0, 3, rows], dtype=T.int32, device="cuda")
+    many = T.zeros(30000, device="cuda")
+    far = T.tensor([0, 3, 30000], dtype=T.int32, device="cuda")
+    for r in (losses.policy_loss_logits(x, t, adv, cu_seqlens=cu), losses.policy_loss(many, adv, cu_seqlens=far)):
+        assert r.stats.untyped_storage().nbytes() == 32 and r.tokens.untyped_storage().nbytes() == 32
+        assert int(r.tokens) in (rows, 30000)
