@@ -414,18 +414,24 @@ def policy_step(optimizer, forward, backward, n_micro, max_grad_norm, fused_clip
     backward pass gives `out` too (a tensor for the gradient, or None for a new one), without which torch raises in that pass.
     Nothing is read by the host before the clip.
     Returns (loss, pre-clip norm, statistics per micro-batch)."""
-    import numpy as np
     import torch
-    from . import losses
     if n_micro < 1:
         raise ValueError("policy_step needs at least one micro-batch")
     if "norm" in loss_args or "out" in loss_args:
         raise ValueError("policy_step sets norm and out itself")
-    # one stream for all of it: the loss operators follow torch's current one
-    if stream is not None and stream != _stream():
+    # one device and one stream for all of it: the loss operators follow their tensors' device and torch's current stream
+    with torch.cuda.device(optimizer.store.device):
+        if stream is None or stream == _stream():
+            return _policy_step(optimizer, forward, backward, n_micro, max_grad_norm, fused_clip, freeze, loss_args)
         with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=optimizer.store.device)):
-            return policy_step(optimizer, forward, backward, n_micro, max_grad_norm, fused_clip, freeze, None,
-                               **loss_args)
+            return _policy_step(optimizer, forward, backward, n_micro, max_grad_norm, fused_clip, freeze, loss_args)
+
+
+def _policy_step(optimizer, forward, backward, n_micro, max_grad_norm, fused_clip, freeze, loss_args):
+    """policy_step on the current device and stream."""
+    import numpy as np
+    import torch
+    from . import losses
     st = _stream()
     optimizer.store.zero_grads(st)
     norm = float(np.float32(1.0) / np.float32(n_micro))

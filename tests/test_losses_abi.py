@@ -261,3 +261,56 @@ def test_backward_with_log_probabilities_is_checked(B):
                dict(dx=logits(B, data=P + 200))):
         assert call(**kw) == B.ERR_INVALID_ARG, kw
     assert call(logp=P + 2) == B.ERR_MISALIGNED and call(temp=0.0) == B.ERR_BAD_HYPER
+
+
+@pytest.mark.parametrize("side", [None, 77])
+def test_policy_step_works_on_the_optimizers_device(pkg, losses, monkeypatch, side):
+    """Every part of a step runs with the optimizer's device as the current one, and on that device's stream."""
+    import torch
+    host = importlib.import_module(pkg.__name__ + ".host")
+    now, seen = ["cuda:0"], []
+
+    class Device:
+        def __init__(self, device):
+            self.device = str(device)
+
+        def __enter__(self):
+            now.append(self.device)
+
+        def __exit__(self, *exc):
+            now.pop()
+
+    class Stream(Device):
+        def __enter__(self):
+            now.append(self.device + " 77")
+
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch.cuda, "ExternalStream", lambda stream, device: Stream(device))
+    monkeypatch.setattr(torch.cuda, "stream", lambda s: s)
+    monkeypatch.setattr(host, "_stream", lambda: 77 if now[-1].endswith(" 77") else now[-1])
+    monkeypatch.setattr(host, "training_step", lambda *a, **kw: seen.append(("step", now[-1])) or 2.0)
+
+    def loss(**kw):
+        seen.append(("loss", now[-1]))
+        return losses.PolicyLossLogits(torch.ones(6), torch.tensor(1), None, None, kw["logits"])
+
+    monkeypatch.setattr(losses, "policy_loss_logits", loss)
+
+    class Store:
+        device = torch.device("cuda:1")
+
+        def zero_grads(self, st):
+            seen.append(("clear on %s" % st, now[-1]))
+
+    class Optimizer:
+        store = Store()
+
+    def forward(k):
+        seen.append(("forward", now[-1]))
+        return dict(logits=torch.zeros(1))
+
+    r = host.policy_step(Optimizer(), forward, lambda k, d: seen.append(("backward", now[-1])), 2, 1.0, stream=side)
+    assert r[:2] == (2.0, 2.0) and now == ["cuda:0"]
+    where = "cuda:1" if side is None else "cuda:1 77"
+    assert seen == [("clear on %s" % ("cuda:1" if side is None else 77), where)] + [
+        (what, where) for what in ("forward", "loss", "backward") * 2] + [("step", where)]
