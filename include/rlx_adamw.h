@@ -322,8 +322,8 @@ int rlx_token_logprob(const rlx_logits* x, const void* targets, int index_type, 
  * size, infinite ones included (nothing but the type's lowest value, say), gets its p, log p and entropy from its logits again,
  * at four times the cost and more: such an lse holds too little of log vocab.  dx has x's rows, vocab and dtype;
  * it may be x itself (same data and strides) but may not overlap it otherwise.
- * An lse of FP32 leaves a probability off by up to 2^-24 |lse| of itself, and so the target's 1 - p by up to
- * 2^-24 |lse| / (1 - p) of itself: nothing of it is left where 1 - p is below that.  The second form takes
+ * An lse of FP32 leaves a probability off by a few times 2^-24 |lse| of itself, and so the target's 1 - p by as much
+ * divided by 1 - p: nothing of it is left where 1 - p is below that.  The second form takes
  * rlx_token_logprob's logp too (NULL: as the first form), from which the target's own gradient keeps the
  * precision of 1 - p, as in rlx_policy_loss_logits.
  * Replaces the backward half of the log-softmax gather (src/model/qwen3.cu:170).

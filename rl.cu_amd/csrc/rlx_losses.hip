@@ -657,8 +657,8 @@ __global__ __launch_bounds__(kJoinBlock) void token_logprob_join_kernel(Logits x
 // dx from the saved lse (and entropy), 4 KiB of a row per workgroup.  Bound by HBM, reads and writes: 4,096 rows of 151,936
 // BF16, a quarter of them ignored, 335 us = 6.5 TB/s (8 KiB per workgroup 357, 16 KiB 372, a workgroup per row 437); rows
 // that do not start on 16 bytes do better with half the lanes and two groups each (50,257 BF16: 143 against 156 us).
-// p = exp(z - lse) is formed as 2^((z/T - lse) log2 e), the difference first; what it inherits is the rounding of lse, up to
-// u |lse| of p (u = 2^-24) and, at a target, u |lse| / (1 - p) of 1 - p.  Where log p of the target is given, its own gradient
+// p = exp(z - lse) is formed as 2^((z/T - lse) log2 e), the difference first; what it inherits is the rounding of lse and of
+// the temperature's reciprocal, a few u |lse| of p (u = 2^-24) and, at a target, as much over 1 - p of 1 - p.  Where log p of the target is given, its own gradient
 // comes from that and keeps the precision of 1 - p.  Rows whose lse is so large that even log V drowns in its rounding (nothing but
 // the type's lowest value), or that overflowed, are worked out again from their logits.
 template <typename T, int BLOCK, int NG, bool DOT, bool ONCE>
@@ -1307,7 +1307,10 @@ __device__ __forceinline__ RowTerms row_terms(const Policy& a, const Row& row, f
 // statistics and gradient as launches of their own 22 % more (4,096 unmasked rows: 479 and 586 us).
 // Bound by the memory system on this pattern of one long row per compute unit: without any arithmetic the same accesses
 // take 640 us, and workgroups that stay and load the next row while they write the present one gained nothing (272
-// against 274 us at 90,000 FP16).
+// against 274 us at 90,000 FP16).  With the gradient over the logits the same memory is read and written: 10 to 15 % more time
+// (4,096 rows of 151,936 FP16 492 and 539 us).  FP32 rows of 151,936 are held by half and their rest read twice: 2,048 of them
+// 552 us, 4.5 TB/s.  DOT, the entropy's part of the gradient, is left out where there is none: 1,974 rows of 151,936 FP16 246
+// against 252 us, BF16 248 against 255; within 2 % either way at 12,000 to 76,000.
 template <typename T, int BLOCK, int NG, bool DOT, bool ONCE>
 __global__ __launch_bounds__(BLOCK) void policy_loss_row_kernel(
     Logits x, Logits dx, const void* __restrict__ targets, int wide, float k, float inv_t, Policy a,
@@ -1804,6 +1807,8 @@ struct Cut {
 // 6.1 / 8.3; 50,257 FP16 1 row 5.7 / 4.8, 8,192 rows 153 / 147.  (512 x 6 beside 512 x 8: 16,384 rows of 17,000 97 / 106.)  In between, for 97 to 256 rows, a launch less weighs more
 // than what the few lanes of a workgroup cost: 129 rows of 50,257 FP16 7.8 / 9.1 us, of 90,000 9.7 / 10.0; 64 rows 7.5 / 7.3
 // and 9.2 / 7.7; beyond 12,288 groups chunks do better for any number of rows (129 rows of 151,936 13.9 / 12.3).
+// 8 KiB / 32 KiB chunks: 151,936 FP16 1 row 4.7 / 5.6 us, 16 rows 5.8 / 6.2, 51 rows 7.4 / 8.0, 64 rows 8.8 / 8.4, 300 rows
+// 21.2 / 18.7; FP32 16 rows 6.3 / 7.0, 40 rows 9.4 / 8.2; 50,257 FP16 64 rows 6.1 / 6.5, 90 rows 6.7 / 7.6.
 Cut cut_of(const rlx_logits& x) {
     const int groups = row_groups(x);
     if (groups <= 64 * 8) return {64, 8, 1};
@@ -1824,9 +1829,9 @@ Cut cut_of(const rlx_logits& x) {
 }
 
 // Whether the loss from logits is better off with its rows in chunks, read twice, than with a workgroup per row: long rows,
-// too few of them to fill the chip.  Time on the GPU, chunks / workgroup per row: 14 rows of 151,936 FP16 11.1 / 23.8 us,
-// 85 rows 20.7 / 24.6, 145 rows 32.9 / 26.0; 85 rows of 151,936 FP32 33.1 / 36.1, 145 rows 53.8 / 43.4; 57 rows of 50,257
-// BF16 12.5 / 17.0, 164 rows 18.6 / 17.5; 57 rows of 32,000 11.1 / 12.8, 145 rows 14.4 / 13.4; rows of 16,000 gain nothing.
+// too few of them to fill the chip.  Time on the GPU, chunks / workgroup per row: 14 rows of 151,936 FP16 11.0 / 24.3 us,
+// 85 rows 24.4 / 25.5, 145 rows 35.7 / 27.5; 85 rows of 151,936 FP32 36.8 / 38.4, 145 rows 55.5 / 48.0; 57 rows of 50,257
+// BF16 12.4 / 16.6, 164 rows 20.1 / 18.4; 57 rows of 32,000 10.9 / 12.9, 145 rows 14.4 / 13.3; rows of 16,000 gain nothing.
 constexpr int64_t kFewRows = 96;
 bool few_rows(const rlx_logits& x) { return x.rows > 0 && x.rows <= kFewRows && row_groups(x) > 256 * 8; }
 int64_t few_chunks(const rlx_logits& x) { return (row_groups(x) + kChunkBlock * kFewGroups - 1) / (kChunkBlock * kFewGroups); }
@@ -1967,7 +1972,9 @@ void for_cut(const Cut& c, Fn f) {
 // Calls f(lanes, 16-byte groups per lane) for the shape that holds a row of `groups` groups in registers.  Groups that a shape
 // has and the row has not are loaded all the same (the last one again), so the steps are small: with 512 x 8, 512 x 14, 1,024 x
 // 12 and 1,024 x 19 alone 17,000 FP16 took 255 us for 300 M logits, not 233, 36,000 239 and 225, 64,000 265 and 221, 100,000
-// 277 and 252, 128,256 243 and 233.  Two workgroups of 512 lanes do better on a compute unit than one of 1,024 (64,000 as
+// 277 and 252, 128,256 243 and 233; of FP32, 150 M logits, 18,000 232 and 224, 32,000 249 and 221, 50,000 257 and 244, 57,000 257
+// and 252.  One wavefront of 4 groups beside 8: 200 M logits of 1,000 FP16 351 and 468 us, 2,000 218 and 247; FP32 600 511 and
+// 624, 1,000 430 and 411.  Two workgroups of 512 lanes do better on a compute unit than one of 1,024 (64,000 as
 // 1,024 x 8: 230), as long as they have the registers (98,304 as 512 x 24: 246, as 1,024 x 12 236).
 template <typename Fn>
 void for_row_shape(int groups, Fn f) {

@@ -190,7 +190,7 @@ def token_logprobs_backward(logits, targets, lse, dlogp, temperature=1.0, entrop
                             logp=None):
     """Gradient of the logits from the gradients of token_logprobs' logp and (with its entropy) entropy.
     out=logits writes it over the logits.  With token_logprobs' logp the gradients of likely targets keep the relative
-    precision of 1 - p; an lse alone leaves them off by up to 2^-24 |lse| / (1 - p) of themselves."""
+    precision of 1 - p; an lse alone leaves them off by a few times 2^-24 |lse| / (1 - p) of themselves."""
     x = _logits("logits", logits)
     device, shape = logits.device, logits.shape[:-1]
     target_ptr, index_type = _targets(targets, device, shape)
