@@ -110,6 +110,33 @@ def test_statistics_of_the_loss_from_logits_are_rounded_once(losses, T, rows):
         within(r.stats, stats, once(stats, terms), reduction)
 
 
+def test_policy_gradients_of_values_out_of_range(losses, T):
+    """Infinities, NaN and differences whose exponential overflows or vanishes, each token by the formula and none by its neighbours."""
+    inf, nan = math.inf, math.nan
+    rows = [(0, -inf, 0, 1), (0, -inf, 0, -1), (-inf, 0, 0, 1), (0, 0, -inf, 1), (nan, 0, 0, 1), (0, nan, 0, 1), (0, 0, nan, 1),
+            (0, 3e38, 0, 1), (3e38, 0, 3e38, -1), (0, 0, 3e38, 1), (0, -800, 0, -1), (0, -300, 0, -1), (0, -85, 0, -1),
+            (-1, -1, -1, 1), (0, 0, 0, 0), (0, 0, -3e38, 1), (-2000.5, 0, -2000, 1)]
+    for copies in (1, 200):                                   # one workgroup, and more
+        logp, old, ref, adv = (np.tile(np.array(c, np.float32), copies) for c in zip(*rows))
+        n = len(logp)
+        put = lambda a: T.tensor(a).cuda()  # noqa: E731
+        r = losses.policy_loss(put(logp), put(adv), old_logp=put(old), ref_logp=put(ref), kl_coef=0.25, reduction="sum",
+                               cu_seqlens=T.tensor([0, n - 1, n], dtype=T.int32).cuda())
+        seq = LO.sequences(n, [0, n - 1, n])
+        with np.errstate(all="ignore"):
+            _, _, dlogp, _, size, _, _ = LO.policy(logp, adv, seq, 2, np.ones(n, bool), old=old, ref=ref, kl_coef=0.25, reduction="sum")
+            want = np.where(np.abs(dlogp) > 3.4e38, np.sign(dlogp) * np.inf, dlogp)
+        got = host64(r.dlogp)
+        assert np.array_equal(np.isnan(got), np.isnan(want)) and np.isnan(want).sum() == 3 * copies
+        fine = np.isfinite(want)
+        assert np.array_equal(got[~fine & ~np.isnan(want)], want[~fine & ~np.isnan(want)])
+        assert (np.abs(got - want)[fine] <= once(want, size)[fine]).all()
+        # the KL estimate itself: infinite where either exponential or difference is
+        for i, kl in ((3, inf), (9, inf), (13, 0.0), (15, inf)):
+            one = losses.policy_loss(put(logp[i:i + 1]), T.ones(1).cuda(), old_logp=put(old[i:i + 1]), ref_logp=put(ref[i:i + 1]))
+            assert float(one.stats[2]) == (kl if i != 15 else float(np.float32(3e38)))
+
+
 # --- gradients of near-certain targets ---------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("rows,vocab", [(1, 1), (3, 7), (6, 513), (300, 1003), (120, 50257), (2, 151936)])
